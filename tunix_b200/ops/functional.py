@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import math
 import threading
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 import torch.nn.functional as F
@@ -410,3 +410,172 @@ def linear_logprob(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Te
     return lp, ent
   lp, ent = ref.linear_logprob(hidden.reshape(-1, D), weight, targets.reshape(-1), temperature, softcap, want_entropy)
   return lp.view(lead), (ent.view(lead) if ent is not None else None)
+
+
+# ------------------------------------------------------------------------------ alternatives of a row of logits
+class TopLogprobs(NamedTuple):
+  """What `top_logprobs` says of every row of logits."""
+  ids: torch.Tensor                    # int64 [..., k], likeliest first
+  top: torch.Tensor                    # fp32 [..., k], their log-probabilities
+  target: Optional[torch.Tensor]       # fp32 [...], log-probability of the given token
+  entropy: Optional[torch.Tensor]      # fp32 [...]
+
+
+class DistillLoss(NamedTuple):
+  """Per-row terms of `top_distill_loss`."""
+  kl: torch.Tensor                     # fp32 [...]
+  nll: Optional[torch.Tensor]          # fp32 [...]
+
+
+def _grad32(g: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+  return None if g is None else g.float().contiguous()
+
+
+class _TopLogprobsFn(torch.autograd.Function):
+
+  @staticmethod
+  def forward(ctx, x2, k, targets, inv_temp, want_entropy):
+    ids, top, target, ent, stats = kernels.top_logprobs_fwd(x2, k, targets, inv_temp, want_entropy)
+    ctx.save_for_backward(x2, ids, targets, stats, ent)
+    ctx.inv_temp = inv_temp
+    ctx.mark_non_differentiable(ids)
+    ctx.set_materialize_grads(False)
+    return ids, top, target, ent
+
+  @staticmethod
+  @torch.autograd.function.once_differentiable
+  def backward(ctx, _, g_top, g_target, g_ent):
+    x2, ids, targets, stats, ent = ctx.saved_tensors
+    if g_top is None and g_target is None and g_ent is None:
+      return None, None, None, None, None
+    dx = kernels.top_logprobs_bwd(x2, ids, targets, stats, ent, _grad32(g_top), _grad32(g_target), _grad32(g_ent),
+                                  ctx.inv_temp)
+    return dx, None, None, None, None
+
+
+class _TopDistillFn(torch.autograd.Function):
+
+  @staticmethod
+  def forward(ctx, x2, ids, values, labels, inv_temp, full):
+    kl, nll, stats = kernels.top_distill_fwd(x2, ids, values, labels, inv_temp, full)
+    ctx.save_for_backward(x2, ids, values, labels, stats)
+    ctx.cfg = (inv_temp, full)
+    ctx.set_materialize_grads(False)
+    return kl, nll
+
+  @staticmethod
+  @torch.autograd.function.once_differentiable
+  def backward(ctx, g_kl, g_nll):
+    x2, ids, values, labels, stats = ctx.saved_tensors
+    inv_temp, full = ctx.cfg
+    if g_kl is None and g_nll is None:
+      return None, None, None, None, None, None
+    dx = kernels.top_distill_bwd(x2, ids, values, labels, stats, _grad32(g_kl), _grad32(g_nll), inv_temp, full)
+    return dx, None, None, None, None, None
+
+
+def _check_rows(name: str, logits: torch.Tensor, temperature: float, **indexed) -> None:
+  """Arguments that `top_logprobs` and `top_distill_loss` share: floating logits [..., V], a positive temperature,
+  integer tensors on the logits' device."""
+  if logits.dim() < 1 or not logits.is_floating_point():
+    raise ValueError(f"{name}: logits must be a floating tensor [..., V], got {logits.dtype} {tuple(logits.shape)}")
+  if not (temperature > 0 and math.isfinite(temperature)):
+    raise ValueError(f"{name}: temperature must be positive and finite, got {temperature}")
+  for what, (t, shape) in indexed.items():
+    if t is None:
+      continue
+    if t.dtype not in (torch.int32, torch.int64):
+      raise ValueError(f"{name}: {what} must be int32 or int64, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+      raise ValueError(f"{name}: {what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.device != logits.device:
+      raise ValueError(f"{name}: {what} is on {t.device}, the logits on {logits.device}")
+
+
+def _rows(name: str, logits: torch.Tensor) -> Optional[torch.Tensor]:
+  """The logits as the kernels read them ([T, V], unit column stride), or None where the plain statement runs."""
+  if not logits.is_cuda or logits.dtype not in (bf16, torch.float32):
+    return None
+  _lib.require()
+  _lib.bind_thread()
+  if logits.device.index != torch.cuda.current_device():
+    raise ValueError(f"{name}: logits are on {logits.device}, this process drives cuda:{torch.cuda.current_device()}")
+  x2 = logits.reshape(-1, logits.shape[-1])
+  if x2.stride(1) != 1 and x2.shape[1] > 1 or x2.stride(0) < x2.shape[1] and x2.shape[0] > 1:
+    x2 = x2.contiguous()
+  return x2
+
+
+def _ids64(t: Optional[torch.Tensor], *shape) -> Optional[torch.Tensor]:
+  return None if t is None else t.reshape(shape).to(torch.int64).contiguous()
+
+
+def top_logprobs(logits: torch.Tensor, k: int, targets: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                 want_entropy: bool = False) -> TopLogprobs:
+  """The `k` likeliest tokens of every row of logits [..., V] under softmax(logits / temperature), with their
+  log-probabilities, the log-probability of `targets` [...] and the entropy; all differentiable but for the ids.
+
+  Tokens of equal logits come by the lowest id, a NaN counts as the largest logit. A target outside the vocabulary
+  is ignored (0, no gradient). Logits of -inf are masked out; a row that has nothing else gets log-probabilities of
+  -inf, entropy 0 and no gradient. fp32 and bf16 logits on the GPU, rows of any alignment and stride, take one
+  kernel in each direction; there `k` is at most 256."""
+  V = logits.shape[-1] if logits.dim() else 0
+  lead = logits.shape[:-1]
+  _check_rows("top_logprobs", logits, temperature, targets=(targets, lead))
+  k = int(k)
+  if not 1 <= k <= V:
+    raise ValueError(f"top_logprobs: k must be between 1 and the vocabulary's {V}, got {k}")
+  x2 = _rows("top_logprobs", logits)
+  tg = _ids64(targets, -1)
+  if x2 is None:
+    ids, top, target, ent = ref.top_logprobs(logits.reshape(-1, V), k, tg, float(temperature), want_entropy)
+  else:
+    if k > kernels.MAX_TOP_K:
+      raise ValueError(f"top_logprobs: k is at most {kernels.MAX_TOP_K} on the GPU, got {k}")
+    ids, top, target, ent = _TopLogprobsFn.apply(x2, k, tg, 1.0 / float(temperature), bool(want_entropy))
+  return TopLogprobs(ids.view(*lead, k), top.view(*lead, k), None if target is None else target.view(lead),
+                     None if ent is None else ent.view(lead))
+
+
+def top_distill_loss(logits: torch.Tensor, top_ids: torch.Tensor, top_values: torch.Tensor,
+                     labels: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                     normalize: str = "top") -> DistillLoss:
+  """Distillation from a teacher's best tokens: per row of the student's logits [..., V] the divergence from the
+  teacher's list (`top_ids`, `top_values` [..., k]) and, with `labels` [...], the cross entropy at temperature 1.
+
+  normalize="top": both sides are renormalised over the list, KL(softmax(values / T) || softmax(logits[ids] / T));
+    the values may be logits or log-probabilities.
+  normalize="full": the values are log-probabilities t of the teacher over its whole vocabulary at this temperature
+    (`top_logprobs(teacher, k, temperature=T).top`), the student is normalised over its whole vocabulary:
+    sum_i exp(t_i) (t_i - log p_T(ids_i)). What the list leaves out does not count.
+
+  The gradient goes to the logits only. An id outside the vocabulary is an absent entry and a label outside it is
+  ignored; an entry of probability 0 adds nothing. A row without a usable entry (no id left, teacher's values all
+  -inf, student's logits there all -inf) has divergence 0 and no gradient, a row of -inf also no cross entropy.
+  fp32 and bf16 logits on the GPU take one kernel in each direction; there the list has at most 1024 entries."""
+  lead = logits.shape[:-1]
+  V = logits.shape[-1] if logits.dim() else 0
+  k = top_ids.shape[-1] if top_ids.dim() else 0
+  _check_rows("top_distill_loss", logits, temperature, top_ids=(top_ids, (*lead, k)), labels=(labels, lead))
+  if normalize not in ("top", "full"):
+    raise ValueError(f"top_distill_loss: normalize must be 'top' or 'full', got {normalize!r}")
+  if k < 1 or V < 1:
+    raise ValueError(f"top_distill_loss: needs a list of at least one entry and a vocabulary, got k={k}, V={V}")
+  if tuple(top_values.shape) != tuple(top_ids.shape) or not top_values.is_floating_point():
+    raise ValueError(f"top_distill_loss: top_values must be floating and shaped like top_ids {tuple(top_ids.shape)}, "
+                     f"got {top_values.dtype} {tuple(top_values.shape)}")
+  if top_values.device != logits.device:
+    raise ValueError(f"top_distill_loss: top_values is on {top_values.device}, the logits on {logits.device}")
+  if top_values.requires_grad and torch.is_grad_enabled():
+    raise ValueError("top_distill_loss: the teacher's values get no gradient; detach them")
+  x2 = _rows("top_distill_loss", logits)
+  ids, tg = _ids64(top_ids, -1, k), _ids64(labels, -1)
+  full = normalize == "full"
+  if x2 is None:
+    kl, nll = ref.top_distill_loss(logits.reshape(-1, V), ids, top_values.reshape(-1, k), tg, float(temperature), full)
+  else:
+    if k > kernels.MAX_TOP_LIST:
+      raise ValueError(f"top_distill_loss: the list has at most {kernels.MAX_TOP_LIST} entries on the GPU, got {k}")
+    values = top_values.detach().reshape(-1, k).float().contiguous()
+    kl, nll = _TopDistillFn.apply(x2, ids, values, tg, 1.0 / float(temperature), full)
+  return DistillLoss(kl.view(lead), None if nll is None else nll.view(lead))

@@ -248,6 +248,67 @@ def logprob_bwd(logits, targets, lse, entropy, g_logp, g_ent, inv_temp=1.0, soft
   return out
 
 
+MAX_TOP_K = 256           # longest list of alternatives of `top_logprobs_fwd` (csrc/top_logprob.cu: kMaxTop)
+MAX_TOP_LIST = 1024       # longest teacher's list of `top_distill_fwd` (kMaxList)
+
+
+def top_logprobs_fwd(logits: torch.Tensor, k: int, targets: Optional[torch.Tensor], inv_temp: float,
+                     want_entropy: bool):
+  """logits [T, V] fp32/bf16 with unit column stride, targets [T] int64 or None ->
+  (ids int64 [T, k], top [T, k], target [T] or None, entropy [T] or None, stats [T, 2]); fp32 but for the ids."""
+  T, V = logits.shape
+  dev = logits.device
+  f32 = torch.float32
+  ids = torch.empty((T, k), dtype=torch.int64, device=dev)
+  top = torch.empty((T, k), dtype=f32, device=dev)
+  target = torch.empty(T, dtype=f32, device=dev) if targets is not None else None
+  ent = torch.empty(T, dtype=f32, device=dev) if want_entropy else None
+  stats = torch.empty((T, 2), dtype=f32, device=dev)
+  _lib.check_rc(_lib.require().tx_top_logprob_fwd(
+      logits.data_ptr(), int(logits.dtype == f32), logits.stride(0), T, V, k, float(inv_temp), _p(targets),
+      ids.data_ptr(), top.data_ptr(), _p(target), _p(ent), stats.data_ptr(), _lib.stream_ptr()), "tx_top_logprob_fwd")
+  return ids, top, target, ent, stats
+
+
+def top_logprobs_bwd(logits, ids, targets, stats, entropy, g_top, g_target, g_entropy, inv_temp: float) -> torch.Tensor:
+  """Gradient of `top_logprobs_fwd` in the logits' dtype; gradients are fp32 and contiguous, or None."""
+  T, V = logits.shape
+  dx = torch.empty((T, V), dtype=logits.dtype, device=logits.device)
+  _lib.check_rc(_lib.require().tx_top_logprob_bwd(
+      logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0), T, V, ids.shape[1], float(inv_temp),
+      ids.data_ptr(), _p(g_top), _p(targets), _p(g_target), _p(g_entropy), _p(entropy), stats.data_ptr(),
+      dx.data_ptr(), V, _lib.stream_ptr()), "tx_top_logprob_bwd")
+  return dx
+
+
+def top_distill_fwd(logits: torch.Tensor, ids: torch.Tensor, values: torch.Tensor, labels: Optional[torch.Tensor],
+                    inv_temp: float, full: bool):
+  """logits [T, V] fp32/bf16 with unit column stride, ids [T, k] int64 and values [T, k] fp32 contiguous, labels [T]
+  int64 or None -> (kl [T], nll [T] or None, stats [T, 4]), fp32."""
+  T, V = logits.shape
+  dev = logits.device
+  f32 = torch.float32
+  kl = torch.empty(T, dtype=f32, device=dev)
+  nll = torch.empty(T, dtype=f32, device=dev) if labels is not None else None
+  stats = torch.empty((T, 4), dtype=f32, device=dev)
+  _lib.check_rc(_lib.require().tx_top_distill_fwd(
+      logits.data_ptr(), int(logits.dtype == f32), logits.stride(0), T, V, ids.shape[1], float(inv_temp), int(full),
+      ids.data_ptr(), values.data_ptr(), _p(labels), kl.data_ptr(), _p(nll), stats.data_ptr(), _lib.stream_ptr()),
+                "tx_top_distill_fwd")
+  return kl, nll, stats
+
+
+def top_distill_bwd(logits, ids, values, labels, stats, g_kl, g_nll, inv_temp: float, full: bool) -> torch.Tensor:
+  """Gradient of `top_distill_fwd` in the logits' dtype; gradients are fp32 and contiguous, or None."""
+  T, V = logits.shape
+  dx = torch.empty((T, V), dtype=logits.dtype, device=logits.device)
+  _lib.check_rc(_lib.require().tx_top_distill_bwd(
+      logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0), T, V, ids.shape[1], float(inv_temp),
+      int(full), ids.data_ptr(), values.data_ptr(), _p(labels), _p(g_kl), _p(g_nll), stats.data_ptr(), dx.data_ptr(),
+      V, _lib.stream_ptr()), "tx_top_distill_bwd")
+  return dx
+
+
 def rope_table(max_pos: int, head_dim: int, theta: float, device, scale: float = 1.0) -> torch.Tensor:
   """[max_pos, head_dim] fp32 = [cos(H/2) | sin(H/2)], timescale theta^(2i/H)."""
   half = head_dim // 2

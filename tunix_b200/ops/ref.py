@@ -101,3 +101,71 @@ def linear_logprob(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Te
   if softcap > 0:
     logits = torch.tanh(logits / softcap) * softcap
   return selective_log_softmax(logits, targets, temperature, want_entropy)
+
+
+def _masked_log_softmax(z: torch.Tensor, dim: int = -1) -> torch.Tensor:
+  """log_softmax that takes a row of -inf for an empty distribution (all -inf, zero gradient) instead of NaN."""
+  empty = (z == float("-inf")).all(dim, keepdim=True)
+  lp = F.log_softmax(torch.where(empty, torch.zeros_like(z), z), dim)
+  return torch.where(empty, torch.full_like(lp, float("-inf")), lp)
+
+
+def _from_max(x: torch.Tensor) -> torch.Tensor:
+  """Rows relative to their maximum, so that dividing by a temperature cannot overflow; rows of -inf stay as they are."""
+  m = x.detach().amax(-1, keepdim=True)
+  return x - torch.where(m == float("-inf"), torch.zeros_like(m), m)
+
+
+def _wide(x: torch.Tensor) -> torch.Tensor:
+  return x if x.dtype == torch.float64 else x.float()
+
+
+def top_logprobs(logits: torch.Tensor, k: int, targets: Optional[torch.Tensor], temperature: float,
+                 want_entropy: bool):
+  """(ids, top, target, entropy) of `functional.top_logprobs` for logits [T, V]."""
+  x = _wide(logits)
+  V = x.shape[1]
+  lp = _masked_log_softmax(_from_max(x) / temperature)
+  ids = torch.sort(x.detach(), dim=1, descending=True, stable=True).indices[:, :k]
+  top = lp.gather(1, ids)
+  target = entropy = None
+  if targets is not None:
+    known = (targets >= 0) & (targets < V)
+    target = torch.where(known, lp.gather(1, targets.clamp(0, V - 1)[:, None])[:, 0], torch.zeros_like(lp[:, 0]))
+  if want_entropy:
+    p = lp.exp()
+    entropy = -(p * torch.where(p == 0, torch.zeros_like(lp), lp)).sum(1)
+  return ids, top, target, entropy
+
+
+def top_distill_loss(logits: torch.Tensor, ids: torch.Tensor, values: torch.Tensor, labels: Optional[torch.Tensor],
+                     temperature: float, full: bool):
+  """(kl, nll) of `functional.top_distill_loss` for logits [T, V], ids and values [T, k]."""
+  x = _wide(logits)
+  T, V = x.shape
+  low = float("-inf")
+  there = (ids >= 0) & (ids < V)
+  at = ids.clamp(0, V - 1)
+  empty = (x == low).all(1)
+  safe = torch.where(empty[:, None], torch.zeros_like(x), x)     # rows without a finite logit: no loss, no gradient
+  t = _wide(values).detach().to(x.dtype)
+  t = torch.where(there, t, torch.full_like(t, low))
+  if full:
+    lq = t
+    lp = F.log_softmax(_from_max(safe) / temperature, dim=1).gather(1, at)
+    none = empty
+  else:
+    picked = torch.where(there, x.gather(1, at), torch.full_like(t, low))
+    none = (t == low).all(1) | (picked == low).all(1)
+    lq = _masked_log_softmax(_from_max(t) / temperature)
+    lp = _masked_log_softmax(_from_max(torch.where(none[:, None], torch.zeros_like(picked), picked)) / temperature)
+  q = lq.exp()
+  use = (q != 0) & ~none[:, None]
+  zero = torch.zeros_like(q)
+  kl = (torch.where(use, q, zero) * (torch.where(use, lq, zero) - torch.where(use, lp, zero))).sum(1)
+  nll = None
+  if labels is not None:
+    known = (labels >= 0) & (labels < V) & ~empty
+    lp1 = F.log_softmax(safe, dim=1).gather(1, labels.clamp(0, V - 1)[:, None])[:, 0]
+    nll = torch.where(known, -lp1, torch.zeros_like(lp1))
+  return kl, nll
