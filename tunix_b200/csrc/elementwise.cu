@@ -1,5 +1,5 @@
-// Bandwidth-bound kernels: gated activations (SwiGLU / GeGLU), embedding gather and its
-// scatter-add backward, the flat AdamW update with fp32 master weights, fp32 gradient norm
+// Bandwidth-bound kernels: gated activations (SwiGLU / GeGLU), the embedding
+// gather, the flat AdamW update with fp32 master weights, fp32 gradient norm
 // with clipping, and a few cast / scale helpers. 16-byte vector accesses throughout.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -110,25 +110,6 @@ __global__ void embedding_fwd_kernel(const int* __restrict__ ids, const __nv_bfl
       for (int e = 0; e < 8; ++e) v[e] *= scale;
     }
     store8(out + t * D + c, v);
-  }
-}
-
-// grad_table[ids[t], :] += dout[t, :] * scale   (fp32 accumulation with atomics)
-__global__ void embedding_bwd_kernel(const int* __restrict__ ids, const __nv_bfloat16* __restrict__ dout,
-                                     float* __restrict__ grad_table, long long T, int D, int V, float scale) {
-  const int dv = D / 8;
-  const long long total = T * dv;
-  for (long long i = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; i < total;
-       i += static_cast<long long>(gridDim.x) * blockDim.x) {
-    const long long t = i / dv;
-    const int c = static_cast<int>(i - t * dv) * 8;
-    const int id = ids[t];
-    if (id < 0 || id >= V) continue;
-    float v[8];
-    load8(dout + t * D + c, v);
-    float* dst = grad_table + static_cast<long long>(id) * D + c;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) atomicAdd(dst + e, v[e] * scale);
   }
 }
 
@@ -291,15 +272,6 @@ extern "C" int tx_embedding_fwd(const int* ids, const void* table, void* out, lo
   if (T <= 0) return 0;
   embedding_fwd_kernel<<<grid_for(T * (D / 8), 256), 256, 0, s>>>(ids, (const __nv_bfloat16*)table,
                                                                   (__nv_bfloat16*)out, T, D, V, scale);
-  return TX_OK();
-}
-
-extern "C" int tx_embedding_bwd(const int* ids, const void* dout, float* grad_table, long long T, int D, int V,
-                                float scale, cudaStream_t s) {
-  if (D % 8) return 1;
-  if (T <= 0) return 0;
-  embedding_bwd_kernel<<<grid_for(T * (D / 8), 256), 256, 0, s>>>(ids, (const __nv_bfloat16*)dout, grad_table,
-                                                                  T, D, V, scale);
   return TX_OK();
 }
 

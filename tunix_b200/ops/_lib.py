@@ -46,7 +46,7 @@ def _declare(lib):
       "tx_glu_fwd": [P, P, L, I, I, P],
       "tx_glu_bwd": [P, P, P, L, I, I, P],
       "tx_embedding_fwd": [P, P, P, L, I, I, F, P],
-      "tx_embedding_bwd": [P, P, P, L, I, I, F, P],
+      "tx_embedding_grad": [P, I, P, P, I, I, I, I, F, P, P],
       "tx_adamw": [P, P, P, P, P, L, F, F, F, F, F, F, F, P, I, P],
       "tx_sumsq_partials": [],
       "tx_sumsq": [P, L, P, P, I, P],
@@ -94,6 +94,9 @@ def _declare(lib):
       continue
     fn.argtypes = argtypes
     fn.restype = c_int
+  if hasattr(lib, "tx_embedding_grad_workspace"):
+    lib.tx_embedding_grad_workspace.argtypes = [I, I]
+    lib.tx_embedding_grad_workspace.restype = L
   return lib
 
 
@@ -130,8 +133,8 @@ def set_deterministic(flag: bool) -> None:
   """Bitwise-reproducible mode (also `TUNIX_B200_DETERMINISTIC=1`): products whose partial sums would meet through
   floating-point atomics take their single-pass form - no split-K in skinny GEMMs, and tensor-parallel exits
   all-reduce through the collective library instead of the atomic-add epilogue. Flash attention (fixed reduction
-  order), the log-prob kernels, the grouped expert GEMMs and the Philox sampler are reproducible in either mode;
-  the embedding gradient switches from fp32 atomic adds to a sorted accumulation."""
+  order), the log-prob kernels, the embedding gradient (summed by sorted tokens), the grouped expert GEMMs and the
+  Philox sampler are reproducible in either mode."""
   global _DETERMINISTIC
   _DETERMINISTIC = bool(flag)
   lib = load()

@@ -275,18 +275,13 @@ class _EmbeddingFn(torch.autograd.Function):
   def backward(ctx, dout):
     (ids,) = ctx.saved_tensors
     mg = _main_grad(ctx.holder)
-    from . import _lib
-    if _lib.deterministic():
-      # sorted accumulation (index_put_ with accumulate sorts the indices on CUDA) instead of fp32 atomics
-      g = mg if mg is not None else torch.zeros(ctx.shape, dtype=torch.float32, device=dout.device)
-      g.index_put_((ids.long(),), dout.float() * ctx.scale, accumulate=True)
-      return None, (None if mg is not None else g.to(dout.dtype)), None, None
+    dout = dout.contiguous()
     if mg is not None:
-      kernels.embedding_bwd(ids, dout.contiguous(), mg, ctx.scale)
+      kernels.embedding_bwd(ids, dout, mg, ctx.scale)
       return None, None, None, None
-    g = torch.zeros(ctx.shape, dtype=torch.float32, device=dout.device)
-    kernels.embedding_bwd(ids, dout.contiguous(), g, ctx.scale)
-    return None, g.to(dout.dtype), None, None
+    g = torch.zeros(ctx.shape, dtype=dout.dtype, device=dout.device)
+    kernels.embedding_bwd(ids, dout, g, ctx.scale)
+    return None, g, None, None
 
 
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:

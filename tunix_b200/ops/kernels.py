@@ -161,12 +161,23 @@ def embedding_fwd(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) ->
 
 
 def embedding_bwd(ids: torch.Tensor, dout: torch.Tensor, grad_table: torch.Tensor, scale: float = 1.0) -> None:
-  """grad_table (fp32 [V, D]) += scatter of dout rows."""
-  ids32 = ids.reshape(-1).to(torch.int32)
+  """Sums scale * dout [T, D] (bf16) over the positions of every id, in a fixed order. grad_table [V, D] fp32 is added
+  to; a bf16 one (zeroed by the caller) gets the rows that occur. Ids outside the vocabulary are left out."""
+  ids = ids.reshape(-1)
+  if ids.dtype not in (torch.int32, torch.int64):
+    ids = ids.to(torch.int64)
+  ids = ids.contiguous()
+  T = ids.numel()
   V, D = grad_table.shape
-  _lib.check_rc(_lib.require().tx_embedding_bwd(ids32.data_ptr(), dout.data_ptr(), grad_table.data_ptr(),
-                                                ids32.numel(), D, V, float(scale), _lib.stream_ptr()),
-                "tx_embedding_bwd")
+  assert dout.dtype == bf16 and dout.is_contiguous() and dout.numel() == T * D and grad_table.is_contiguous()
+  assert grad_table.dtype in (bf16, torch.float32)
+  if dout.data_ptr() % 16:
+    dout = dout.clone()
+  lib = _lib.require()
+  work = torch.empty(lib.tx_embedding_grad_workspace(T, D), dtype=torch.uint8, device=dout.device)
+  _lib.check_rc(lib.tx_embedding_grad(ids.data_ptr(), int(ids.dtype == torch.int64), dout.data_ptr(),
+                                      grad_table.data_ptr(), int(grad_table.dtype == bf16), T, D, V, float(scale),
+                                      work.data_ptr(), _lib.stream_ptr()), "tx_embedding_grad")
 
 
 def adamw_step(master, m, v, grad, param_bf16, *, lr, beta1, beta2, eps, weight_decay, step: int,
