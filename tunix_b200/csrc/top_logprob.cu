@@ -10,12 +10,15 @@
 // Everything is kept relative to m, so log-probabilities do not lose the bits of a large log-sum-exp, and the
 // running maximum starts at the lowest finite float: a row of -inf sums to 0 instead of to NaN (it is reported as
 // an empty row: ln s is stored as +inf, log-probabilities are -inf, losses and gradients 0).
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <float.h>
 #include <stdint.h>
 
 #include "tx_host.h"
+
+namespace cg = cooperative_groups;
 
 namespace {
 
@@ -25,7 +28,10 @@ constexpr int kVec = 8;                       // elements a thread takes at a ti
 constexpr int kChunk = kThreads * kVec;       // elements the block takes per iteration
 constexpr int kMaxTop = 256;                  // longest list of alternatives
 constexpr int kMaxList = 1024;                // longest teacher's list
-constexpr int kSlots = 8192;                  // candidate slots: the prune limit plus one full iteration, to a power of 2
+constexpr int kSlots = 4096;                  // candidate slots of a block
+constexpr int kPicked = 1024;                 // of which this many may be left for the last sort
+constexpr int kBins = 256;
+constexpr int kMaxSplit = 8;                  // blocks (one cluster) a row is spread over when there are few rows
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -77,15 +83,26 @@ __device__ __forceinline__ int misalign(const T* p) {
   return static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
 }
 
-// Elements j .. j+7 of a row with V columns; those outside are -inf. `aligned`: the address of j is.
+// Elements j .. j+7 of a row; those outside [lo, hi) are -inf. `aligned`: the address of j is.
 template <typename T>
-__device__ __forceinline__ void load8(const T* row, int j, int V, bool aligned, float (&z)[8]) {
-  if (aligned && j >= 0 && j + kVec <= V) {
+__device__ __forceinline__ void load8(const T* row, int j, int lo, int hi, bool aligned, float (&z)[8]) {
+  if (aligned && j >= lo && j + kVec <= hi) {
     vec_load(row + j, z);
   } else {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) z[i] = (j + i >= 0 && j + i < V) ? to_f(row[j + i]) : -INFINITY;
+    for (int i = 0; i < kVec; ++i) z[i] = (j + i >= lo && j + i < hi) ? to_f(row[j + i]) : -INFINITY;
   }
+}
+
+__device__ __forceinline__ float max8(const float (&z)[8]) {
+  return max_nan(max_nan(max_nan(z[0], z[1]), max_nan(z[2], z[3])), max_nan(max_nan(z[4], z[5]), max_nan(z[6], z[7])));
+}
+
+// Columns of a row that block `rank` of `blocks` takes: equal parts, cut at multiples of kVec from the first one.
+__device__ __forceinline__ int2 part_of(int V, int rank, int blocks) {
+  const int vecs = (V + kVec - 1) / kVec;
+  const int per = (vecs + blocks - 1) / blocks * kVec;
+  return make_int2(min(V, rank * per), min(V, rank * per + per));
 }
 
 // ---- softmax statistics --------------------------------------------------------------------------------
@@ -168,15 +185,46 @@ __device__ __forceinline__ int key_index(unsigned long long key) {
   return static_cast<int>(0xffffffffu - static_cast<uint32_t>(key));
 }
 
-// Sorts n keys in shared memory from high to low (bitonic; slots n .. P-1 are filled with 0). All threads call it.
+__device__ __forceinline__ unsigned long long shfl_key(unsigned long long k, int stride) {
+  const uint32_t lo = __shfl_xor_sync(0xffffffffu, static_cast<uint32_t>(k), stride);
+  const uint32_t hi = __shfl_xor_sync(0xffffffffu, static_cast<uint32_t>(k >> 32), stride);
+  return (static_cast<unsigned long long>(hi) << 32) | lo;
+}
+
+// Sorts n keys in shared memory from high to low (bitonic; slots n .. P-1 are filled with 0, P the next power of 2).
+// All threads call it. Up to one key per thread stays in a register and strides below a warp are shuffles.
 __device__ __forceinline__ void sort_keys(unsigned long long* keys, int n) {
-  int P = 2;
+  int P = 32;
   while (P < n) P <<= 1;
-  for (int i = n + threadIdx.x; i < P; i += kThreads) keys[i] = 0;
+  const int tid = threadIdx.x;
+  if (P <= kThreads) {
+    const bool in = (tid & ~31) < P;
+    unsigned long long key = tid < n ? keys[tid] : 0;
+    for (int size = 2; size <= P; size <<= 1) {
+      for (int stride = size >> 1; stride > 0; stride >>= 1) {
+        unsigned long long other = 0;
+        if (stride >= 32) {
+          __syncthreads();
+          if (in) keys[tid] = key;
+          __syncthreads();
+          if (in) other = keys[tid ^ stride];
+        } else if (in) {
+          other = shfl_key(key, stride);
+        }
+        const bool larger = ((tid & stride) == 0) == ((tid & size) == 0);
+        if (larger == (other > key)) key = other;
+      }
+    }
+    __syncthreads();
+    if (in) keys[tid] = key;
+    __syncthreads();
+    return;
+  }
+  for (int i = n + tid; i < P; i += kThreads) keys[i] = 0;
   __syncthreads();
   for (int size = 2; size <= P; size <<= 1) {
     for (int stride = size >> 1; stride > 0; stride >>= 1) {
-      for (int i = threadIdx.x; i < P / 2; i += kThreads) {
+      for (int i = tid; i < P / 2; i += kThreads) {
         const int a = 2 * i - (i & (stride - 1));
         const int b = a + stride;
         const unsigned long long x = keys[a], y = keys[b];
@@ -204,85 +252,240 @@ struct TopArgs {
   float2* stats;               // [T]: m, ln s
 };
 
-// One block per row. A candidate is an element above a running threshold that at least k earlier elements reach:
-// first the smallest over the warps of the ceil(k / warps)-th largest of a warp's per-thread maxima of the first
-// iteration, later the k-th best of all candidates so far, taken whenever their number passes the prune limit.
-template <typename LT, int X>
-__global__ void __launch_bounds__(kThreads) top_fwd_kernel(TopArgs a) {
-  extern __shared__ unsigned long long keys[];
-  __shared__ Stat sh_stat[kWarps];
-  __shared__ float sh_thr[kWarps];
-  __shared__ int sh_count;
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
-  const LT* x = static_cast<const LT*>(a.logits) + static_cast<long long>(row) * a.ld;
-  const float c = a.inv_temp * kLog2e;
-  const int V = a.V, k = a.k;
-  const int limit = max(512, 4 * k);
-  const int shift = misalign(x);
-  if (tid == 0) sh_count = 0;
-  __syncthreads();
-  Stat st = stat_init();
+// Selection state of a block.
+//
+// A candidate is an element that is not below a threshold which k elements of the block's part are known to reach.
+// The first threshold comes from the first iteration: the smallest over the warps of the ceil(k / warps)-th largest of
+// a warp's per-thread maxima (of the warps that have 256 elements). From then on candidates are counted in bins of equal width above it, and every 64
+// candidates the threshold moves up to half a bin below the lowest bin that k of them reach. Bin numbers and that
+// edge are computed with monotone roundings, so an element of such a bin is never below the edge.
+struct Select {
+  unsigned long long keys[kSlots];
+  unsigned long long picked[kPicked];
+  int bins[kBins];
+  int count, n_picked;
+  float thr0, width, thr;
+  float warp_nth[kWarps], warp_max[kWarps];
+  Stat stat[kWarps];
+  Stat part;                   // this block's statistics, read by the cluster's first block
+};
+
+__device__ __forceinline__ int bin_of(float x, float thr0, float inv_width) {
+  return static_cast<int>(fminf((x - thr0) * inv_width, static_cast<float>(kBins - 1)));     // NaN: the last one
+}
+
+// Lowest bin that k counted candidates reach or pass (0 while there are fewer), by one warp.
+__device__ __forceinline__ int cut_bin(const volatile int* bins, int k) {
+  const int lane = threadIdx.x & 31;
+  const int top = kBins - 1 - lane * (kBins / 32);           // lane 0 has the highest bins
+  int n[kBins / 32], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kBins / 32; ++i) {
+    n[i] = bins[top - i];
+    sum += n[i];
+  }
+  int upto = sum;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  const unsigned reach = __ballot_sync(0xffffffffu, upto >= k);
+  if (reach == 0) return 0;
+  const int who = __ffs(reach) - 1;
+  int b = top, seen = upto - sum;
+#pragma unroll
+  for (int i = 0; i < kBins / 32; ++i) {
+    seen += n[i];
+    if (seen < k) b = top - i - 1;
+  }
+  return __shfl_sync(0xffffffffu, b, who);
+}
+
+// The k best of columns [lo, hi) into keys[0 .. k), sorted, for rows whose candidates do not fit: elements come in
+// order of their index, one per thread and iteration, so from the first full set on only larger ones than the k-th
+// can enter.
+template <typename LT>
+__device__ void select_in_order(Select& s, const LT* x, int lo, int hi, int k) {
+  const int limit = kSlots - kThreads;
   float thr = -INFINITY;
-  bool first = true;
-  for (int base = -shift; base < V; base += kChunk) {
-    const int j = base + tid * kVec;
-    const bool active = j < V && j + kVec > 0;
-    float z[8];
-    float vm = -INFINITY;
-    if (active) {
-      load8(x, j, V, true, z);
-      vm = z[0];
-#pragma unroll
-      for (int i = 1; i < kVec; ++i) vm = max_nan(vm, z[i]);
-      stat_push8<X>(st, z, vm, c, 0.f);
-    }
-    if (first) {
-      float v = vm != vm ? INFINITY : vm;
-      for (int size = 2; size <= 32; size <<= 1)
-        for (int stride = size >> 1; stride > 0; stride >>= 1) {
-          const float o = __shfl_xor_sync(0xffffffffu, v, stride);
-          const bool lower = (lane & stride) == 0;
-          v = (lower == ((lane & size) == 0)) ? fmaxf(v, o) : fminf(v, o);
-        }
-      const float nth = __shfl_sync(0xffffffffu, v, (k + kWarps - 1) / kWarps - 1);
-      if (lane == 0) sh_thr[tid >> 5] = nth;
-      __syncthreads();
-      thr = sh_thr[0];
-      for (int w = 1; w < kWarps; ++w) thr = fminf(thr, sh_thr[w]);
-    }
+  bool any = true;                                   // no threshold yet
+  __syncthreads();
+  if (threadIdx.x == 0) s.count = 0;
+  __syncthreads();
+  for (int base = lo; base < hi; base += kThreads) {
+    const int j = base + threadIdx.x;
     int over = 0;
-    if (active && (first ? !(vm < thr) : !(vm <= thr))) {
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        const bool in = j + i >= 0 && j + i < V && (first ? !(z[i] < thr) : !(z[i] <= thr));
-        if (in) {
-          const int pos = atomicAdd(&sh_count, 1);
-          keys[pos] = key_of(z[i], j + i);       // below the limit before this iteration: at most limit + kChunk
-          over |= pos >= limit;
-        }
+    if (j < hi) {
+      const float v = to_f(x[j]);
+      if (any || !(v <= thr)) {
+        const int pos = atomicAdd(&s.count, 1);
+        s.keys[pos] = key_of(v, j);                  // below the limit before this iteration
+        over = pos >= limit - 1;
       }
     }
-    first = false;
-    if (__syncthreads_or(over)) {
-      sort_keys(keys, sh_count);
-      thr = key_value(keys[k - 1]);
+    // the first set is cut at once: it holds every element so far
+    if (__syncthreads_or(over || (any && base + kThreads - lo >= k))) {
+      sort_keys(s.keys, s.count);
+      any = s.count < k;
+      if (!any) thr = key_value(s.keys[k - 1]);
       __syncthreads();
-      if (tid == 0) sh_count = k;
+      if (threadIdx.x == 0) s.count = min(s.count, k);
       __syncthreads();
     }
   }
-  sort_keys(keys, sh_count);
-  st = stat_block<X>(st, sh_stat, c, 0.f);
+  sort_keys(s.keys, s.count);
+}
+
+template <typename LT, int X>
+__global__ void __launch_bounds__(kThreads, 2) top_fwd_kernel(TopArgs a) {
+  extern __shared__ unsigned char shared[];
+  Select& s = *reinterpret_cast<Select*>(shared);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int row = blockIdx.x / blocks, tid = threadIdx.x, lane = tid & 31;
+  const LT* x = static_cast<const LT*>(a.logits) + static_cast<long long>(row) * a.ld;
+  const float c = a.inv_temp * kLog2e;
+  const int k = a.k;
+  const int2 part = part_of(a.V, rank, blocks);
+  const int lo = part.x, hi = part.y;
+  for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0;
+  if (tid == 0) {
+    s.count = 0;
+    s.n_picked = 0;
+  }
+  Stat st = stat_init();
+  // ---- first iteration: the first threshold
+  const int base = lo - misalign(x + lo);
+  float z[8];
+  const int j0 = base + tid * kVec;
+  load8(x, j0, lo, hi, true, z);
+  const float v0 = max8(z);
+  stat_push8<X>(st, z, v0, c, 0.f);
+  float v = v0 != v0 ? INFINITY : v0;
+  for (int size = 2; size <= 32; size <<= 1)
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      const float o = __shfl_xor_sync(0xffffffffu, v, stride);
+      const bool larger = ((lane & stride) == 0) == ((lane & size) == 0);
+      v = larger ? fmaxf(v, o) : fminf(v, o);
+    }
+  // only warps whose 256 elements all lie in the part count; too few of them give no threshold
+  const int whole = min(kWarps, max(0, hi - base) / (32 * kVec));
+  const int nth_of = whole ? (k + whole - 1) / whole : 33;
+  const float nth = __shfl_sync(0xffffffffu, v, min(nth_of, 32) - 1);
+  if (lane == 0) {
+    s.warp_nth[tid >> 5] = nth;
+    s.warp_max[tid >> 5] = v;
+  }
+  __syncthreads();
+  float thr0 = INFINITY, most = s.warp_max[0];
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < whole) thr0 = fminf(thr0, s.warp_nth[w]);
+    most = fmaxf(most, s.warp_max[w]);
+  }
+  if (nth_of > 32) thr0 = -INFINITY;
+  // 64 bins up to the first iteration's maximum; any positive width is correct
+  float width = (most - thr0) * (1.f / 64.f);
+  if (!(width > 1e-30f && width < 1e30f)) width = 1.f;
+  const float inv_width = 1.f / width;
+  if (tid == 0) s.thr = thr0;
+  float thr = thr0;
+  __syncthreads();
+  auto offer = [&](const float (&e)[8], int j, float vm) {
+    bool full = false;
+    if (!(vm < thr)) {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) {
+        if (!(e[i] < thr) && j + i >= lo && j + i < hi) {
+          const int pos = atomicAdd(&s.count, 1);
+          if (pos < kSlots) s.keys[pos] = key_of(e[i], j + i);
+          atomicAdd(&s.bins[bin_of(e[i], thr0, inv_width)], 1);
+          full |= (pos & 63) == 63;
+        }
+      }
+    }
+    if (__any_sync(0xffffffffu, full)) {
+      const int b = cut_bin(s.bins, k);
+      const float t = fmaf(b - 0.5f, width, thr0);
+      if (lane == 0 && b > 0 && t > *const_cast<volatile float*>(&s.thr)) *const_cast<volatile float*>(&s.thr) = t;
+      __syncwarp();
+    }
+  };
+  offer(z, j0, v0);
+  for (int at = base + kChunk; at < hi; at += 2 * kChunk) {
+    const int j = at + tid * kVec;
+    float y[8];
+    load8(x, j, lo, hi, true, z);
+    load8(x, j + kChunk, lo, hi, true, y);
+    const float vz = max8(z), vy = max8(y);
+    stat_push8<X>(st, z, vz, c, 0.f);
+    stat_push8<X>(st, y, vy, c, 0.f);
+    thr = *const_cast<volatile float*>(&s.thr);
+    offer(z, j, vz);
+    offer(y, j + kChunk, vy);
+  }
+  __syncthreads();
+  // ---- the block's k best, sorted
+  const int n = s.count;
+  const int want = min(k, hi - lo);
+  const unsigned long long* best = s.keys;
+  if (n > kSlots) {
+    select_in_order(s, x, lo, hi, k);
+  } else if (n <= 128) {
+    sort_keys(s.keys, n);
+  } else {
+    const int b = cut_bin(s.bins, k);
+    for (int i = tid; i < n; i += kThreads) {
+      const unsigned long long key = s.keys[i];
+      if (bin_of(key_value(key), thr0, inv_width) >= b) {
+        const int pos = atomicAdd(&s.n_picked, 1);
+        if (pos < kPicked) s.picked[pos] = key;
+      }
+    }
+    __syncthreads();
+    if (s.n_picked <= kPicked) {
+      best = s.picked;
+      sort_keys(s.picked, s.n_picked);
+    } else {
+      sort_keys(s.keys, n);
+    }
+  }
+  st = stat_block<X>(st, s.stat, c, 0.f);
+  // ---- over the cluster: the first block collects lists and statistics
+  if (blocks > 1) {
+    if (best != s.picked) {
+      for (int i = tid; i < want; i += kThreads) s.picked[i] = best[i];
+    }
+    if (tid == 0) {
+      s.part = st;
+      s.n_picked = want;
+    }
+    cluster.sync();
+    if (rank == 0) {
+      int at = 0;
+      for (int r = 0; r < blocks; ++r) {
+        const Select* o = cluster.map_shared_rank(&s, r);
+        const int m = o->n_picked;
+        for (int i = tid; i < m; i += kThreads) s.keys[at + i] = o->picked[i];
+        at += m;
+        if (r > 0) stat_merge<X>(st, o->part, c, 0.f);
+      }
+      __syncthreads();
+      sort_keys(s.keys, at);
+      best = s.keys;
+    }
+    cluster.sync();                      // the others' shared memory was read
+    if (rank != 0) return;
+  }
   const float ls = log_sum(st.s);
   for (int i = tid; i < k; i += kThreads) {
-    const unsigned long long key = keys[i];
+    const unsigned long long key = best[i];
     a.ids[static_cast<long long>(row) * k + i] = key_index(key);
     a.top[static_cast<long long>(row) * k + i] = (key_value(key) - st.m) * a.inv_temp - ls;
   }
   if (tid == 0) {
     if (a.target) {
       const long long t = a.targets[row];
-      a.target[row] = (t >= 0 && t < V) ? (to_f(x[t]) - st.m) * a.inv_temp - ls : 0.f;
+      a.target[row] = (t >= 0 && t < a.V) ? (to_f(x[t]) - st.m) * a.inv_temp - ls : 0.f;
     }
     if (a.entropy) a.entropy[row] = st.s == 0.f ? 0.f : ls - a.inv_temp * (st.sd / st.s);
     a.stats[row] = make_float2(st.m, ls);
@@ -345,24 +548,36 @@ __device__ __forceinline__ List list_stats(const LT* x, const long long* ids, co
 // PASSES: how many softmax sums of the row are needed. 0 (only the listed entries matter: one warp per row), 1 (scale
 // c1 in the exponent) or 2 (c1 and c2).
 template <typename LT, int PASSES>
-__global__ void __launch_bounds__(kThreads) distill_fwd_kernel(DistillArgs a, float c1, float c2) {
+__global__ void __launch_bounds__(PASSES ? kThreads : 32) distill_fwd_kernel(DistillArgs a, float c1, float c2) {
   __shared__ Stat sh_stat[kWarps];
-  const int row = blockIdx.x, tid = threadIdx.x;
+  __shared__ Stat sh_part;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = PASSES ? static_cast<int>(cluster.num_blocks()) : 1;
+  const int rank = PASSES ? static_cast<int>(cluster.block_rank()) : 0;
+  const int row = blockIdx.x / blocks, tid = threadIdx.x;
   const LT* x = static_cast<const LT*>(a.logits) + static_cast<long long>(row) * a.ld;
   const int V = a.V, k = a.k;
   Stat st = stat_init();
   constexpr int X = PASSES == 2 ? kSecond : kNone;
   if (PASSES > 0) {
-    for (int j = -misalign(x) + tid * kVec; j < V; j += kChunk) {
-      if (j + kVec <= 0) continue;
-      float z[8];
-      load8(x, j, V, true, z);
-      float vm = z[0];
-#pragma unroll
-      for (int i = 1; i < kVec; ++i) vm = max_nan(vm, z[i]);
-      stat_push8<X>(st, z, vm, c1, c2);
+    const int2 part = part_of(V, rank, blocks);
+    const int lo = part.x, hi = part.y;
+    for (int j = lo - misalign(x + lo) + tid * kVec; j < hi; j += 2 * kChunk) {
+      float z[8], y[8];
+      load8(x, j, lo, hi, true, z);
+      load8(x, j + kChunk, lo, hi, true, y);
+      stat_push8<X>(st, z, max8(z), c1, c2);
+      stat_push8<X>(st, y, max8(y), c1, c2);
     }
     st = stat_block<X>(st, sh_stat, c1, c2);
+    if (blocks > 1) {
+      if (tid == 0) sh_part = st;
+      cluster.sync();
+      if (rank == 0)
+        for (int r = 1; r < blocks; ++r) stat_merge<X>(st, *cluster.map_shared_rank(&sh_part, r), c1, c2);
+      cluster.sync();
+      if (rank != 0) return;
+    }
   }
   if (tid >= 32) return;
   // With one pass both sums are the same number and only the one that is asked for gets used.
@@ -425,6 +640,7 @@ struct BwdArgs {
   int stat_stride, stat_one, stat_temp;
   void* dx;
   long long ldd;
+  int blocks;                  // a row's columns are cut into this many parts
 };
 
 // d_j = A p_j (temperature) + B p_j (temperature 1) - G p_j (log p_j + H), then the listed columns get their own
@@ -434,7 +650,9 @@ __global__ void __launch_bounds__(kThreads) top_bwd_kernel(BwdArgs a) {
   __shared__ int sh_id[kMaxList + 1];
   __shared__ float sh_coef[kMaxList + 1];
   __shared__ float sh_dense[2];
-  const int row = blockIdx.x, tid = threadIdx.x;
+  const int row = blockIdx.x / a.blocks, tid = threadIdx.x;
+  const int2 part = part_of(a.V, blockIdx.x - row * a.blocks, a.blocks);
+  const int lo = part.x, hi = part.y;
   const LT* x = static_cast<const LT*>(a.logits) + static_cast<long long>(row) * a.ld;
   LT* dx = static_cast<LT*>(a.dx) + static_cast<long long>(row) * a.ldd;
   const int V = a.V, k = a.k;
@@ -517,31 +735,30 @@ __global__ void __launch_bounds__(kThreads) top_bwd_kernel(BwdArgs a) {
     if (DENSE & 2) r = fmaf(B, ex2(fmaf(d, kLog2e, -ls12)), r);
     return r;
   };
-  const int shift = misalign(dx);
-  const bool aligned = misalign(x) == shift;
-  for (int j = tid * kVec - shift; j < V; j += kChunk) {
-    if (j + kVec <= 0) continue;
+  const int shift = misalign(dx + lo);
+  const bool aligned = misalign(x + lo) == shift;
+  for (int j = lo - shift + tid * kVec; j < hi; j += kChunk) {
     float z[8];
     if (DENSE) {
-      load8(x, j, V, aligned, z);
+      load8(x, j, lo, hi, aligned, z);
 #pragma unroll
       for (int i = 0; i < kVec; ++i) z[i] = dense(z[i]);
     } else {
 #pragma unroll
       for (int i = 0; i < kVec; ++i) z[i] = 0.f;
     }
-    if (j >= 0 && j + kVec <= V) {
+    if (j >= lo && j + kVec <= hi) {
       vec_store(dx + j, z);
     } else {
 #pragma unroll
       for (int i = 0; i < kVec; ++i)
-        if (j + i >= 0 && j + i < V) from_f(z[i], dx + j + i);
+        if (j + i >= lo && j + i < hi) from_f(z[i], dx + j + i);
     }
   }
   __syncthreads();
   for (int i = tid; i <= k; i += kThreads) {
     const int at = sh_id[i];
-    if (at < 0) continue;
+    if (at < lo || at >= hi) continue;
     float sum = 0.f;
     bool mine = true;
     for (int n = 0; n <= k; ++n) {
@@ -553,26 +770,41 @@ __global__ void __launch_bounds__(kThreads) top_bwd_kernel(BwdArgs a) {
   }
 }
 
-template <auto Kernel>       // one flag per kernel: instantiations share a type
-int opt_in(int bytes) {
-  static txh::DeviceFlag flag;
-  if (flag.cur()) return 0;
-  if (cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return 401;
-  flag.cur() = true;
-  return 0;
+// Blocks per row of a forward pass: one while the rows fill the GPU, else up to kMaxSplit as long as a part is a full
+// iteration of its block.
+int split_of(int T, int V) {
+  int n = 1;
+  while (n < kMaxSplit && 2ll * n * T <= 2ll * txh::sm_count() && V / (2 * n) >= kChunk) n *= 2;
+  return n;
 }
 
-template <typename LT, int X>
-int launch_top(const TopArgs& a, cudaStream_t s) {
-  const int bytes = kSlots * 8;
-  if (const int rc = opt_in<top_fwd_kernel<LT, X>>(bytes)) return rc;
-  top_fwd_kernel<LT, X><<<a.T, kThreads, bytes, s>>>(a);
-  return cudaGetLastError() == cudaSuccess ? 0 : 400;
+template <auto Kernel, typename... Args>       // static flag: one per kernel, instantiations share a type
+int launch_rows(int T, int blocks, int bytes, cudaStream_t s, Args... args) {
+  static txh::DeviceFlag flag;
+  if (bytes > 48 * 1024 && !flag.cur()) {
+    if (cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return 401;
+    flag.cur() = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(T) * blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = blocks;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, Kernel, args...) == cudaSuccess ? 0 : 400;
 }
 
 template <typename LT>
-int launch_bwd(const BwdArgs& a, int dense, cudaStream_t s) {
-#define TX_BWD(D) case D: top_bwd_kernel<LT, D><<<a.T, kThreads, 0, s>>>(a); break
+int launch_bwd(BwdArgs a, int dense, cudaStream_t s) {
+  const int want = 4 * txh::sm_count(), most = (a.V + kChunk - 1) / kChunk;
+  a.blocks = min(most, a.T >= want ? 1 : (want + a.T - 1) / a.T);
+#define TX_BWD(D) case D: top_bwd_kernel<LT, D><<<a.T * a.blocks, kThreads, 0, s>>>(a); break
   switch (dense) {
     TX_BWD(0); TX_BWD(1); TX_BWD(2); TX_BWD(3); TX_BWD(5);
     default: return 2;
@@ -593,8 +825,12 @@ extern "C" int tx_top_logprob_fwd(const void* logits, int logits_fp32, long long
   if (T <= 0) return 0;
   if (V < 1 || k < 1 || k > kMaxTop || k > V || V > 0x7fff0000) return 1;
   const TopArgs a{logits, ld, T, V, k, inv_temp, targets, ids, top, target, entropy, reinterpret_cast<float2*>(stats)};
-  if (logits_fp32) return entropy ? launch_top<float, kEntropy>(a, s) : launch_top<float, kNone>(a, s);
-  return entropy ? launch_top<__nv_bfloat16, kEntropy>(a, s) : launch_top<__nv_bfloat16, kNone>(a, s);
+  const int n = split_of(T, V), bytes = sizeof(Select);
+  if (logits_fp32)
+    return entropy ? launch_rows<top_fwd_kernel<float, kEntropy>>(T, n, bytes, s, a)
+                   : launch_rows<top_fwd_kernel<float, kNone>>(T, n, bytes, s, a);
+  return entropy ? launch_rows<top_fwd_kernel<__nv_bfloat16, kEntropy>>(T, n, bytes, s, a)
+                 : launch_rows<top_fwd_kernel<__nv_bfloat16, kNone>>(T, n, bytes, s, a);
 }
 
 extern "C" int tx_top_distill_fwd(const void* logits, int logits_fp32, long long ld, int T, int V, int k,
@@ -606,10 +842,11 @@ extern "C" int tx_top_distill_fwd(const void* logits, int logits_fp32, long long
   const float c = inv_temp * kLog2e;
   const int passes = (nll ? 1 : 0) + (full ? 1 : 0) - (nll && full && inv_temp == 1.f ? 1 : 0);
   const float c1 = nll ? kLog2e : c;
-#define TX_FWD(LT)                                                                 \
-  if (passes == 0) distill_fwd_kernel<LT, 0><<<T, 32, 0, s>>>(a, c1, c);           \
-  else if (passes == 1) distill_fwd_kernel<LT, 1><<<T, kThreads, 0, s>>>(a, c1, c); \
-  else distill_fwd_kernel<LT, 2><<<T, kThreads, 0, s>>>(a, c1, c)
+  const int n = split_of(T, V);
+#define TX_FWD(LT)                                                                          \
+  if (passes == 1) return launch_rows<distill_fwd_kernel<LT, 1>>(T, n, 0, s, a, c1, c);      \
+  if (passes == 2) return launch_rows<distill_fwd_kernel<LT, 2>>(T, n, 0, s, a, c1, c);      \
+  distill_fwd_kernel<LT, 0><<<T, 32, 0, s>>>(a, c1, c)
   if (logits_fp32) { TX_FWD(float); } else { TX_FWD(__nv_bfloat16); }
 #undef TX_FWD
   return cudaGetLastError() == cudaSuccess ? 0 : 400;
@@ -623,7 +860,7 @@ extern "C" int tx_top_logprob_bwd(const void* logits, int logits_fp32, long long
   if (T <= 0) return 0;
   if (V < 1 || k < 1 || k > kMaxTop || V > 0x7fff0000) return 1;
   const BwdArgs a{logits, ld, T, V, k, kScore, inv_temp, ids, g_top, targets, nullptr, g_target, g_entropy, entropy,
-                  stats, 2, 1, 1, dx, ldd};
+                  stats, 2, 1, 1, dx, ldd, 1};
   const int dense = g_entropy ? 5 : 1;
   return logits_fp32 ? launch_bwd<float>(a, dense, s) : launch_bwd<__nv_bfloat16>(a, dense, s);
 }
@@ -636,7 +873,7 @@ extern "C" int tx_top_distill_bwd(const void* logits, int logits_fp32, long long
   if (T <= 0) return 0;
   if (V < 1 || k < 1 || k > kMaxList || V > 0x7fff0000) return 1;
   const BwdArgs a{logits, ld, T, V, k, full ? kFull : kListed, inv_temp, ids, values, labels, g_kl, g_nll, nullptr,
-                  nullptr, stats, 4, 1, 2, dx, ldd};
+                  nullptr, stats, 4, 1, 2, dx, ldd, 1};
   const int dense = (full && g_kl ? 1 : 0) | (g_nll ? 2 : 0);
   return logits_fp32 ? launch_bwd<float>(a, dense, s) : launch_bwd<__nv_bfloat16>(a, dense, s);
 }

@@ -154,8 +154,8 @@ def require():
 _HOME_DEVICE = None    # one process drives one GPU: the device current when the first kernel is launched
 
 
-def bind_thread() -> None:
-  """Makes this host thread use the process's GPU.
+def bind_thread() -> int:
+  """Makes this host thread use the process's GPU and returns its index.
 
   The CUDA current device is per thread and starts at 0, so a helper thread of rank r (a rollout
   producer, an asyncio loop) would otherwise launch on GPU 0 with pointers that live on GPU r."""
@@ -165,11 +165,12 @@ def bind_thread() -> None:
     _HOME_DEVICE = cur
   elif cur != _HOME_DEVICE:
     torch.cuda.set_device(_HOME_DEVICE)
+  return _HOME_DEVICE
 
 
 def stream_ptr() -> int:
-  bind_thread()
-  return torch.cuda.current_stream().cuda_stream
+  # the handle alone: building a Stream object costs more than a kernel launch
+  return torch._C._cuda_getCurrentRawStream(bind_thread())
 
 
 _status = {}

@@ -266,9 +266,9 @@ def glu(gu: torch.Tensor, kind: str = "silu") -> torch.Tensor:
 class _EmbeddingFn(torch.autograd.Function):
 
   @staticmethod
-  def forward(ctx, ids, table, scale, holder):
+  def forward(ctx, ids, table, scale):
     ctx.save_for_backward(ids)
-    ctx.scale, ctx.holder, ctx.shape = scale, holder, table.shape
+    ctx.scale, ctx.holder, ctx.shape = scale, table, table.shape
     return kernels.embedding_fwd(ids, table, scale)
 
   @staticmethod
@@ -278,16 +278,19 @@ class _EmbeddingFn(torch.autograd.Function):
     dout = dout.contiguous()
     if mg is not None:
       kernels.embedding_bwd(ids, dout, mg, ctx.scale)
-      return None, None, None, None
+      return None, None, None
     g = torch.zeros(ctx.shape, dtype=dout.dtype, device=dout.device)
     kernels.embedding_bwd(ids, dout, g, ctx.scale)
-    return None, g, None, None
+    return None, g, None
 
 
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+  """Rows of `table` [V, D] times `scale`. The table's gradient is summed by sorted tokens: repeatable to the bit,
+  fp32 sums rounded once, straight into `main_grad` where the table has one."""
   if _use_kernels(table) and table.shape[1] % 8 == 0:
-    out = _EmbeddingFn.apply(ids.reshape(-1), table, scale, table)
-    return out.view(*ids.shape, table.shape[1])
+    flat = ids if ids.dim() == 1 else ids.reshape(-1)
+    out = _EmbeddingFn.apply(flat, table, scale)
+    return out if ids.dim() == 1 else out.view(*ids.shape, table.shape[1])
   return ref.embedding(ids, table, scale)
 
 
@@ -423,7 +426,9 @@ class DistillLoss(NamedTuple):
 
 
 def _grad32(g: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-  return None if g is None else g.float().contiguous()
+  if g is None or (g.dtype == torch.float32 and g.is_contiguous()):
+    return g
+  return g.float().contiguous()
 
 
 class _TopLogprobsFn(torch.autograd.Function):
@@ -492,17 +497,23 @@ def _rows(name: str, logits: torch.Tensor) -> Optional[torch.Tensor]:
   if not logits.is_cuda or logits.dtype not in (bf16, torch.float32):
     return None
   _lib.require()
-  _lib.bind_thread()
-  if logits.device.index != torch.cuda.current_device():
-    raise ValueError(f"{name}: logits are on {logits.device}, this process drives cuda:{torch.cuda.current_device()}")
-  x2 = logits.reshape(-1, logits.shape[-1])
+  home = _lib.bind_thread()
+  if logits.get_device() != home:
+    raise ValueError(f"{name}: logits are on {logits.device}, this process drives cuda:{home}")
+  x2 = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])     # a view is a node of the graph
   if x2.stride(1) != 1 and x2.shape[1] > 1 or x2.stride(0) < x2.shape[1] and x2.shape[0] > 1:
     x2 = x2.contiguous()
   return x2
 
 
 def _ids64(t: Optional[torch.Tensor], *shape) -> Optional[torch.Tensor]:
-  return None if t is None else t.reshape(shape).to(torch.int64).contiguous()
+  if t is None or (t.dtype == torch.int64 and t.dim() == len(shape) and t.is_contiguous()):
+    return t
+  return t.reshape(shape).to(torch.int64).contiguous()
+
+
+def _lead(t: Optional[torch.Tensor], *shape) -> Optional[torch.Tensor]:
+  return t if t is None or t.dim() == len(shape) else t.view(shape)
 
 
 def top_logprobs(logits: torch.Tensor, k: int, targets: Optional[torch.Tensor] = None, temperature: float = 1.0,
@@ -528,8 +539,7 @@ def top_logprobs(logits: torch.Tensor, k: int, targets: Optional[torch.Tensor] =
     if k > kernels.MAX_TOP_K:
       raise ValueError(f"top_logprobs: k is at most {kernels.MAX_TOP_K} on the GPU, got {k}")
     ids, top, target, ent = _TopLogprobsFn.apply(x2, k, tg, 1.0 / float(temperature), bool(want_entropy))
-  return TopLogprobs(ids.view(*lead, k), top.view(*lead, k), None if target is None else target.view(lead),
-                     None if ent is None else ent.view(lead))
+  return TopLogprobs(_lead(ids, *lead, k), _lead(top, *lead, k), _lead(target, *lead), _lead(ent, *lead))
 
 
 def top_distill_loss(logits: torch.Tensor, top_ids: torch.Tensor, top_values: torch.Tensor,
@@ -573,4 +583,4 @@ def top_distill_loss(logits: torch.Tensor, top_ids: torch.Tensor, top_values: to
       raise ValueError(f"top_distill_loss: the list has at most {kernels.MAX_TOP_LIST} entries on the GPU, got {k}")
     values = top_values.detach().reshape(-1, k).float().contiguous()
     kl, nll = _TopDistillFn.apply(x2, ids, values, tg, 1.0 / float(temperature), full)
-  return DistillLoss(kl.view(lead), None if nll is None else nll.view(lead))
+  return DistillLoss(_lead(kl, *lead), _lead(nll, *lead))
