@@ -22,17 +22,18 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kVec = 8;                       // elements a thread takes at a time
-constexpr int kChunk = kThreads * kVec;       // elements the block takes per iteration
+constexpr int kUnroll = 4;                    // 16-byte vectors a thread has in flight
 constexpr int kMaxTop = 256;                  // longest list of alternatives
 constexpr int kMaxList = 1024;                // longest teacher's list
-constexpr int kSlots = 4096;                  // candidate slots of a block
-constexpr int kPicked = 1024;                 // of which this many may be left for the last sort
+constexpr int kCand = 2048;                   // candidate vectors of a block
+constexpr int kKeys = 2048;                   // candidate elements; a cluster's lists fit: kMaxSplit * kMaxTop
 constexpr int kBins = 256;
 constexpr int kMaxSplit = 8;                  // blocks (one cluster) a row is spread over when there are few rows
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kMinPart = 4096;                // columns of such a part at least
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kFloor = -1e37f;              // lowest running maximum
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -45,19 +46,55 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
   return y;
 }
+__device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t y;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+  return y;
+}
+
+// Two floats in one 64-bit register: half the instructions of the scalar forms.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ void from_f(float v, float* p) { *p = v; }
 __device__ __forceinline__ void from_f(float v, __nv_bfloat16* p) { *p = __float2bfloat16_rn(v); }
 
-// Eight consecutive elements from a 16-byte aligned address.
-__device__ __forceinline__ void vec_load(const float* p, float (&z)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  z[0] = a.x; z[1] = a.y; z[2] = a.z; z[3] = a.w; z[4] = b.x; z[5] = b.y; z[6] = b.z; z[7] = b.w;
+// ---- 16-byte vectors of a row ---------------------------------------------------------------------------
+template <typename T>
+constexpr int kVec = 16 / static_cast<int>(sizeof(T));
+template <typename T>
+constexpr int kChunk = kThreads * kVec<T>;    // elements the block takes with one vector per thread
+
+__device__ __forceinline__ void unpack(uint4 u, float (&z)[4]) {
+  z[0] = __uint_as_float(u.x); z[1] = __uint_as_float(u.y); z[2] = __uint_as_float(u.z); z[3] = __uint_as_float(u.w);
 }
-__device__ __forceinline__ void vec_load(const __nv_bfloat16* p, float (&z)[8]) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ void unpack(uint4 u, float (&z)[8]) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -65,16 +102,26 @@ __device__ __forceinline__ void vec_load(const __nv_bfloat16* p, float (&z)[8]) 
     z[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
 }
-__device__ __forceinline__ void vec_store(float* p, const float (&z)[8]) {
-  *reinterpret_cast<float4*>(p) = make_float4(z[0], z[1], z[2], z[3]);
-  *reinterpret_cast<float4*>(p + 4) = make_float4(z[4], z[5], z[6], z[7]);
+__device__ __forceinline__ uint4 pack(const float (&z)[4]) {
+  return make_uint4(__float_as_uint(z[0]), __float_as_uint(z[1]), __float_as_uint(z[2]), __float_as_uint(z[3]));
 }
-__device__ __forceinline__ void vec_store(__nv_bfloat16* p, const float (&z)[8]) {
+__device__ __forceinline__ uint4 pack(const float (&z)[8]) {
   uint4 u;
   __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
 #pragma unroll
   for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(z[2 * i], z[2 * i + 1]);
-  *reinterpret_cast<uint4*>(p) = u;
+  return u;
+}
+template <typename T>
+__device__ __forceinline__ float vec_max(uint4 u);
+template <>
+__device__ __forceinline__ float vec_max<float>(uint4 u) {
+  return max_nan(max_nan(__uint_as_float(u.x), __uint_as_float(u.y)), max_nan(__uint_as_float(u.z), __uint_as_float(u.w)));
+}
+template <>
+__device__ __forceinline__ float vec_max<__nv_bfloat16>(uint4 u) {
+  const uint32_t m = max_nan_bf16x2(max_nan_bf16x2(u.x, u.y), max_nan_bf16x2(u.z, u.w));
+  return max_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
 }
 
 // How many elements an address lies behind the last 16-byte boundary.
@@ -83,69 +130,105 @@ __device__ __forceinline__ int misalign(const T* p) {
   return static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
 }
 
-// Elements j .. j+7 of a row; those outside [lo, hi) are -inf. `aligned`: the address of j is.
+// The vector that begins at element j of a row; elements outside [lo, hi) are -inf. `aligned`: the address of j is.
 template <typename T>
-__device__ __forceinline__ void load8(const T* row, int j, int lo, int hi, bool aligned, float (&z)[8]) {
-  if (aligned && j >= lo && j + kVec <= hi) {
-    vec_load(row + j, z);
-  } else {
+__device__ __forceinline__ uint4 load_vec(const T* row, int j, int lo, int hi, bool aligned) {
+  if (aligned && j >= lo && j + kVec<T> <= hi) return *reinterpret_cast<const uint4*>(row + j);
+  float z[kVec<T>];
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) z[i] = (j + i >= lo && j + i < hi) ? to_f(row[j + i]) : -INFINITY;
-  }
+  for (int i = 0; i < kVec<T>; ++i) z[i] = (j + i >= lo && j + i < hi) ? to_f(row[j + i]) : -INFINITY;
+  return pack(z);
 }
 
-__device__ __forceinline__ float max8(const float (&z)[8]) {
-  return max_nan(max_nan(max_nan(z[0], z[1]), max_nan(z[2], z[3])), max_nan(max_nan(z[4], z[5]), max_nan(z[6], z[7])));
-}
-
-// Columns of a row that block `rank` of `blocks` takes: equal parts, cut at multiples of kVec from the first one.
+// Columns of a row that block `rank` of `blocks` takes: equal parts, cut at multiples of 8 from the first one.
 __device__ __forceinline__ int2 part_of(int V, int rank, int blocks) {
-  const int vecs = (V + kVec - 1) / kVec;
-  const int per = (vecs + blocks - 1) / blocks * kVec;
+  const int vecs = (V + 7) / 8;
+  const int per = (vecs + blocks - 1) / blocks * 8;
   return make_int2(min(V, rank * per), min(V, rank * per + per));
 }
 
 // ---- softmax statistics --------------------------------------------------------------------------------
-struct Stat {
-  float m;    // running maximum, never below the lowest finite float
-  float s;    // sum 2^(d c)
-  float sd;   // sum 2^(d c) d, for the entropy; or the sum at a second temperature
-};
-
+// A thread sums 2^(x c - M) with M = m c rounded: one packed multiply-add per two elements. The rounding of M is the
+// same in every term and is taken back from the logarithm at the end. Where m c leaves fp32, or every element lies
+// below the floor of the running maximum, the sum comes out as 0 or NaN and the row is summed again the careful way.
 constexpr int kNone = 0, kEntropy = 1, kSecond = 2;
 
-__device__ __forceinline__ Stat stat_init() { return Stat{-FLT_MAX, 0.f, 0.f}; }
+struct Stat {
+  float m;    // maximum
+  float s;    // sum 2^(x c - M)
+  float t;    // kEntropy: sum 2^(x c - M) (x c - M); kSecond: the sum at the scale c2
+};
+
+__device__ __forceinline__ float scaled_max(float m, float c) { return fmaxf(m * c, -FLT_MAX); }
 
 template <int X>
-__device__ __forceinline__ void stat_rescale(Stat& a, float m, float c, float c2) {
-  const float d = a.m - m;
-  const float e = ex2(d * c);
-  if (X == kEntropy) a.sd = e == 0.f ? 0.f : e * (a.sd + a.s * d);
-  if (X == kSecond) a.sd *= ex2(d * c2);
+struct Acc {
+  float m, M, M2;
+  f32x2 s, t;
+
+  __device__ __forceinline__ void init(float first, float c, float c2) {
+    m = fmaxf(first, kFloor);
+    M = scaled_max(m, c);
+    if (X == kSecond) M2 = scaled_max(m, c2);
+    s = t = 0;
+  }
+  __device__ __forceinline__ void raise(float v, float c, float c2) {
+    const float n = scaled_max(v, c), d = M - n, e = ex2(d);
+    const f32x2 ee = pack2(e, e);
+    if (X == kEntropy) t = e == 0.f ? 0 : mul2(fma2(s, pack2(d, d), t), ee);
+    if (X == kSecond) {
+      const float n2 = scaled_max(v, c2), e2 = ex2(M2 - n2);
+      t = mul2(t, pack2(e2, e2));
+      M2 = n2;
+    }
+    s = mul2(s, ee);
+    m = v;
+    M = n;
+  }
+  template <typename LT>
+  __device__ __forceinline__ void push(uint4 u, float vm, float c, float c2) {
+    if (vm > m) raise(vm, c, c2);
+    float z[kVec<LT>];
+    unpack(u, z);
+    const f32x2 cc = pack2(c, c), mm = pack2(-M, -M);
+    const f32x2 cc2 = pack2(c2, c2), mm2 = pack2(-M2, -M2);
+#pragma unroll
+    for (int i = 0; i < kVec<LT>; i += 2) {
+      const f32x2 zz = pack2(z[i], z[i + 1]);
+      const float2 g = unpack2(fma2(zz, cc, mm));
+      const f32x2 w = pack2(ex2(g.x), ex2(g.y));
+      s = add2(s, w);
+      if (X == kEntropy) t = fma2(w, pack2(fmaxf(g.x, -1e30f), fmaxf(g.y, -1e30f)), t);     // 0 * -inf would be NaN
+      if (X == kSecond) {
+        const float2 h = unpack2(fma2(zz, cc2, mm2));
+        t = add2(t, pack2(ex2(h.x), ex2(h.y)));
+      }
+    }
+  }
+  __device__ __forceinline__ Stat stat() const {
+    const float2 a = unpack2(s), b = unpack2(t);
+    return Stat{m, a.x + a.y, b.x + b.y};
+  }
+};
+
+template <int X>
+__device__ __forceinline__ void stat_raise(Stat& a, float m, float c, float c2) {
+  const float d = scaled_max(a.m, c) - scaled_max(m, c), e = ex2(d);
+  if (X == kEntropy) a.t = e == 0.f ? 0.f : e * fmaf(a.s, d, a.t);
+  if (X == kSecond) a.t *= ex2(scaled_max(a.m, c2) - scaled_max(m, c2));
   a.s *= e;
   a.m = m;
 }
 
 template <int X>
-__device__ __forceinline__ void stat_push8(Stat& a, const float (&z)[8], float vm, float c, float c2) {
-  if (vm > a.m) stat_rescale<X>(a, vm, c, c2);
-#pragma unroll
-  for (int i = 0; i < kVec; ++i) {
-    const float d = z[i] - a.m;
-    const float w = ex2(d * c);
-    a.s += w;
-    if (X == kEntropy) a.sd = fmaf(w, fmaxf(d, -FLT_MAX), a.sd);     // 0 * -inf would be NaN
-    if (X == kSecond) a.sd += ex2(d * c2);
-  }
-}
-
-template <int X>
 __device__ __forceinline__ void stat_merge(Stat& a, Stat b, float c, float c2) {
-  const float m = fmaxf(a.m, b.m);
-  stat_rescale<X>(a, m, c, c2);
-  stat_rescale<X>(b, m, c, c2);
+  if (a.m != b.m) {
+    const float m = fmaxf(a.m, b.m);
+    stat_raise<X>(a, m, c, c2);
+    stat_raise<X>(b, m, c, c2);
+  }
   a.s += b.s;
-  a.sd += b.sd;
+  a.t += b.t;
 }
 
 // Leaves the block's statistics in every thread. `sh` holds kWarps entries.
@@ -156,7 +239,7 @@ __device__ __forceinline__ Stat stat_block(Stat a, Stat* sh, float c, float c2) 
     Stat b;
     b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
     b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-    b.sd = __shfl_xor_sync(0xffffffffu, a.sd, o);
+    b.t = __shfl_xor_sync(0xffffffffu, a.t, o);
     stat_merge<X>(a, b, c, c2);
   }
   __syncthreads();
@@ -167,8 +250,85 @@ __device__ __forceinline__ Stat stat_block(Stat a, Stat* sh, float c, float c2) 
   return a;
 }
 
-// ln s, or +inf for a row without a finite logit.
+// What a row's softmax comes to. ls = +inf marks a row without an element above -inf.
+struct Row {
+  float m, ls;      // maximum, ln sum exp((x - m) at the scale)
+  float x;          // kEntropy: the entropy; kSecond: ln of the sum at the scale c2
+};
+
 __device__ __forceinline__ float log_sum(float s) { return s == 0.f ? INFINITY : logf(s); }
+
+// Row statistics from differences to the true maximum, by the whole block over the whole row.
+template <typename LT, int X>
+__device__ __noinline__ Row careful_row(const LT* x, int V, Stat* sh, float c, float c2) {
+  float m = -INFINITY;
+  for (int j = threadIdx.x; j < V; j += kThreads) m = fmaxf(m, to_f(x[j]));
+  Stat a{m, 0.f, 0.f};
+  __syncthreads();
+  for (int o = 16; o > 0; o >>= 1) a.m = fmaxf(a.m, __shfl_xor_sync(0xffffffffu, a.m, o));
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = a;
+  __syncthreads();
+  m = -FLT_MAX;
+  for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sh[w].m);
+  float s = 0.f, t = 0.f;
+  for (int j = threadIdx.x; j < V; j += kThreads) {
+    const float d = to_f(x[j]) - m, w = ex2(d * c);
+    s += w;
+    if (X == kEntropy) t = fmaf(w, fmaxf(d * c, -1e30f), t);
+    if (X == kSecond) t += ex2(d * c2);
+  }
+  for (int o = 16; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    t += __shfl_xor_sync(0xffffffffu, t, o);
+  }
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = Stat{m, s, t};
+  __syncthreads();
+  s = t = 0.f;
+  for (int w = 0; w < kWarps; ++w) {
+    s += sh[w].s;
+    t += sh[w].t;
+  }
+  Row r{m, log_sum(s), 0.f};
+  if (X == kEntropy) r.x = s == 0.f ? 0.f : r.ls - kLn2 * (t / s);
+  if (X == kSecond) r.x = log_sum(t);
+  return r;
+}
+
+// All threads of the block call it with the row's statistics.
+template <typename LT, int X>
+__device__ __forceinline__ Row finish_row(const Stat& a, const LT* x, int V, Stat* sh, float c, float c2) {
+  if (!(a.s > 0.f && a.s < INFINITY && (X != kSecond || (a.t > 0.f && a.t < INFINITY))))
+    return careful_row<LT, X>(x, V, sh, c, c2);
+  Row r;
+  r.m = a.m;
+  const float ln = logf(a.s);
+  r.ls = fmaf(-kLn2, fmaf(a.m, c, -scaled_max(a.m, c)), ln);          // M - m c, exactly
+  r.x = 0.f;
+  if (X == kEntropy) r.x = ln - kLn2 * (a.t / a.s);
+  if (X == kSecond) r.x = fmaf(-kLn2, fmaf(a.m, c2, -scaled_max(a.m, c2)), logf(a.t));
+  return r;
+}
+
+// All 16-byte vectors of columns [lo, hi), kUnroll per thread at a time: fn(first element, vectors).
+template <typename LT, typename Fn>
+__device__ __forceinline__ void each_vec(const LT* x, int from, int lo, int hi, Fn fn) {
+  constexpr int step = kUnroll * kChunk<LT>;
+  int at = from;
+  uint4 u[kUnroll];
+  for (; at >= lo && at + step <= hi; at += step) {
+    const int j = at + threadIdx.x * kVec<LT>;
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) u[i] = *reinterpret_cast<const uint4*>(x + j + i * kChunk<LT>);
+    fn(j, u);
+  }
+  for (; at < hi; at += step) {
+    const int j = at + threadIdx.x * kVec<LT>;
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) u[i] = load_vec(x, j + i * kChunk<LT>, lo, hi, true);
+    fn(j, u);
+  }
+}
 
 // ---- keys of candidates --------------------------------------------------------------------------------
 // 64 bits that order by value from high to low (NaN highest, -0 equal to 0), equal values by the lowest index.
@@ -254,17 +414,19 @@ struct TopArgs {
 
 // Selection state of a block.
 //
-// A candidate is an element that is not below a threshold which k elements of the block's part are known to reach.
-// The first threshold comes from the first iteration: the smallest over the warps of the ceil(k / warps)-th largest of
-// a warp's per-thread maxima (of the warps that have 256 elements). From then on candidates are counted in bins of equal width above it, and every 64
-// candidates the threshold moves up to half a bin below the lowest bin that k of them reach. Bin numbers and that
-// edge are computed with monotone roundings, so an element of such a bin is never below the edge.
+// A candidate is a 16-byte vector whose largest element is not below a threshold that k elements of the block's part
+// are known to reach. The first threshold comes from the first iteration: the smallest over the warps of the
+// ceil(k / warps)-th largest of a warp's per-thread maxima (of the warps that have a whole vector per thread). From
+// then on the maxima of candidates are counted in bins of equal width above it, and every 32 candidates the threshold
+// moves up to half a bin below the lowest bin that k of them reach. Bin numbers and that edge are computed with
+// monotone roundings, so an element of such a bin is never below the edge. At the end the candidates are read again
+// (from L2) and their elements that reach the last threshold are sorted: little more than k.
 struct Select {
-  unsigned long long keys[kSlots];
-  unsigned long long picked[kPicked];
+  unsigned long long keys[kKeys];
+  int cand[kCand];
   int bins[kBins];
-  int count, n_picked;
-  float thr0, width, thr;
+  int count, n_keys;
+  float thr;
   float warp_nth[kWarps], warp_max[kWarps];
   Stat stat[kWarps];
   Stat part;                   // this block's statistics, read by the cluster's first block
@@ -301,16 +463,16 @@ __device__ __forceinline__ int cut_bin(const volatile int* bins, int k) {
   return __shfl_sync(0xffffffffu, b, who);
 }
 
-// The k best of columns [lo, hi) into keys[0 .. k), sorted, for rows whose candidates do not fit: elements come in
-// order of their index, one per thread and iteration, so from the first full set on only larger ones than the k-th
-// can enter.
+// The k best of columns [lo, hi) into keys[0 .. k), sorted, for rows whose candidates do not fit (many equal or masked
+// elements): elements come in order of their index, one per thread and iteration, so from the first full set on only
+// larger ones than the k-th can enter.
 template <typename LT>
-__device__ void select_in_order(Select& s, const LT* x, int lo, int hi, int k) {
-  const int limit = kSlots - kThreads;
+__device__ __noinline__ void select_in_order(Select& s, const LT* x, int lo, int hi, int k) {
+  constexpr int limit = kKeys - kThreads;
   float thr = -INFINITY;
   bool any = true;                                   // no threshold yet
   __syncthreads();
-  if (threadIdx.x == 0) s.count = 0;
+  if (threadIdx.x == 0) s.n_keys = 0;
   __syncthreads();
   for (int base = lo; base < hi; base += kThreads) {
     const int j = base + threadIdx.x;
@@ -318,26 +480,26 @@ __device__ void select_in_order(Select& s, const LT* x, int lo, int hi, int k) {
     if (j < hi) {
       const float v = to_f(x[j]);
       if (any || !(v <= thr)) {
-        const int pos = atomicAdd(&s.count, 1);
+        const int pos = atomicAdd(&s.n_keys, 1);
         s.keys[pos] = key_of(v, j);                  // below the limit before this iteration
         over = pos >= limit - 1;
       }
     }
-    // the first set is cut at once: it holds every element so far
+    // the first full set is cut at once: it holds every element so far
     if (__syncthreads_or(over || (any && base + kThreads - lo >= k))) {
-      sort_keys(s.keys, s.count);
-      any = s.count < k;
+      sort_keys(s.keys, s.n_keys);
+      any = s.n_keys < k;
       if (!any) thr = key_value(s.keys[k - 1]);
       __syncthreads();
-      if (threadIdx.x == 0) s.count = min(s.count, k);
+      if (threadIdx.x == 0) s.n_keys = min(s.n_keys, k);
       __syncthreads();
     }
   }
-  sort_keys(s.keys, s.count);
+  sort_keys(s.keys, s.n_keys);
 }
 
 template <typename LT, int X>
-__global__ void __launch_bounds__(kThreads, 2) top_fwd_kernel(TopArgs a) {
+__global__ void __launch_bounds__(kThreads) top_fwd_kernel(TopArgs a) {
   extern __shared__ unsigned char shared[];
   Select& s = *reinterpret_cast<Select*>(shared);
   cg::cluster_group cluster = cg::this_cluster();
@@ -348,34 +510,39 @@ __global__ void __launch_bounds__(kThreads, 2) top_fwd_kernel(TopArgs a) {
   const int k = a.k;
   const int2 part = part_of(a.V, rank, blocks);
   const int lo = part.x, hi = part.y;
+  constexpr int N = kVec<LT>, chunk = kChunk<LT>;
   for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0;
-  if (tid == 0) {
-    s.count = 0;
-    s.n_picked = 0;
-  }
-  Stat st = stat_init();
+  if (tid == 0) s.count = s.n_keys = 0;
   // ---- first iteration: the first threshold
   const int base = lo - misalign(x + lo);
-  float z[8];
-  const int j0 = base + tid * kVec;
-  load8(x, j0, lo, hi, true, z);
-  const float v0 = max8(z);
-  stat_push8<X>(st, z, v0, c, 0.f);
-  float v = v0 != v0 ? INFINITY : v0;
+  const int j0 = base + tid * N;
+  Acc<X> acc;
+  uint4 first[kUnroll];
+  float vm[kUnroll];
+#pragma unroll
+  for (int i = 0; i < kUnroll; ++i) first[i] = load_vec(x, j0 + i * chunk, lo, hi, true);
+#pragma unroll
+  for (int i = 0; i < kUnroll; ++i) vm[i] = vec_max<LT>(first[i]);
+  float v = max_nan(max_nan(vm[0], vm[1]), max_nan(vm[2], vm[3]));
+  static_assert(kUnroll == 4, "");
+  v = v != v ? INFINITY : v;
   for (int size = 2; size <= 32; size <<= 1)
     for (int stride = size >> 1; stride > 0; stride >>= 1) {
       const float o = __shfl_xor_sync(0xffffffffu, v, stride);
       const bool larger = ((lane & stride) == 0) == ((lane & size) == 0);
       v = larger ? fmaxf(v, o) : fminf(v, o);
     }
-  // only warps whose 256 elements all lie in the part count; too few of them give no threshold
-  const int whole = min(kWarps, max(0, hi - base) / (32 * kVec));
-  const int nth_of = whole ? (k + whole - 1) / whole : 33;
+  const int whole = min(kWarps, max(0, hi - base) / (32 * N));
+  const int nth_of = whole ? (k + whole - 1) / whole : 33;             // more than a warp's threads: no threshold
   const float nth = __shfl_sync(0xffffffffu, v, min(nth_of, 32) - 1);
+  const float warp_max = __shfl_sync(0xffffffffu, v, 0);
   if (lane == 0) {
     s.warp_nth[tid >> 5] = nth;
-    s.warp_max[tid >> 5] = v;
+    s.warp_max[tid >> 5] = warp_max;
   }
+  acc.init(warp_max, c, 0.f);                                          // later maxima are rare
+#pragma unroll
+  for (int i = 0; i < kUnroll; ++i) acc.template push<LT>(first[i], vm[i], c, 0.f);
   __syncthreads();
   float thr0 = INFINITY, most = s.warp_max[0];
   for (int w = 0; w < kWarps; ++w) {
@@ -390,105 +557,97 @@ __global__ void __launch_bounds__(kThreads, 2) top_fwd_kernel(TopArgs a) {
   if (tid == 0) s.thr = thr0;
   float thr = thr0;
   __syncthreads();
-  auto offer = [&](const float (&e)[8], int j, float vm) {
+  volatile float* shared_thr = &s.thr;
+  auto offer = [&](int j, const float (&top)[kUnroll]) {
     bool full = false;
-    if (!(vm < thr)) {
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        if (!(e[i] < thr) && j + i >= lo && j + i < hi) {
-          const int pos = atomicAdd(&s.count, 1);
-          if (pos < kSlots) s.keys[pos] = key_of(e[i], j + i);
-          atomicAdd(&s.bins[bin_of(e[i], thr0, inv_width)], 1);
-          full |= (pos & 63) == 63;
-        }
+    for (int i = 0; i < kUnroll; ++i) {
+      if (!(top[i] < thr) && j + i * chunk < hi && j + i * chunk + N > lo) {
+        const int pos = atomicAdd(&s.count, 1);
+        if (pos < kCand) s.cand[pos] = j + i * chunk;
+        atomicAdd(&s.bins[bin_of(top[i], thr0, inv_width)], 1);
+        full |= (pos & 31) == 31;
       }
     }
     if (__any_sync(0xffffffffu, full)) {
       const int b = cut_bin(s.bins, k);
       const float t = fmaf(b - 0.5f, width, thr0);
-      if (lane == 0 && b > 0 && t > *const_cast<volatile float*>(&s.thr)) *const_cast<volatile float*>(&s.thr) = t;
+      if (lane == 0 && b > 0 && t > *shared_thr) *shared_thr = t;
       __syncwarp();
     }
   };
-  offer(z, j0, v0);
-  for (int at = base + kChunk; at < hi; at += 2 * kChunk) {
-    const int j = at + tid * kVec;
-    float y[8];
-    load8(x, j, lo, hi, true, z);
-    load8(x, j + kChunk, lo, hi, true, y);
-    const float vz = max8(z), vy = max8(y);
-    stat_push8<X>(st, z, vz, c, 0.f);
-    stat_push8<X>(st, y, vy, c, 0.f);
-    thr = *const_cast<volatile float*>(&s.thr);
-    offer(z, j, vz);
-    offer(y, j + kChunk, vy);
-  }
+  offer(j0, vm);
+  each_vec(x, base + kUnroll * chunk, lo, hi, [&](int j, const uint4 (&u)[kUnroll]) {
+    float top[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) top[i] = vec_max<LT>(u[i]);
+    thr = *shared_thr;
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) acc.template push<LT>(u[i], top[i], c, 0.f);
+    offer(j, top);
+  });
   __syncthreads();
   // ---- the block's k best, sorted
   const int n = s.count;
-  const int want = min(k, hi - lo);
-  const unsigned long long* best = s.keys;
-  if (n > kSlots) {
-    select_in_order(s, x, lo, hi, k);
-  } else if (n <= 128) {
-    sort_keys(s.keys, n);
-  } else {
+  bool fits = n <= kCand;
+  if (fits) {
     const int b = cut_bin(s.bins, k);
+    thr = b > 0 ? fmaxf(*shared_thr, fmaf(b - 0.5f, width, thr0)) : *shared_thr;
     for (int i = tid; i < n; i += kThreads) {
-      const unsigned long long key = s.keys[i];
-      if (bin_of(key_value(key), thr0, inv_width) >= b) {
-        const int pos = atomicAdd(&s.n_picked, 1);
-        if (pos < kPicked) s.picked[pos] = key;
+      const int j = s.cand[i];
+      float z[N];
+      unpack(load_vec(x, j, lo, hi, true), z);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        if (!(z[e] < thr) && j + e >= lo && j + e < hi) {
+          const int pos = atomicAdd(&s.n_keys, 1);
+          if (pos < kKeys) s.keys[pos] = key_of(z[e], j + e);
+        }
       }
     }
     __syncthreads();
-    if (s.n_picked <= kPicked) {
-      best = s.picked;
-      sort_keys(s.picked, s.n_picked);
-    } else {
-      sort_keys(s.keys, n);
-    }
+    fits = s.n_keys <= kKeys;
   }
-  st = stat_block<X>(st, s.stat, c, 0.f);
+  if (fits)
+    sort_keys(s.keys, s.n_keys);
+  else
+    select_in_order(s, x, lo, hi, k);
+  Stat st = stat_block<X>(acc.stat(), s.stat, c, 0.f);
   // ---- over the cluster: the first block collects lists and statistics
   if (blocks > 1) {
-    if (best != s.picked) {
-      for (int i = tid; i < want; i += kThreads) s.picked[i] = best[i];
-    }
     if (tid == 0) {
       s.part = st;
-      s.n_picked = want;
+      s.n_keys = min(k, hi - lo);
     }
     cluster.sync();
     if (rank == 0) {
-      int at = 0;
-      for (int r = 0; r < blocks; ++r) {
+      int at = s.n_keys;
+      for (int r = 1; r < blocks; ++r) {
         const Select* o = cluster.map_shared_rank(&s, r);
-        const int m = o->n_picked;
-        for (int i = tid; i < m; i += kThreads) s.keys[at + i] = o->picked[i];
+        const int m = o->n_keys;
+        for (int i = tid; i < m; i += kThreads) s.keys[at + i] = o->keys[i];
         at += m;
-        if (r > 0) stat_merge<X>(st, o->part, c, 0.f);
+        stat_merge<X>(st, o->part, c, 0.f);
       }
       __syncthreads();
       sort_keys(s.keys, at);
-      best = s.keys;
     }
     cluster.sync();                      // the others' shared memory was read
     if (rank != 0) return;
   }
-  const float ls = log_sum(st.s);
+  const Row r = finish_row<LT, X>(st, x, a.V, s.stat, c, 0.f);
   for (int i = tid; i < k; i += kThreads) {
-    const unsigned long long key = best[i];
+    const unsigned long long key = s.keys[i];
     a.ids[static_cast<long long>(row) * k + i] = key_index(key);
-    a.top[static_cast<long long>(row) * k + i] = (key_value(key) - st.m) * a.inv_temp - ls;
+    a.top[static_cast<long long>(row) * k + i] = (key_value(key) - r.m) * a.inv_temp - r.ls;
   }
   if (tid == 0) {
     if (a.target) {
       const long long t = a.targets[row];
-      a.target[row] = (t >= 0 && t < a.V) ? (to_f(x[t]) - st.m) * a.inv_temp - ls : 0.f;
+      a.target[row] = (t >= 0 && t < a.V) ? (to_f(x[t]) - r.m) * a.inv_temp - r.ls : 0.f;
     }
-    if (a.entropy) a.entropy[row] = st.s == 0.f ? 0.f : ls - a.inv_temp * (st.sd / st.s);
-    a.stats[row] = make_float2(st.m, ls);
+    if (a.entropy) a.entropy[row] = r.x;
+    a.stats[row] = make_float2(r.m, r.ls);
   }
 }
 
@@ -504,121 +663,128 @@ struct DistillArgs {
   const long long* labels;     // [T] or null; a label outside the vocabulary is ignored
   float* kl;                   // [T]
   float* nll;                  // [T] or null
-  float4* stats;               // [T]: m, ln s at temperature 1, ln s at the temperature, unused
+  float* stats;                // [T, kDistillStats]
 };
 
-struct List {                  // statistics of the list, the same in every lane
-  float mt, st, mx, sx;        // teacher: max, sum; student: max, sum (relative to the max)
-};
+// Per row: m, ln s at temperature 1, ln s at the temperature, the list's teacher mass (full); then for a list that is
+// normalised over itself the teacher's maximum and ln sum, the student's maximum and ln sum (+inf: nothing usable).
+constexpr int kDistillStats = 8;
 
-__device__ __forceinline__ float warp_max(float v) {
+__device__ __forceinline__ float warp_max_of(float v) {
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-__device__ __forceinline__ float warp_sum(float v) {
+__device__ __forceinline__ float warp_sum_of(float v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// Statistics of a row's list normalised over the list itself, by one warp.
+// The list of one row, by one warp; writes the row's outputs. ls1, ls2: ln s at temperature 1 and at the temperature.
 template <typename LT>
-__device__ __forceinline__ List list_stats(const LT* x, const long long* ids, const float* values, int V, int k,
-                                           float c) {
-  List l{-FLT_MAX, 0.f, -FLT_MAX, 0.f};
-  const int lane = threadIdx.x & 31;
-  for (int i = lane; i < k; i += 32) {
-    const long long id = ids[i];
-    if (id < 0 || id >= V) continue;
-    l.mt = fmaxf(l.mt, values[i]);
-    l.mx = fmaxf(l.mx, to_f(x[id]));
-  }
-  l.mt = warp_max(l.mt);
-  l.mx = warp_max(l.mx);
-  for (int i = lane; i < k; i += 32) {
-    const long long id = ids[i];
-    if (id < 0 || id >= V) continue;
-    l.st += ex2((values[i] - l.mt) * c);
-    l.sx += ex2((to_f(x[id]) - l.mx) * c);
-  }
-  l.st = warp_sum(l.st);
-  l.sx = warp_sum(l.sx);
-  return l;
-}
-
-// PASSES: how many softmax sums of the row are needed. 0 (only the listed entries matter: one warp per row), 1 (scale
-// c1 in the exponent) or 2 (c1 and c2).
-template <typename LT, int PASSES>
-__global__ void __launch_bounds__(PASSES ? kThreads : 32) distill_fwd_kernel(DistillArgs a, float c1, float c2) {
-  __shared__ Stat sh_stat[kWarps];
-  __shared__ Stat sh_part;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int blocks = PASSES ? static_cast<int>(cluster.num_blocks()) : 1;
-  const int rank = PASSES ? static_cast<int>(cluster.block_rank()) : 0;
-  const int row = blockIdx.x / blocks, tid = threadIdx.x;
-  const LT* x = static_cast<const LT*>(a.logits) + static_cast<long long>(row) * a.ld;
-  const int V = a.V, k = a.k;
-  Stat st = stat_init();
-  constexpr int X = PASSES == 2 ? kSecond : kNone;
-  if (PASSES > 0) {
-    const int2 part = part_of(V, rank, blocks);
-    const int lo = part.x, hi = part.y;
-    for (int j = lo - misalign(x + lo) + tid * kVec; j < hi; j += 2 * kChunk) {
-      float z[8], y[8];
-      load8(x, j, lo, hi, true, z);
-      load8(x, j + kChunk, lo, hi, true, y);
-      stat_push8<X>(st, z, max8(z), c1, c2);
-      stat_push8<X>(st, y, max8(y), c1, c2);
-    }
-    st = stat_block<X>(st, sh_stat, c1, c2);
-    if (blocks > 1) {
-      if (tid == 0) sh_part = st;
-      cluster.sync();
-      if (rank == 0)
-        for (int r = 1; r < blocks; ++r) stat_merge<X>(st, *cluster.map_shared_rank(&sh_part, r), c1, c2);
-      cluster.sync();
-      if (rank != 0) return;
-    }
-  }
-  if (tid >= 32) return;
-  // With one pass both sums are the same number and only the one that is asked for gets used.
-  const float ls1 = log_sum(st.s);
-  const float ls2 = PASSES == 2 ? log_sum(st.sd) : ls1;
+__device__ __forceinline__ void distill_list(const DistillArgs& a, int row, const LT* x, float m, float ls1, float ls2) {
+  const int lane = threadIdx.x & 31, V = a.V, k = a.k;
   const long long* ids = a.ids + static_cast<long long>(row) * k;
   const float* values = a.values + static_cast<long long>(row) * k;
-  float kl = 0.f;
+  float kl = 0.f, mass = 0.f, mt = -FLT_MAX, mx = -FLT_MAX, lt = 0.f, lx = 0.f;
   if (a.full) {
-    for (int i = tid; i < k; i += 32) {
+    for (int i = lane; i < k; i += 32) {
       const long long id = ids[i];
       if (id < 0 || id >= V) continue;
       const float t = values[i], q = expf(t);
+      mass += q;
       if (q == 0.f) continue;
-      kl += q * (t - ((to_f(x[id]) - st.m) * a.inv_temp - ls2));
+      kl += q * (t - ((to_f(x[id]) - m) * a.inv_temp - ls2));
     }
-    kl = warp_sum(kl);
+    mass = warp_sum_of(mass);
+    kl = warp_sum_of(kl);
     if (ls2 == INFINITY) kl = 0.f;
   } else {
     const float c = a.inv_temp * kLog2e;
-    const List l = list_stats(x, ids, values, V, k, c);
-    const float lt = logf(l.st), lx = logf(l.sx);
-    for (int i = tid; i < k; i += 32) {
+    float st = 0.f, sx = 0.f;
+    for (int i = lane; i < k; i += 32) {
       const long long id = ids[i];
       if (id < 0 || id >= V) continue;
-      const float lq = (values[i] - l.mt) * a.inv_temp - lt;
+      mt = fmaxf(mt, values[i]);
+      mx = fmaxf(mx, to_f(x[id]));
+    }
+    mt = warp_max_of(mt);
+    mx = warp_max_of(mx);
+    for (int i = lane; i < k; i += 32) {
+      const long long id = ids[i];
+      if (id < 0 || id >= V) continue;
+      st += ex2((values[i] - mt) * c);
+      sx += ex2((to_f(x[id]) - mx) * c);
+    }
+    lt = log_sum(warp_sum_of(st));
+    lx = log_sum(warp_sum_of(sx));
+    for (int i = lane; i < k; i += 32) {
+      const long long id = ids[i];
+      if (id < 0 || id >= V) continue;
+      const float lq = (values[i] - mt) * a.inv_temp - lt;
       const float q = expf(lq);
       if (q == 0.f) continue;
-      kl += q * (lq - ((to_f(x[id]) - l.mx) * a.inv_temp - lx));
+      kl += q * (lq - ((to_f(x[id]) - mx) * a.inv_temp - lx));
     }
-    kl = warp_sum(kl);
-    if (l.st == 0.f || l.sx == 0.f) kl = 0.f;
+    kl = warp_sum_of(kl);
+    if (lt == INFINITY || lx == INFINITY) kl = 0.f;
   }
-  if (tid == 0) {
+  if (lane == 0) {
     a.kl[row] = kl;
     if (a.nll) {
       const long long t = a.labels[row];
-      a.nll[row] = (t >= 0 && t < V && ls1 != INFINITY) ? ls1 - (to_f(x[t]) - st.m) : 0.f;
+      a.nll[row] = (t >= 0 && t < V && ls1 != INFINITY) ? ls1 - (to_f(x[t]) - m) : 0.f;
     }
-    a.stats[row] = make_float4(st.m, ls1, ls2, 0.f);
+    float4* out = reinterpret_cast<float4*>(a.stats + static_cast<long long>(row) * kDistillStats);
+    out[0] = make_float4(m, ls1, ls2, mass);
+    out[1] = make_float4(mt, lt, mx, lx);
   }
+}
+
+// Only the listed entries matter: one warp per row.
+template <typename LT>
+__global__ void __launch_bounds__(kThreads) distill_list_kernel(DistillArgs a) {
+  const int row = blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (row >= a.T) return;
+  distill_list(a, row, static_cast<const LT*>(a.logits) + static_cast<long long>(row) * a.ld, -FLT_MAX, INFINITY, INFINITY);
+}
+
+// X: kNone (one softmax sum of the row, scale c1 in the exponent) or kSecond (c1 and c2).
+template <typename LT, int X>
+__global__ void __launch_bounds__(kThreads) distill_fwd_kernel(DistillArgs a, float c1, float c2) {
+  __shared__ Stat sh_stat[kWarps];
+  __shared__ Stat sh_part;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int row = blockIdx.x / blocks, tid = threadIdx.x;
+  const LT* x = static_cast<const LT*>(a.logits) + static_cast<long long>(row) * a.ld;
+  const int2 part = part_of(a.V, rank, blocks);
+  const int lo = part.x, hi = part.y;
+  Acc<X> acc;
+  acc.init(-INFINITY, c1, c2);
+  bool fresh = true;
+  each_vec(x, lo - misalign(x + lo), lo, hi, [&](int, const uint4 (&u)[kUnroll]) {
+    float top[kUnroll];
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) top[i] = vec_max<LT>(u[i]);
+    if (fresh) {                         // begin with the warp's maximum: later ones are rare
+      acc.init(warp_max_of(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))), c1, c2);
+      fresh = false;
+    }
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i) acc.template push<LT>(u[i], top[i], c1, c2);
+  });
+  Stat st = stat_block<X>(acc.stat(), sh_stat, c1, c2);
+  if (blocks > 1) {
+    if (tid == 0) sh_part = st;
+    cluster.sync();
+    if (rank == 0)
+      for (int r = 1; r < blocks; ++r) stat_merge<X>(st, *cluster.map_shared_rank(&sh_part, r), c1, c2);
+    cluster.sync();
+    if (rank != 0) return;
+  }
+  const Row r = finish_row<LT, X>(st, x, a.V, sh_stat, c1, c2);
+  // With one sum both logarithms are the same number and only the one that is asked for gets used.
+  if (tid < 32) distill_list(a, row, x, r.m, r.ls, X == kSecond ? r.x : r.ls);
 }
 
 // ---- backward -------------------------------------------------------------------------------------------
@@ -636,145 +802,193 @@ struct BwdArgs {
   const float* g_given;        // [T] gradient of nll / of the target's log-probability, or null
   const float* g_entropy;      // [T] or null
   const float* entropy;        // [T] when g_entropy
-  const float* m;              // row statistics: m, ln s at temperature 1, ln s at the temperature, `stat_stride` floats
-  int stat_stride, stat_one, stat_temp;
+  const float* stats;          // [T, 2] (score: m, ln s) or [T, kDistillStats]
   void* dx;
   long long ldd;
   int blocks;                  // a row's columns are cut into this many parts
+  int one;                     // both softmaxes are the same: their factors are added
 };
 
 // d_j = A p_j (temperature) + B p_j (temperature 1) - G p_j (log p_j + H), then the listed columns get their own
 // terms on top: they are computed from the same fp32 value and rounded once, by the thread of the first occurrence.
 template <typename LT, int DENSE>   // bit 0: temperature, bit 1: temperature 1, bit 2: entropy
 __global__ void __launch_bounds__(kThreads) top_bwd_kernel(BwdArgs a) {
-  __shared__ int sh_id[kMaxList + 1];
-  __shared__ float sh_coef[kMaxList + 1];
-  __shared__ float sh_dense[2];
+  __shared__ __align__(16) int sh_id[kMaxList];
+  __shared__ float sh_coef[kMaxList];
+  __shared__ float sh_sum[kWarps];
+  constexpr int N = kVec<LT>, chunk = kChunk<LT>;
   const int row = blockIdx.x / a.blocks, tid = threadIdx.x;
   const int2 part = part_of(a.V, blockIdx.x - row * a.blocks, a.blocks);
   const int lo = part.x, hi = part.y;
   const LT* x = static_cast<const LT*>(a.logits) + static_cast<long long>(row) * a.ld;
   LT* dx = static_cast<LT*>(a.dx) + static_cast<long long>(row) * a.ldd;
-  const int V = a.V, k = a.k;
-  const float* st = a.m + static_cast<long long>(row) * a.stat_stride;
-  const float m = st[0], ls1 = st[a.stat_one], lst = st[a.stat_temp];
+  const int V = a.V, k = a.k, mode = a.mode;
+  const int from = lo - misalign(dx + lo);
+  const bool aligned = misalign(x + lo) == misalign(dx + lo);
+  uint4 u[kUnroll];
+  auto load = [&](int j) {
+#pragma unroll
+    for (int i = 0; i < kUnroll; ++i)
+      if (j + i * chunk < hi) u[i] = load_vec(x, j + i * chunk, lo, hi, aligned);
+  };
+  if (DENSE) load(from + tid * N);                 // on their way while the list is looked at
+  const float* st = a.stats + static_cast<long long>(row) * (mode == kScore ? 2 : kDistillStats);
+  const float m = st[0], ls1 = st[1], lst = mode == kScore ? st[1] : st[2];
   const float c = a.inv_temp * kLog2e;
-  if (tid < 32) {
-    const long long* ids = a.ids + static_cast<long long>(row) * k;
-    const float* values = a.values ? a.values + static_cast<long long>(row) * k : nullptr;
-    const float g = a.g_list ? a.g_list[row] : 0.f;
-    float sum = 0.f;                      // of what multiplies p at the temperature
-    List l{};
-    float lt = 0.f, lx = 0.f;
-    bool live = true;
-    if (a.mode == kListed) {
-      l = list_stats(x, ids, values, V, k, c);
-      lt = logf(l.st);
-      lx = logf(l.sx);
-      live = l.st != 0.f && l.sx != 0.f;
-    } else {
-      live = lst != INFINITY;
-    }
-    live = live && (a.mode == kScore ? values != nullptr : a.g_list != nullptr);
-    for (int i = tid; i < k; i += 32) {
+  // ---- factors of the list
+  const long long* ids = a.ids + static_cast<long long>(row) * k;
+  const float* values = a.values ? a.values + static_cast<long long>(row) * k : nullptr;
+  const float g = a.g_list ? a.g_list[row] : 0.f;
+  float mt = 0.f, lt = 0.f, mx = 0.f, lx = 0.f;
+  bool live = mode == kScore ? values != nullptr : a.g_list != nullptr;
+  if (mode == kListed) {
+    mt = st[4]; lt = st[5]; mx = st[6]; lx = st[7];
+    live = live && lt != INFINITY && lx != INFINITY;
+  } else {
+    live = live && lst != INFINITY;
+  }
+  float sum = 0.f;
+  for (int i = tid; i < (k + 3) / 4 * 4; i += kThreads) {
+    int at = -1;
+    float coef = 0.f;
+    if (live && i < k) {
       const long long id = ids[i];
-      int at = -1;
-      float coef = 0.f;
-      if (live && id >= 0 && id < V) {
+      if (id >= 0 && id < V) {
         at = static_cast<int>(id);
-        if (a.mode == kScore) {
+        if (mode == kScore) {
           coef = values[i];
-          sum -= coef;
-        } else if (a.mode == kFull) {
-          const float q = expf(values[i]);
-          coef = -g * q;
-          sum -= coef;
+          sum += coef;
+        } else if (mode == kFull) {
+          coef = -g * expf(values[i]);
         } else {
-          const float q = expf((values[i] - l.mt) * a.inv_temp - lt);
-          const float p = expf((to_f(x[id]) - l.mx) * a.inv_temp - lx);
+          const float q = expf((values[i] - mt) * a.inv_temp - lt);
+          const float p = expf((to_f(x[id]) - mx) * a.inv_temp - lx);
           coef = g * (p - q);
         }
       }
-      sh_id[i] = at;
-      sh_coef[i] = coef * a.inv_temp;
     }
-    sum = warp_sum(sum);
-    if (tid == 0) {
-      int at = -1;
-      float coef = 0.f;
-      if (a.g_given) {
-        const long long t = a.given[row];
-        if (t >= 0 && t < V && (a.mode == kScore ? lst : ls1) != INFINITY) {
-          at = static_cast<int>(t);
-          coef = a.g_given[row];
-        }
-      }
-      sh_id[k] = at;
-      sh_coef[k] = a.mode == kScore ? coef * a.inv_temp : -coef;
-      if (a.mode == kScore) sum -= coef;
-      sh_dense[0] = sum * a.inv_temp;
-      sh_dense[1] = a.mode == kScore ? 0.f : coef;
+    sh_id[i] = at;
+    if (i < k) sh_coef[i] = coef * a.inv_temp;
+  }
+  if (mode == kScore) {
+    sum = warp_sum_of(sum);
+    if ((tid & 31) == 0) sh_sum[tid >> 5] = sum;
+  }
+  int given = -1;
+  float g_given = 0.f;
+  if (a.g_given) {
+    const long long t = a.given[row];
+    if (t >= 0 && t < V && (mode == kScore ? lst : ls1) != INFINITY) {
+      given = static_cast<int>(t);
+      g_given = a.g_given[row];
     }
   }
   __syncthreads();
-  const float A = sh_dense[0], B = sh_dense[1];
-  const float lst2 = lst * kLog2e, ls12 = ls1 * kLog2e;
-  float G = 0.f, H = 0.f;
-  if (DENSE & 4) {
-    G = a.g_entropy[row] * a.inv_temp;
-    H = a.entropy[row];
+  float A = 0.f, B = 0.f, given_coef = 0.f;
+  if (mode == kScore) {
+    A = 0.f;
+    for (int w = 0; w < kWarps; ++w) A += sh_sum[w];
+    A = -(A + g_given) * a.inv_temp;
+    given_coef = g_given * a.inv_temp;
+  } else {
+    if (mode == kFull && live) A = g * a.inv_temp * st[3];
+    if (a.one) A += g_given; else B = g_given;
+    given_coef = -g_given;
   }
-  auto dense = [&](float v) -> float {
-    const float d = v - m;
-    float r = 0.f;
+  const float lst2 = lst * kLog2e, ls12 = ls1 * kLog2e;
+  float G = 0.f;
+  if (DENSE & 4) {
+    const float ge = a.g_entropy[row] * a.inv_temp;
+    G = -ge * kLn2;                                // p (A - ge (log p + H)) = p (A - ge H + G log2 p)
+    A -= ge * a.entropy[row];
+  }
+  const f32x2 mm = pack2(-m, -m), cc = pack2(c, c), ll = pack2(-lst2, -lst2), AA = pack2(A, A), GG = pack2(G, G);
+  const f32x2 cc1 = pack2(kLog2e, kLog2e), ll1 = pack2(-ls12, -ls12), BB = pack2(B, B);
+  auto dense2 = [&](f32x2 v) -> f32x2 {
+    const f32x2 d = add2(v, mm);
+    f32x2 r = 0;
     if (DENSE & 5) {
-      const float p = ex2(fmaf(d, c, -lst2));
-      r = A * p;
-      if (DENSE & 4) r -= p == 0.f ? 0.f : G * p * (d * a.inv_temp - lst + H);
+      const float2 e = unpack2(fma2(d, cc, ll));
+      const f32x2 p = pack2(ex2(e.x), ex2(e.y));
+      if (DENSE & 4)
+        r = mul2(p, fma2(GG, pack2(fmaxf(e.x, -1e30f), fmaxf(e.y, -1e30f)), AA));
+      else
+        r = mul2(p, AA);
     }
-    if (DENSE & 2) r = fmaf(B, ex2(fmaf(d, kLog2e, -ls12)), r);
+    if (DENSE & 2) {
+      const float2 e = unpack2(fma2(d, cc1, ll1));
+      r = fma2(pack2(ex2(e.x), ex2(e.y)), BB, r);
+    }
     return r;
   };
-  const int shift = misalign(dx + lo);
-  const bool aligned = misalign(x + lo) == shift;
-  for (int j = lo - shift + tid * kVec; j < hi; j += kChunk) {
-    float z[8];
-    if (DENSE) {
-      load8(x, j, lo, hi, aligned, z);
+  // ---- the whole part
+  for (int at = from; at < hi; at += kUnroll * chunk) {
+    const int j = at + tid * N;
+    if (DENSE && at != from) load(j);
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) z[i] = dense(z[i]);
-    } else {
+    for (int i = 0; i < kUnroll; ++i) {
+      const int ji = j + i * chunk;
+      if (ji >= hi) break;
+      float z[N];
+      if (DENSE) {
+        unpack(u[i], z);
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) z[i] = 0.f;
-    }
-    if (j >= lo && j + kVec <= hi) {
-      vec_store(dx + j, z);
-    } else {
+        for (int e = 0; e < N; e += 2) {
+          const float2 r = unpack2(dense2(pack2(z[e], z[e + 1])));
+          z[e] = r.x;
+          z[e + 1] = r.y;
+        }
+      } else {
 #pragma unroll
-      for (int i = 0; i < kVec; ++i)
-        if (j + i >= lo && j + i < hi) from_f(z[i], dx + j + i);
+        for (int e = 0; e < N; ++e) z[e] = 0.f;
+      }
+      if (ji >= lo && ji + N <= hi) {
+        *reinterpret_cast<uint4*>(dx + ji) = pack(z);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (ji + e >= lo && ji + e < hi) from_f(z[e], dx + ji + e);
+      }
     }
   }
   __syncthreads();
-  for (int i = tid; i <= k; i += kThreads) {
+  // ---- the listed columns of the part
+  auto put = [&](int at, float extra) {
+    const float v = DENSE ? to_f(x[at]) : 0.f;
+    from_f((DENSE ? unpack2(dense2(pack2(v, v))).x : 0.f) + extra, dx + at);
+  };
+  for (int i = tid; i < k; i += kThreads) {
     const int at = sh_id[i];
     if (at < lo || at >= hi) continue;
-    float sum = 0.f;
-    bool mine = true;
-    for (int n = 0; n <= k; ++n) {
-      if (sh_id[n] != at) continue;
-      if (n < i) mine = false;
-      sum += sh_coef[n];
+    int same = 0;
+    for (int n = 0; n < k; n += 4) {
+      const int4 o = *reinterpret_cast<const int4*>(sh_id + n);
+      same += (o.x == at) + (o.y == at) + (o.z == at) + (o.w == at);
     }
-    if (mine) from_f((DENSE ? dense(to_f(x[at])) : 0.f) + sum, dx + at);
+    float extra = sh_coef[i];
+    bool mine = true;
+    if (same > 1) {                                // a column that is listed more than once
+      extra = 0.f;
+      for (int n = 0; n < k; ++n) {
+        if (sh_id[n] != at) continue;
+        if (n < i) mine = false;
+        extra += sh_coef[n];
+      }
+    }
+    if (mine) put(at, extra + (at == given ? given_coef : 0.f));
+  }
+  if (given >= lo && given < hi) {
+    int listed = 0;
+    for (int i = tid; i < k; i += kThreads) listed |= sh_id[i] == given;
+    listed = __syncthreads_or(listed);             // `given` is the same in all threads
+    if (tid == 0 && !listed) put(given, given_coef);
   }
 }
 
-// Blocks per row of a forward pass: one while the rows fill the GPU, else up to kMaxSplit as long as a part is a full
-// iteration of its block.
+// Blocks per row of a forward pass: one while the rows fill the GPU, else up to kMaxSplit.
 int split_of(int T, int V) {
   int n = 1;
-  while (n < kMaxSplit && 2ll * n * T <= 2ll * txh::sm_count() && V / (2 * n) >= kChunk) n *= 2;
+  while (n < kMaxSplit && 2ll * n * T <= 4ll * txh::sm_count() && V / (2 * n) >= kMinPart) n *= 2;
   return n;
 }
 
@@ -802,7 +1016,7 @@ int launch_rows(int T, int blocks, int bytes, cudaStream_t s, Args... args) {
 
 template <typename LT>
 int launch_bwd(BwdArgs a, int dense, cudaStream_t s) {
-  const int want = 4 * txh::sm_count(), most = (a.V + kChunk - 1) / kChunk;
+  const int want = 8 * txh::sm_count(), most = (a.V + kMinPart - 1) / kMinPart;
   a.blocks = min(most, a.T >= want ? 1 : (want + a.T - 1) / a.T);
 #define TX_BWD(D) case D: top_bwd_kernel<LT, D><<<a.T * a.blocks, kThreads, 0, s>>>(a); break
   switch (dense) {
@@ -815,10 +1029,7 @@ int launch_bwd(BwdArgs a, int dense, cudaStream_t s) {
 
 }  // namespace
 
-extern "C" int tx_top_max_k() { return kMaxTop; }
-extern "C" int tx_top_max_list() { return kMaxList; }
-
-// logits [T, V] with row stride ld (elements), fp32 or bf16; 1 <= k <= min(V, tx_top_max_k()).
+// logits [T, V] with row stride ld (elements), fp32 or bf16; 1 <= k <= min(V, 256).
 extern "C" int tx_top_logprob_fwd(const void* logits, int logits_fp32, long long ld, int T, int V, int k,
                                   float inv_temp, const long long* targets, long long* ids, float* top, float* target,
                                   float* entropy, float* stats, cudaStream_t s) {
@@ -833,26 +1044,29 @@ extern "C" int tx_top_logprob_fwd(const void* logits, int logits_fp32, long long
                  : launch_rows<top_fwd_kernel<__nv_bfloat16, kNone>>(T, n, bytes, s, a);
 }
 
+// 1 <= k <= 1024; stats [T, 8].
 extern "C" int tx_top_distill_fwd(const void* logits, int logits_fp32, long long ld, int T, int V, int k,
                                   float inv_temp, int full, const long long* ids, const float* values,
                                   const long long* labels, float* kl, float* nll, float* stats, cudaStream_t s) {
   if (T <= 0) return 0;
   if (V < 1 || k < 1 || k > kMaxList || V > 0x7fff0000) return 1;
-  const DistillArgs a{logits, ld, T, V, k, inv_temp, full, ids, values, labels, kl, nll, reinterpret_cast<float4*>(stats)};
-  const float c = inv_temp * kLog2e;
-  const int passes = (nll ? 1 : 0) + (full ? 1 : 0) - (nll && full && inv_temp == 1.f ? 1 : 0);
-  const float c1 = nll ? kLog2e : c;
+  const DistillArgs a{logits, ld, T, V, k, inv_temp, full, ids, values, labels, kl, nll, stats};
+  const float c = inv_temp * kLog2e, c1 = nll ? kLog2e : c;
   const int n = split_of(T, V);
-#define TX_FWD(LT)                                                                          \
-  if (passes == 1) return launch_rows<distill_fwd_kernel<LT, 1>>(T, n, 0, s, a, c1, c);      \
-  if (passes == 2) return launch_rows<distill_fwd_kernel<LT, 2>>(T, n, 0, s, a, c1, c);      \
-  distill_fwd_kernel<LT, 0><<<T, 32, 0, s>>>(a, c1, c)
-  if (logits_fp32) { TX_FWD(float); } else { TX_FWD(__nv_bfloat16); }
-#undef TX_FWD
-  return cudaGetLastError() == cudaSuccess ? 0 : 400;
+  if (!nll && !full) {
+    const int grid = (T + kWarps - 1) / kWarps;
+    if (logits_fp32) distill_list_kernel<float><<<grid, kThreads, 0, s>>>(a);
+    else             distill_list_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(a);
+    return cudaGetLastError() == cudaSuccess ? 0 : 400;
+  }
+  if (nll && full && inv_temp != 1.f)
+    return logits_fp32 ? launch_rows<distill_fwd_kernel<float, kSecond>>(T, n, 0, s, a, c1, c)
+                       : launch_rows<distill_fwd_kernel<__nv_bfloat16, kSecond>>(T, n, 0, s, a, c1, c);
+  return logits_fp32 ? launch_rows<distill_fwd_kernel<float, kNone>>(T, n, 0, s, a, c1, c)
+                     : launch_rows<distill_fwd_kernel<__nv_bfloat16, kNone>>(T, n, 0, s, a, c1, c);
 }
 
-// Gradient of tx_top_logprob_fwd: values = gradients of the list (or null), given = targets.
+// Gradient of tx_top_logprob_fwd: g_top or null, g_target with targets or null, g_entropy with entropy or null.
 extern "C" int tx_top_logprob_bwd(const void* logits, int logits_fp32, long long ld, int T, int V, int k,
                                   float inv_temp, const long long* ids, const float* g_top, const long long* targets,
                                   const float* g_target, const float* g_entropy, const float* entropy,
@@ -860,7 +1074,7 @@ extern "C" int tx_top_logprob_bwd(const void* logits, int logits_fp32, long long
   if (T <= 0) return 0;
   if (V < 1 || k < 1 || k > kMaxTop || V > 0x7fff0000) return 1;
   const BwdArgs a{logits, ld, T, V, k, kScore, inv_temp, ids, g_top, targets, nullptr, g_target, g_entropy, entropy,
-                  stats, 2, 1, 1, dx, ldd, 1};
+                  stats, dx, ldd, 1, 0};
   const int dense = g_entropy ? 5 : 1;
   return logits_fp32 ? launch_bwd<float>(a, dense, s) : launch_bwd<__nv_bfloat16>(a, dense, s);
 }
@@ -872,8 +1086,9 @@ extern "C" int tx_top_distill_bwd(const void* logits, int logits_fp32, long long
                                   void* dx, long long ldd, cudaStream_t s) {
   if (T <= 0) return 0;
   if (V < 1 || k < 1 || k > kMaxList || V > 0x7fff0000) return 1;
+  const int both = full && g_kl && g_nll && inv_temp == 1.f;
   const BwdArgs a{logits, ld, T, V, k, full ? kFull : kListed, inv_temp, ids, values, labels, g_kl, g_nll, nullptr,
-                  nullptr, stats, 4, 1, 2, dx, ldd, 1};
-  const int dense = (full && g_kl ? 1 : 0) | (g_nll ? 2 : 0);
+                  nullptr, stats, dx, ldd, 1, both};
+  const int dense = (full && g_kl ? 1 : 0) | (g_nll && !both ? 2 : 0);
   return logits_fp32 ? launch_bwd<float>(a, dense, s) : launch_bwd<__nv_bfloat16>(a, dense, s);
 }

@@ -295,13 +295,13 @@ def top_logprobs_bwd(logits, ids, targets, stats, entropy, g_top, g_target, g_en
 def top_distill_fwd(logits: torch.Tensor, ids: torch.Tensor, values: torch.Tensor, labels: Optional[torch.Tensor],
                     inv_temp: float, full: bool):
   """logits [T, V] fp32/bf16 with unit column stride, ids [T, k] int64 and values [T, k] fp32 contiguous, labels [T]
-  int64 or None -> (kl [T], nll [T] or None, stats [T, 4]), fp32."""
+  int64 or None -> (kl [T], nll [T] or None, stats [T, 8]), fp32."""
   T, V = logits.shape
   dev = logits.device
   f32 = torch.float32
   kl = torch.empty(T, dtype=f32, device=dev)
   nll = torch.empty(T, dtype=f32, device=dev) if labels is not None else None
-  stats = torch.empty((T, 4), dtype=f32, device=dev)
+  stats = torch.empty((T, 8), dtype=f32, device=dev)
   _lib.check_rc(_lib.require().tx_top_distill_fwd(
       logits.data_ptr(), int(logits.dtype == f32), logits.stride(0), T, V, ids.shape[1], float(inv_temp), int(full),
       ids.data_ptr(), values.data_ptr(), _p(labels), kl.data_ptr(), _p(nll), stats.data_ptr(), _lib.stream_ptr()),
