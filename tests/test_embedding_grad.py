@@ -69,7 +69,7 @@ def check(ids, D, V, scale, grad_dtype, seed=0):
 @pytest.mark.gpu
 @pytest.mark.parametrize("grad_dtype", [torch.float32, bf16])
 @pytest.mark.parametrize("kind", ["one", "distinct", "rising", "falling", "tail", "padded", "outside"])
-@pytest.mark.parametrize("T,V,D", [(1, 1, 8), (2, 5, 24), (31, 1000, 64), (33, 7, 1152), (1000, 300, 520),
+@pytest.mark.parametrize("T,V,D", [(1, 1, 8), (2, 5, 24), (8, 3, 8), (12, 1, 16), (16, 2, 8), (31, 1000, 64), (33, 7, 1152), (1000, 300, 520),
                                    (4096, 128256, 64), (4097, 1024, 256), (9001, 262144, 40)])
 def test_sorted_sums(kernel_lib, grad_dtype, kind, T, V, D):
   check(id_list(kind, T, V), D, V, 1.0 if T % 2 else 2.5, grad_dtype)
@@ -81,6 +81,9 @@ def test_long_lists_and_large_tables(kernel_lib):
   check(id_list("tail", 20_000, 1_048_577), 8, 1_048_577, 1.0, bf16)       # three passes of the sort
   check(id_list("padded", 5000, 100), 4104, 100, 1.0, torch.float32)       # several column tiles
   check(id_list("one", 0, 10), 8, 10, 1.0, torch.float32)
+  for T in (5, 40, 700, 4096, 9000, 20_000):                               # runs that end on and around chunk borders
+    for length in (1, 3, 4, 5, 8, 9, 15, 16, 31, 32, 33, 63, 64, 65, 97):
+      check(torch.arange(T) // length, 8, T, 1.0, torch.float32)
   check(id_list("tail", 5000, 100).to(torch.int32), 64, 100, 1.0, torch.float32)
 
 

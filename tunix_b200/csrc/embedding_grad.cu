@@ -1,12 +1,13 @@
 // Gradient of an embedding table, summed by sorted tokens: grad[v, :] (+)= scale * sum over the positions t with
 // ids[t] == v of dout[t, :], every sum in one fixed order and no atomics.
 //
-// Three launches. (1) One cluster sorts the pairs (id, position) by id, equal ids by position: a radix sort from the
-// low digit up whose per-warp digit counts live in shared memory and whose per-block totals are read through
-// distributed shared memory. (2) Blocks walk `chunk` sorted positions each, so a frequent token is spread over many
-// blocks; a run of equal ids inside a chunk is written at once, one that crosses a border leaves an fp32 partial sum.
-// (3) The chunk where such a run begins adds its partial sums in order. dout is read once and every present row of
-// the table is touched once. Ids outside the vocabulary sort behind all others and are left out.
+// Three launches. (1) The pairs (id, position) are sorted by id, equal ids by position. Few tokens: every pair counts
+// the pairs before it. More: one cluster, a radix sort from the low digit up whose per-warp digit counts live in shared
+// memory and whose per-block totals are read through distributed shared memory. (2) Blocks walk `chunk` sorted positions
+// each. A run of equal ids is summed by the block where it begins, also a little into the next chunk; a run that covers
+// a whole chunk (a frequent token, the padding id) is summed by every block it touches, into fp32 partial sums.
+// (3) The partial sums of such a run are added in order. dout is read once and every present row of the table is
+// touched once. Ids outside the vocabulary sort behind all others and are left out.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -22,6 +23,10 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kMaxDigits = 1024;              // 10 bits a pass
 constexpr int kSortCluster = 8;
+constexpr int kSortTile = 8;                  // pairs a lane has in flight
+constexpr int kCountTokens = 4096;            // up to here every pair counts the pairs before it: T^2 / 2 comparisons
+constexpr int kCountThreads = 256;
+constexpr int kCountPer = 8;                  // threads per pair
 
 struct SortArgs {
   const void* ids;
@@ -30,13 +35,39 @@ struct SortArgs {
   int passes, bits;           // digit width
   int2* a;                    // [T]; the sorted pairs end up here
   int2* b;                    // [T]
+  int* n_long;                // set to 0 here: length of the list of long runs
 };
+
+// Ids outside the vocabulary become V.
+__device__ __forceinline__ int id_at(const SortArgs& s, int i) {
+  const long long id = s.ids64 ? static_cast<const long long*>(s.ids)[i] : static_cast<const int*>(s.ids)[i];
+  return (id < 0 || id >= s.V) ? s.V : static_cast<int>(id);
+}
 
 // Pair `i` of the input of pass `p`.
 __device__ __forceinline__ int2 sort_load(const SortArgs& s, const int2* src, int p, int i) {
-  if (p > 0) return src[i];
-  const long long id = s.ids64 ? static_cast<const long long*>(s.ids)[i] : static_cast<const int*>(s.ids)[i];
-  return make_int2((id < 0 || id >= s.V) ? s.V : static_cast<int>(id), i);
+  return p > 0 ? src[i] : make_int2(id_at(s, i), i);
+}
+
+__global__ void __launch_bounds__(kCountThreads) count_sort_kernel(SortArgs s) {
+  __shared__ int4 ids4[kCountTokens / 4];
+  int* ids = reinterpret_cast<int*>(ids4);
+  const int padded = (s.T + 3) / 4 * 4;
+  for (int i = threadIdx.x; i < padded; i += kCountThreads) ids[i] = i < s.T ? id_at(s, i) : 0x7fffffff;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *s.n_long = 0;
+  __syncthreads();
+  const int i = blockIdx.x * (kCountThreads / kCountPer) + threadIdx.x / kCountPer;
+  const int id = i < s.T ? ids[i] : 0;
+  int before = 0;
+  for (int j = threadIdx.x % kCountPer; j < padded / 4; j += kCountPer) {
+    const int4 o = ids4[j];
+    const int p = 4 * j;
+    before += (o.x < id || (o.x == id && p < i)) + (o.y < id || (o.y == id && p + 1 < i)) +
+              (o.z < id || (o.z == id && p + 2 < i)) + (o.w < id || (o.w == id && p + 3 < i));
+  }
+#pragma unroll
+  for (int o = 1; o < kCountPer; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  if (i < s.T && threadIdx.x % kCountPer == 0) s.a[before] = make_int2(id, i);
 }
 
 // Every warp owns a contiguous part of its block's part of the pairs, which keeps each pass stable.
@@ -53,6 +84,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_ids_kernel(SortArgs s) {
   const int per = (s.T + parts - 1) / parts;
   const int lo = min(s.T, (rank * kSortWarps + warp) * per), hi = min(s.T, lo + per);
   int* mine = hist + warp * digits;
+  if (rank == 0 && tid == 0) *s.n_long = 0;
   for (int p = 0; p < s.passes; ++p) {
     // the last pass writes `a`
     int2* dst = ((s.passes - 1 - p) & 1) ? s.b : s.a;
@@ -60,15 +92,27 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_ids_kernel(SortArgs s) {
     const int shift = p * s.bits;
     for (int d = lane; d < digits; d += 32) mine[d] = 0;
     __syncwarp();
-    for (int i0 = lo; i0 < hi; i0 += 32) {
-      const int i = i0 + lane;
-      const unsigned live = __ballot_sync(0xffffffffu, i < hi);
-      if (i < hi) {
-        const int d = (sort_load(s, src, p, i).x >> shift) & (digits - 1);
-        const unsigned same = __match_any_sync(live, d);
-        if ((same & ((1u << lane) - 1)) == 0) mine[d] += __popc(same);
+    int2 pair[kSortTile];
+    auto load_tile = [&](int i0) {
+#pragma unroll
+      for (int u = 0; u < kSortTile; ++u) {
+        const int i = i0 + u * 32 + lane;
+        pair[u] = i < hi ? sort_load(s, src, p, i) : make_int2(0, 0);
       }
-      __syncwarp();
+    };
+    for (int i0 = lo; i0 < hi; i0 += 32 * kSortTile) {
+      load_tile(i0);
+#pragma unroll
+      for (int u = 0; u < kSortTile; ++u) {
+        const bool in = i0 + u * 32 + lane < hi;
+        const unsigned live = __ballot_sync(0xffffffffu, in);
+        if (in) {
+          const int d = (pair[u].x >> shift) & (digits - 1);
+          const unsigned same = __match_any_sync(live, d);
+          if ((same & ((1u << lane) - 1)) == 0) mine[d] += __popc(same);
+        }
+        __syncwarp();
+      }
     }
     __syncthreads();
     int sum = 0;
@@ -107,61 +151,53 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_ids_kernel(SortArgs s) {
     __syncthreads();
     if (tid < digits) base[tid] = scan - all + (warp ? warp_sums[warp - 1] : 0) + before;
     __syncthreads();
-    for (int i0 = lo; i0 < hi; i0 += 32) {
-      const int i = i0 + lane;
-      const unsigned live = __ballot_sync(0xffffffffu, i < hi);
-      int2 pair;
-      unsigned same = 0;
-      int d = 0, at = 0;
-      if (i < hi) {
-        pair = sort_load(s, src, p, i);
-        d = (pair.x >> shift) & (digits - 1);
-        same = __match_any_sync(live, d);
-        const unsigned below = same & ((1u << lane) - 1);
-        at = base[d] + mine[d] + __popc(below);
-        dst[at] = pair;
+    for (int i0 = lo; i0 < hi; i0 += 32 * kSortTile) {
+      if (hi - lo > 32 * kSortTile) load_tile(i0);                 // else the tile is still in the registers
+#pragma unroll
+      for (int u = 0; u < kSortTile; ++u) {
+        const bool in = i0 + u * 32 + lane < hi;
+        const unsigned live = __ballot_sync(0xffffffffu, in);
+        unsigned same = 0;
+        int d = 0;
+        if (in) {
+          d = (pair[u].x >> shift) & (digits - 1);
+          same = __match_any_sync(live, d);
+          dst[base[d] + mine[d] + __popc(same & ((1u << lane) - 1))] = pair[u];
+        }
+        __syncwarp();
+        if (in && (same & ((1u << lane) - 1)) == 0) mine[d] += __popc(same);
+        __syncwarp();
       }
-      __syncwarp();
-      if (i < hi && (same & ((1u << lane) - 1)) == 0) mine[d] += __popc(same);
-      __syncwarp();
     }
     cluster.sync();                                                // pairs written, totals read
-  }
-}
-
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&f)[8]) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = __uint_as_float(w[i] << 16);
-    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
 }
 
 struct GradArgs {
   const int2* pairs;          // [T] sorted
   const __nv_bfloat16* dout;  // [T, D]
-  float* partial;             // [2 * chunks, D]: sum of a run that came in, sum of a run that begins and goes on
+  float* partial;             // [2 * chunks, D]: sum of a long run that came in, of one that begins and goes on
+  int2* long_runs;            // [chunks]: chunk where it begins, chunk where it ends
+  int* n_long;
   void* grad;                 // [V, D]
   int T, V, D, chunk;
   float scale;
   int vec;                    // grad is 16-byte aligned (a view into a flat buffer may not be)
 };
 
-// One row of the table is written by exactly one thread per column.
+// One row of the table is written by exactly one thread per column. The fp32 buffer is added to by a reduction without
+// a return value: nothing waits for the old value, and with one addition per element the order cannot matter.
 __device__ __forceinline__ void store_row(float* dst, const float (&v)[8], float scale, int vec) {
   if (!vec) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) dst[e] += v[e] * scale;
     return;
   }
-  float4* p = reinterpret_cast<float4*>(dst);
-  float4 a = p[0], b = p[1];
-  a.x += v[0] * scale; a.y += v[1] * scale; a.z += v[2] * scale; a.w += v[3] * scale;
-  b.x += v[4] * scale; b.y += v[5] * scale; b.z += v[6] * scale; b.w += v[7] * scale;
-  p[0] = a;
-  p[1] = b;
+#pragma unroll
+  for (int h = 0; h < 8; h += 4)
+    asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(dst + h), "f"(v[h] * scale), "f"(v[h + 1] * scale),
+                 "f"(v[h + 2] * scale), "f"(v[h + 3] * scale)
+                 : "memory");
 }
 __device__ __forceinline__ void store_row(__nv_bfloat16* dst, const float (&v)[8], float scale, int vec) {
   if (!vec) {
@@ -177,36 +213,68 @@ __device__ __forceinline__ void store_row(__nv_bfloat16* dst, const float (&v)[8
 }
 
 constexpr int kMaxChunk = 32;
+constexpr int kMinChunk = 4;
 
-// Block (chunk, column tile); a thread owns 8 columns.
+// Block (chunk, column tile); a thread owns 8 columns. A run that crosses into the next chunk and ends there belongs to
+// the chunk where it begins; one that covers a whole chunk or more is long.
 template <typename GT>
-__global__ void sum_runs_kernel(GradArgs g) {
-  __shared__ int2 sh[kMaxChunk + 2];                               // with the neighbours on both sides
-  const int lo = blockIdx.x * g.chunk, n = min(g.chunk, g.T - lo);
-  for (int i = threadIdx.x; i < n + 2; i += blockDim.x) {
-    const int at = lo - 1 + i;
-    sh[i] = (at >= 0 && at < g.T) ? g.pairs[at] : make_int2(-1, 0);
+__global__ void __launch_bounds__(256) sum_runs_kernel(GradArgs g) {
+  __shared__ int2 window[3 * kMaxChunk + 2];                       // the chunk before with one more, this one, the next with one more
+  const int size = g.chunk, lo = blockIdx.x * size, n = min(size, g.T - lo);
+  for (int i = threadIdx.x; i < 3 * size + 2; i += blockDim.x) {
+    const int at = lo - size - 1 + i;
+    window[i] = (at >= 0 && at < g.T) ? g.pairs[at] : make_int2(-1, 0);
   }
   __syncthreads();
+  const int2* run = window + size + 1;                             // run[-size - 1 .. 2 size]
+  int begin = 0, end = n;
+  bool long_in = false, long_out = false;
+  const int head = run[0].x, tail = run[n - 1].x;
+  if (run[-1].x == head) {                                         // the first run came in
+    int e = 1;
+    while (e < n && run[e].x == head) ++e;
+    const bool whole = e == n && run[n].x == head;                 // and goes on
+    long_in = whole || run[-size - 1].x == head || (e == n && n == size);
+    if (!long_in) begin = e;
+  }
+  if (n == size && run[n].x == tail && !(run[-1].x == tail && head == tail)) {       // the last run begins here and goes on
+    int e = n + 1;
+    while (e < 2 * size && run[e].x == tail) ++e;
+    // it covers the next chunk
+    long_out = e == 2 * size;
+    if (!long_out) end = e;
+  }
   const int col = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
+  if (long_out && blockIdx.y == 0 && threadIdx.x == 0 && tail < g.V) {
+    int a = (lo / size) + 1, b = (g.T - 1) / size;                 // last chunk whose first position holds the id
+    while (a < b) {
+      const int mid = a + (b - a + 1) / 2;
+      if (g.pairs[mid * size].x == tail) a = mid; else b = mid - 1;
+    }
+    g.long_runs[atomicAdd(g.n_long, 1)] = make_int2(blockIdx.x, a);
+  }
   if (col >= g.D) return;
-  const int2* run = sh + 1;
   float acc[8] = {};
-  for (int i0 = 0; i0 < n; i0 += 4) {
-    float v[4][8];
+  for (int i0 = begin; i0 < end; i0 += 4) {
+    uint4 v[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (i0 + u < n) load8(g.dout + static_cast<long long>(run[i0 + u].y) * g.D + col, v[u]);
+      if (i0 + u < end)
+        v[u] = *reinterpret_cast<const uint4*>(g.dout + static_cast<long long>(run[i0 + u].y) * g.D + col);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int i = i0 + u;
-      if (i >= n) break;
+      if (i >= end) break;
       const int id = run[i].x;
       if (id >= g.V) return;                                       // only ids outside the vocabulary follow
+      const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] += v[u][e];
-      if (i + 1 < n && run[i + 1].x == id) continue;
-      const bool in = run[-1].x == id, on = run[n].x == id;        // came in from the left, goes on to the right
+      for (int e = 0; e < 4; ++e) {
+        acc[2 * e] += __uint_as_float(w[e] << 16);
+        acc[2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u);
+      }
+      if (i + 1 < end && run[i + 1].x == id) continue;
+      const bool in = long_in && id == head, on = long_out && id == tail;
       if (in || on) {
         float4* p = reinterpret_cast<float4*>(g.partial + (2ll * blockIdx.x + (in ? 0 : 1)) * g.D + col);
         p[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
@@ -220,52 +288,45 @@ __global__ void sum_runs_kernel(GradArgs g) {
   }
 }
 
-constexpr int kJoinGroups = 32;      // chunks of a run are summed in this many contiguous parts
+constexpr int kJoinGroups = 32;      // chunks of a long run are summed in this many contiguous parts
 
-// Block (chunk, 64 columns): 8 threads across, kJoinGroups parts. Only the chunk where a crossing run begins works.
+// Work item: (long run, 64 columns); 8 threads across, kJoinGroups parts.
 template <typename GT>
 __global__ void __launch_bounds__(8 * kJoinGroups) join_runs_kernel(GradArgs g) {
   __shared__ float sh[kJoinGroups][8][8];
-  const int last = min(g.T, (static_cast<int>(blockIdx.x) + 1) * g.chunk) - 1;
-  if (last + 1 >= g.T) return;
-  const int id = g.pairs[last].x;
-  if (id >= g.V || g.pairs[last + 1].x != id) return;
-  const int lo = blockIdx.x * g.chunk;
-  if (lo > 0 && g.pairs[lo - 1].x == id) return;                   // it began further left
-  int a = last + 1, b = g.T;                                       // first position behind the run
-  while (a < b) {
-    const int mid = a + (b - a) / 2;
-    if (g.pairs[mid].x == id) a = mid + 1; else b = mid;
-  }
-  const int end = (a - 1) / g.chunk;                               // the chunk that holds its last position
-  const int count = end - static_cast<int>(blockIdx.x) + 1;
+  const int tiles = (g.D + 63) / 64, items = *g.n_long * tiles;
   const int tx = threadIdx.x & 7, part = threadIdx.x >> 3;
-  const int col = blockIdx.y * 64 + tx * 8;
-  const int per = (count + kJoinGroups - 1) / kJoinGroups;
-  float acc[8] = {};
-  if (col < g.D) {
-    for (int i = part * per; i < min(count, (part + 1) * per); ++i) {
-      const float4* p = reinterpret_cast<const float4*>(
-          g.partial + (2ll * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * g.D + col);
-      const float4 x = p[0], y = p[1];
-      acc[0] += x.x; acc[1] += x.y; acc[2] += x.z; acc[3] += x.w;
-      acc[4] += y.x; acc[5] += y.y; acc[6] += y.z; acc[7] += y.w;
+  for (int item = blockIdx.x; item < items; item += gridDim.x) {
+    const int2 run = g.long_runs[item / tiles];
+    const int count = run.y - run.x + 1, col = (item % tiles) * 64 + tx * 8;
+    const int per = (count + kJoinGroups - 1) / kJoinGroups;
+    const int id = g.pairs[run.y * g.chunk].x;
+    float acc[8] = {};
+    if (col < g.D) {
+      for (int i = part * per; i < min(count, (part + 1) * per); ++i) {
+        const float4* p = reinterpret_cast<const float4*>(g.partial + (2ll * (run.x + i) + (i == 0 ? 1 : 0)) * g.D + col);
+        const float4 x = p[0], y = p[1];
+        acc[0] += x.x; acc[1] += x.y; acc[2] += x.z; acc[3] += x.w;
+        acc[4] += y.x; acc[5] += y.y; acc[6] += y.z; acc[7] += y.w;
+      }
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sh[part][tx][e] = acc[e];
+    __syncthreads();
+    if (part == 0 && col < g.D) {
+      for (int q = 1; q < kJoinGroups; ++q)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] += sh[q][tx][e];
+      store_row(static_cast<GT*>(g.grad) + static_cast<long long>(id) * g.D + col, acc, g.scale, g.vec);
+    }
+    __syncthreads();
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) sh[part][tx][e] = acc[e];
-  __syncthreads();
-  if (part != 0 || col >= g.D) return;
-  for (int q = 1; q < kJoinGroups; ++q)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] += sh[q][tx][e];
-  store_row(static_cast<GT*>(g.grad) + static_cast<long long>(id) * g.D + col, acc, g.scale, g.vec);
 }
 
 int chunk_of(int T) {
   // a few chunks per SM while there are few tokens, at most kMaxChunk positions
   const int c = (T + 4 * txh::sm_count() - 1) / (4 * txh::sm_count());
-  return c < 4 ? 4 : (c > kMaxChunk ? kMaxChunk : c);
+  return c < kMinChunk ? kMinChunk : (c > kMaxChunk ? kMaxChunk : c);
 }
 
 template <typename GT>
@@ -273,16 +334,20 @@ int launch_grad(const GradArgs& g, cudaStream_t s) {
   const int chunks = (g.T + g.chunk - 1) / g.chunk;
   const int threads = min(256, (g.D / 8 + 31) / 32 * 32);
   sum_runs_kernel<GT><<<dim3(chunks, (g.D / 8 + threads - 1) / threads), threads, 0, s>>>(g);
-  join_runs_kernel<GT><<<dim3(chunks, (g.D + 63) / 64), 8 * kJoinGroups, 0, s>>>(g);
+  if (chunks < 2) return cudaGetLastError() == cudaSuccess ? 0 : 400;        // a long run covers a chunk behind its first
+  const long long most = static_cast<long long>(chunks) * ((g.D + 63) / 64);
+  const int grid = static_cast<int>(min(most, 4ll * txh::sm_count()));
+  join_runs_kernel<GT><<<grid, 8 * kJoinGroups, 0, s>>>(g);
   return cudaGetLastError() == cudaSuccess ? 0 : 400;
 }
 
 }  // namespace
 
-// Bytes of workspace for T tokens of D columns (16-byte aligned).
+// Bytes of workspace for T tokens of D columns (16-byte aligned): two lists of pairs, the list of long runs and its
+// length, the partial sums.
 extern "C" long long tx_embedding_grad_workspace(int T, int D) {
   const long long chunks = (T + chunk_of(T) - 1) / chunk_of(T);
-  return 2 * ((8ll * T + 15) / 16 * 16) + 2 * chunks * D * 4;
+  return 2 * ((8ll * T + 15) / 16 * 16) + (8 * chunks + 15) / 16 * 16 + 16 + 2 * chunks * D * 4;
 }
 
 // ids int64 or int32 [T], dout bf16 [T, D] with D a multiple of 8. grad_bf16 == 0: grad is fp32 and added to; else it
@@ -291,9 +356,19 @@ extern "C" int tx_embedding_grad(const void* ids, int ids64, const void* dout, v
                                  int V, float scale, void* workspace, cudaStream_t s) {
   if (D % 8 || D <= 0 || V <= 0 || V > 0x3fffffff) return 1;
   if (T <= 0) return 0;
+  const long long chunks = (T + chunk_of(T) - 1) / chunk_of(T);
   int2* a = static_cast<int2*>(workspace);
   int2* b = a + (T + 1ll) / 2 * 2;
-  SortArgs so{ids, ids64, T, V, 1, 1, a, b};
+  int2* long_runs = b + (T + 1ll) / 2 * 2;
+  int* n_long = reinterpret_cast<int*>(long_runs + (chunks + 1) / 2 * 2);
+  SortArgs so{ids, ids64, T, V, 1, 1, a, b, n_long};
+  const GradArgs g{a, static_cast<const __nv_bfloat16*>(dout), reinterpret_cast<float*>(n_long + 4), long_runs, n_long,
+                   grad, T, V, D, chunk_of(T), scale, reinterpret_cast<uintptr_t>(grad) % 16 == 0};
+  if (T <= kCountTokens) {
+    const int per = kCountThreads / kCountPer;
+    count_sort_kernel<<<(T + per - 1) / per, kCountThreads, 0, s>>>(so);
+    return grad_bf16 ? launch_grad<__nv_bfloat16>(g, s) : launch_grad<float>(g, s);
+  }
   int bits = 1;
   while ((V >> bits) != 0) ++bits;                                 // V itself marks ids outside
   so.passes = (bits + 9) / 10;
@@ -305,7 +380,7 @@ extern "C" int tx_embedding_grad(const void* ids, int ids64, const void* dout, v
                              kSortWarps * kMaxDigits * 4) != cudaSuccess) return 401;
     flag.cur() = true;
   }
-  const int blocks = T <= 4096 ? 1 : kSortCluster;
+  const int blocks = kSortCluster;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(blocks);
   cfg.blockDim = dim3(kSortThreads);
@@ -319,7 +394,5 @@ extern "C" int tx_embedding_grad(const void* ids, int ids64, const void* dout, v
   cfg.attrs = at;
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, sort_ids_kernel, so) != cudaSuccess) return 402;
-  const GradArgs g{a, static_cast<const __nv_bfloat16*>(dout), reinterpret_cast<float*>(b + (T + 1ll) / 2 * 2), grad, T,
-                   V, D, chunk_of(T), scale, reinterpret_cast<uintptr_t>(grad) % 16 == 0};
   return grad_bf16 ? launch_grad<__nv_bfloat16>(g, s) : launch_grad<float>(g, s);
 }

@@ -27,7 +27,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kUnroll = 4;                    // 16-byte vectors a thread has in flight
 constexpr int kMaxTop = 256;                  // longest list of alternatives
 constexpr int kMaxList = 1024;                // longest teacher's list
-constexpr int kCand = 2048;                   // candidate vectors of a block
+constexpr int kCand = 24;                     // candidate vectors of a thread
 constexpr int kKeys = 2048;                   // candidate elements; a cluster's lists fit: kMaxSplit * kMaxTop
 constexpr int kBins = 256;
 constexpr int kMaxSplit = 8;                  // blocks (one cluster) a row is spread over when there are few rows
@@ -134,6 +134,8 @@ __device__ __forceinline__ int misalign(const T* p) {
 template <typename T>
 __device__ __forceinline__ uint4 load_vec(const T* row, int j, int lo, int hi, bool aligned) {
   if (aligned && j >= lo && j + kVec<T> <= hi) return *reinterpret_cast<const uint4*>(row + j);
+  const uint32_t none = sizeof(T) == 2 ? 0xff80ff80u : 0xff800000u;
+  if (j >= hi) return make_uint4(none, none, none, none);
   float z[kVec<T>];
 #pragma unroll
   for (int i = 0; i < kVec<T>; ++i) z[i] = (j + i >= lo && j + i < hi) ? to_f(row[j + i]) : -INFINITY;
@@ -231,22 +233,38 @@ __device__ __forceinline__ void stat_merge(Stat& a, Stat b, float c, float c2) {
   a.t += b.t;
 }
 
-// Leaves the block's statistics in every thread. `sh` holds kWarps entries.
+__device__ __forceinline__ float warp_max_of(float v) {
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float warp_sum_of(float v) {
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Leaves the block's statistics in every thread: the maximum first, then sums relative to it. `sh` holds kWarps entries.
 template <int X>
 __device__ __forceinline__ Stat stat_block(Stat a, Stat* sh, float c, float c2) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Stat b;
-    b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-    b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-    b.t = __shfl_xor_sync(0xffffffffu, a.t, o);
-    stat_merge<X>(a, b, c, c2);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float wm = warp_max_of(a.m);
+  __syncthreads();
+  if (lane == 0) sh[warp].m = wm;
+  __syncthreads();
+  float m = sh[0].m;
+  for (int w = 1; w < kWarps; ++w) m = fmaxf(m, sh[w].m);
+  if (a.m != m) stat_raise<X>(a, m, c, c2);
+  a.s = warp_sum_of(a.s);
+  if (X != kNone) a.t = warp_sum_of(a.t);
+  if (lane == 0) {
+    sh[warp].s = a.s;
+    sh[warp].t = a.t;
   }
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = a;
-  __syncthreads();
-  a = sh[0];
-  for (int w = 1; w < kWarps; ++w) stat_merge<X>(a, sh[w], c, c2);
+  a.s = a.t = 0.f;
+  for (int w = 0; w < kWarps; ++w) {
+    a.s += sh[w].s;
+    if (X != kNone) a.t += sh[w].t;
+  }
   return a;
 }
 
@@ -351,9 +369,21 @@ __device__ __forceinline__ unsigned long long shfl_key(unsigned long long k, int
   return (static_cast<unsigned long long>(hi) << 32) | lo;
 }
 
-// Sorts n keys in shared memory from high to low (bitonic; slots n .. P-1 are filled with 0, P the next power of 2).
-// All threads call it. Up to one key per thread stays in a register and strides below a warp are shuffles.
+// Sorts n keys (all different) in shared memory from high to low. All threads call it. Short lists: two threads count
+// how many keys are above theirs. Longer ones: bitonic (slots n .. P-1 are filled with 0, P the next power of 2); up to
+// one key per thread stays in a register and strides below a warp are shuffles.
 __device__ __forceinline__ void sort_keys(unsigned long long* keys, int n) {
+  if (n <= kThreads / 2) {
+    const int i = threadIdx.x >> 1;
+    const unsigned long long key = i < n ? keys[i] : 0;
+    int above = 0;
+    for (int j = threadIdx.x & 1; j < n; j += 2) above += keys[j] > key;
+    above += __shfl_xor_sync(0xffffffffu, above, 1);
+    __syncthreads();
+    if (i < n && (threadIdx.x & 1) == 0) keys[above] = key;
+    __syncthreads();
+    return;
+  }
   int P = 32;
   while (P < n) P <<= 1;
   const int tid = threadIdx.x;
@@ -417,23 +447,25 @@ struct TopArgs {
 // A candidate is a 16-byte vector whose largest element is not below a threshold that k elements of the block's part
 // are known to reach. The first threshold comes from the first iteration: the smallest over the warps of the
 // ceil(k / warps)-th largest of a warp's per-thread maxima (of the warps that have a whole vector per thread). From
-// then on the maxima of candidates are counted in bins of equal width above it, and every 32 candidates the threshold
-// moves up to half a bin below the lowest bin that k of them reach. Bin numbers and that edge are computed with
-// monotone roundings, so an element of such a bin is never below the edge. At the end the candidates are read again
-// (from L2) and their elements that reach the last threshold are sorted: little more than k.
+// then on the maxima of candidates are counted in bins of equal width above it, and in every iteration one warp moves
+// the threshold up to a bin below the lowest bin that k of them reach. Bin numbers (rounded to the nearest) and that
+// edge are computed with monotone roundings, so an element of such a bin is never below the edge. Every thread keeps
+// a list of its candidates (a few); at the end those that still reach the threshold are read again (from L2) and
+// their elements that do are sorted: little more than k.
 struct Select {
   unsigned long long keys[kKeys];
-  int cand[kCand];
+  uint32_t cand[kCand][kThreads];        // largest element as bf16, rounded up | number of the thread's vector
   int bins[kBins];
-  int count, n_keys;
+  int n_keys;
   float thr;
   float warp_nth[kWarps], warp_max[kWarps];
   Stat stat[kWarps];
   Stat part;                   // this block's statistics, read by the cluster's first block
 };
 
+// The nearest bin, read from the low bits of a float that has no fraction left. NaN: the last one.
 __device__ __forceinline__ int bin_of(float x, float thr0, float inv_width) {
-  return static_cast<int>(fminf((x - thr0) * inv_width, static_cast<float>(kBins - 1)));     // NaN: the last one
+  return __float_as_int(fminf((x - thr0) * inv_width, static_cast<float>(kBins - 1)) + 8388608.f) & (kBins - 1);
 }
 
 // Lowest bin that k counted candidates reach or pass (0 while there are fewer), by one warp.
@@ -512,7 +544,7 @@ __global__ void __launch_bounds__(kThreads) top_fwd_kernel(TopArgs a) {
   const int lo = part.x, hi = part.y;
   constexpr int N = kVec<LT>, chunk = kChunk<LT>;
   for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0;
-  if (tid == 0) s.count = s.n_keys = 0;
+  if (tid == 0) s.n_keys = 0;
   // ---- first iteration: the first threshold
   const int base = lo - misalign(x + lo);
   const int j0 = base + tid * N;
@@ -558,25 +590,26 @@ __global__ void __launch_bounds__(kThreads) top_fwd_kernel(TopArgs a) {
   float thr = thr0;
   __syncthreads();
   volatile float* shared_thr = &s.thr;
-  auto offer = [&](int j, const float (&top)[kUnroll]) {
-    bool full = false;
+  int n = 0;                                       // candidates of this thread
+  auto offer = [&](int at, const float (&top)[kUnroll]) {      // `at`: number of the first of the thread's vectors
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) {
-      if (!(top[i] < thr) && j + i * chunk < hi && j + i * chunk + N > lo) {
-        const int pos = atomicAdd(&s.count, 1);
-        if (pos < kCand) s.cand[pos] = j + i * chunk;
+      if (!(top[i] < thr)) {
+        const uint32_t bits = __float_as_uint(top[i]);
+        const uint32_t up = top[i] >= 0.f ? (bits + 0xffffu) & 0xffff0000u : bits & 0xffff0000u;
+        if (n < kCand) s.cand[n][tid] = up | static_cast<uint32_t>(at + i);
+        ++n;
         atomicAdd(&s.bins[bin_of(top[i], thr0, inv_width)], 1);
-        full |= (pos & 31) == 31;
       }
     }
-    if (__any_sync(0xffffffffu, full)) {
+    if (((at / kUnroll) & (kWarps - 1)) == tid >> 5) {
       const int b = cut_bin(s.bins, k);
-      const float t = fmaf(b - 0.5f, width, thr0);
-      if (lane == 0 && b > 0 && t > *shared_thr) *shared_thr = t;
+      const float t = fmaf(b - 1.f, width, thr0);
+      if (lane == 0 && b > 1 && t > *shared_thr) *shared_thr = t;
       __syncwarp();
     }
   };
-  offer(j0, vm);
+  offer(0, vm);
   each_vec(x, base + kUnroll * chunk, lo, hi, [&](int j, const uint4 (&u)[kUnroll]) {
     float top[kUnroll];
 #pragma unroll
@@ -584,17 +617,17 @@ __global__ void __launch_bounds__(kThreads) top_fwd_kernel(TopArgs a) {
     thr = *shared_thr;
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) acc.template push<LT>(u[i], top[i], c, 0.f);
-    offer(j, top);
+    offer((j - j0) / chunk, top);
   });
-  __syncthreads();
-  // ---- the block's k best, sorted
-  const int n = s.count;
-  bool fits = n <= kCand;
+  // ---- the block's k best, sorted: every thread looks at its own candidates again
+  bool fits = !__syncthreads_or(n > kCand || hi - base > 65536 * chunk);
   if (fits) {
     const int b = cut_bin(s.bins, k);
-    thr = b > 0 ? fmaxf(*shared_thr, fmaf(b - 0.5f, width, thr0)) : *shared_thr;
-    for (int i = tid; i < n; i += kThreads) {
-      const int j = s.cand[i];
+    thr = b > 1 ? fmaxf(*shared_thr, fmaf(b - 1.f, width, thr0)) : *shared_thr;
+    for (int i = 0; i < n; ++i) {
+      const uint32_t word = s.cand[i][tid];
+      if (__uint_as_float(word & 0xffff0000u) < thr) continue;
+      const int j = j0 + static_cast<int>(word & 0xffffu) * chunk;
       float z[N];
       unpack(load_vec(x, j, lo, hi, true), z);
 #pragma unroll
@@ -669,15 +702,6 @@ struct DistillArgs {
 // Per row: m, ln s at temperature 1, ln s at the temperature, the list's teacher mass (full); then for a list that is
 // normalised over itself the teacher's maximum and ln sum, the student's maximum and ln sum (+inf: nothing usable).
 constexpr int kDistillStats = 8;
-
-__device__ __forceinline__ float warp_max_of(float v) {
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-__device__ __forceinline__ float warp_sum_of(float v) {
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
 
 // The list of one row, by one warp; writes the row's outputs. ls1, ls2: ln s at temperature 1 and at the temperature.
 template <typename LT>
