@@ -112,17 +112,29 @@ __device__ __forceinline__ uint4 pack(const float (&z)[8]) {
   for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(z[2 * i], z[2 * i + 1]);
   return u;
 }
+// Maxima of vectors, kept packed for bf16: `scalar` is the one number.
 template <typename T>
-__device__ __forceinline__ float vec_max(uint4 u);
+struct Top;
 template <>
-__device__ __forceinline__ float vec_max<float>(uint4 u) {
-  return max_nan(max_nan(__uint_as_float(u.x), __uint_as_float(u.y)), max_nan(__uint_as_float(u.z), __uint_as_float(u.w)));
-}
+struct Top<float> {
+  float v;
+  __device__ __forceinline__ static Top of(uint4 u) {
+    return Top{max_nan(max_nan(__uint_as_float(u.x), __uint_as_float(u.y)), max_nan(__uint_as_float(u.z), __uint_as_float(u.w)))};
+  }
+  __device__ __forceinline__ static Top max(Top a, Top b) { return Top{max_nan(a.v, b.v)}; }
+  __device__ __forceinline__ float scalar() const { return v; }
+};
 template <>
-__device__ __forceinline__ float vec_max<__nv_bfloat16>(uint4 u) {
-  const uint32_t m = max_nan_bf16x2(max_nan_bf16x2(u.x, u.y), max_nan_bf16x2(u.z, u.w));
-  return max_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
-}
+struct Top<__nv_bfloat16> {
+  uint32_t v;
+  __device__ __forceinline__ static Top of(uint4 u) {
+    return Top{max_nan_bf16x2(max_nan_bf16x2(u.x, u.y), max_nan_bf16x2(u.z, u.w))};
+  }
+  __device__ __forceinline__ static Top max(Top a, Top b) { return Top{max_nan_bf16x2(a.v, b.v)}; }
+  __device__ __forceinline__ float scalar() const {
+    return max_nan(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  }
+};
 
 // How many elements an address lies behind the last 16-byte boundary.
 template <typename T>
@@ -187,9 +199,9 @@ struct Acc {
     m = v;
     M = n;
   }
+  // Adds a vector none of whose elements is above m.
   template <typename LT>
-  __device__ __forceinline__ void push(uint4 u, float vm, float c, float c2) {
-    if (vm > m) raise(vm, c, c2);
+  __device__ __forceinline__ void push(uint4 u, float c, float c2) {
     float z[kVec<LT>];
     unpack(u, z);
     const f32x2 cc = pack2(c, c), mm = pack2(-M, -M);
@@ -328,7 +340,8 @@ __device__ __forceinline__ Row finish_row(const Stat& a, const LT* x, int V, Sta
   return r;
 }
 
-// All 16-byte vectors of columns [lo, hi), kUnroll per thread at a time: fn(first element, vectors).
+// The block's vectors of columns [lo, hi) from element `from` on, kUnroll per thread at a time: fn(first element of the
+// thread, vectors, how many of them begin inside; the last may reach out and is then filled with -inf).
 template <typename LT, typename Fn>
 __device__ __forceinline__ void each_vec(const LT* x, int from, int lo, int hi, Fn fn) {
   constexpr int step = kUnroll * kChunk<LT>;
@@ -338,14 +351,36 @@ __device__ __forceinline__ void each_vec(const LT* x, int from, int lo, int hi, 
     const int j = at + threadIdx.x * kVec<LT>;
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) u[i] = *reinterpret_cast<const uint4*>(x + j + i * kChunk<LT>);
-    fn(j, u);
+    fn(j, u, kUnroll);
   }
   for (; at < hi; at += step) {
-    const int j = at + threadIdx.x * kVec<LT>;
+    const int j = at + threadIdx.x * kVec<LT>, n = min(kUnroll, (hi - at + kChunk<LT> - 1) / kChunk<LT>);
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) u[i] = load_vec(x, j + i * kChunk<LT>, lo, hi, true);
-    fn(j, u);
+    for (int i = 0; i < kUnroll; ++i)
+      if (i < n) u[i] = load_vec(x, j + i * kChunk<LT>, lo, hi, true);
+    fn(j, u, n);
   }
+}
+
+// Maxima of n vectors, one by one and together, and their sums.
+template <typename LT, int X>
+__device__ __forceinline__ float take_vecs(Acc<X>& acc, const uint4 (&u)[kUnroll], int n, Top<LT> (&top)[kUnroll], float c,
+                                           float c2) {
+  top[0] = Top<LT>::of(u[0]);
+  Top<LT> all = top[0];
+#pragma unroll
+  for (int i = 1; i < kUnroll; ++i) {
+    if (i < n) {
+      top[i] = Top<LT>::of(u[i]);
+      all = Top<LT>::max(all, top[i]);
+    }
+  }
+  const float most = all.scalar();
+  if (most > acc.m) acc.raise(most, c, c2);
+#pragma unroll
+  for (int i = 0; i < kUnroll; ++i)
+    if (i < n) acc.template push<LT>(u[i], c, c2);
+  return most;
 }
 
 // ---- keys of candidates --------------------------------------------------------------------------------
@@ -549,14 +584,17 @@ __global__ void __launch_bounds__(kThreads) top_fwd_kernel(TopArgs a) {
   const int base = lo - misalign(x + lo);
   const int j0 = base + tid * N;
   Acc<X> acc;
-  uint4 first[kUnroll];
-  float vm[kUnroll];
+  uint4 u0[kUnroll];
+  Top<LT> top0[kUnroll];
+  const int n0 = min(kUnroll, (hi - base + chunk - 1) / chunk);
 #pragma unroll
-  for (int i = 0; i < kUnroll; ++i) first[i] = load_vec(x, j0 + i * chunk, lo, hi, true);
+  for (int i = 0; i < kUnroll; ++i)
+    if (i < n0) u0[i] = load_vec(x, j0 + i * chunk, lo, hi, true);
+  Top<LT> all0 = Top<LT>::of(u0[0]);
 #pragma unroll
-  for (int i = 0; i < kUnroll; ++i) vm[i] = vec_max<LT>(first[i]);
-  float v = max_nan(max_nan(vm[0], vm[1]), max_nan(vm[2], vm[3]));
-  static_assert(kUnroll == 4, "");
+  for (int i = 1; i < kUnroll; ++i)
+    if (i < n0) all0 = Top<LT>::max(all0, Top<LT>::of(u0[i]));
+  float v = all0.scalar();
   v = v != v ? INFINITY : v;
   for (int size = 2; size <= 32; size <<= 1)
     for (int stride = size >> 1; stride > 0; stride >>= 1) {
@@ -573,8 +611,7 @@ __global__ void __launch_bounds__(kThreads) top_fwd_kernel(TopArgs a) {
     s.warp_max[tid >> 5] = warp_max;
   }
   acc.init(warp_max, c, 0.f);                                          // later maxima are rare
-#pragma unroll
-  for (int i = 0; i < kUnroll; ++i) acc.template push<LT>(first[i], vm[i], c, 0.f);
+  const float most0 = take_vecs<LT, X>(acc, u0, n0, top0, c, 0.f);
   __syncthreads();
   float thr0 = INFINITY, most = s.warp_max[0];
   for (int w = 0; w < kWarps; ++w) {
@@ -591,15 +628,19 @@ __global__ void __launch_bounds__(kThreads) top_fwd_kernel(TopArgs a) {
   __syncthreads();
   volatile float* shared_thr = &s.thr;
   int n = 0;                                       // candidates of this thread
-  auto offer = [&](int at, const float (&top)[kUnroll]) {      // `at`: number of the first of the thread's vectors
+  auto offer = [&](int at, const Top<LT> (&top)[kUnroll], int count, float all) {   // `at`: number of the first vector
+    if (!(all < thr)) {
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      if (!(top[i] < thr)) {
-        const uint32_t bits = __float_as_uint(top[i]);
-        const uint32_t up = top[i] >= 0.f ? (bits + 0xffffu) & 0xffff0000u : bits & 0xffff0000u;
-        if (n < kCand) s.cand[n][tid] = up | static_cast<uint32_t>(at + i);
-        ++n;
-        atomicAdd(&s.bins[bin_of(top[i], thr0, inv_width)], 1);
+      for (int i = 0; i < kUnroll; ++i) {
+        if (i >= count) break;
+        const float t = top[i].scalar();
+        if (!(t < thr)) {
+          const uint32_t bits = __float_as_uint(t);
+          const uint32_t up = t >= 0.f ? (bits + 0xffffu) & 0xffff0000u : bits & 0xffff0000u;
+          if (n < kCand) s.cand[n][tid] = up | static_cast<uint32_t>(at + i);
+          ++n;
+          atomicAdd(&s.bins[bin_of(t, thr0, inv_width)], 1);
+        }
       }
     }
     if (((at / kUnroll) & (kWarps - 1)) == tid >> 5) {
@@ -609,21 +650,23 @@ __global__ void __launch_bounds__(kThreads) top_fwd_kernel(TopArgs a) {
       __syncwarp();
     }
   };
-  offer(0, vm);
-  each_vec(x, base + kUnroll * chunk, lo, hi, [&](int j, const uint4 (&u)[kUnroll]) {
-    float top[kUnroll];
-#pragma unroll
-    for (int i = 0; i < kUnroll; ++i) top[i] = vec_max<LT>(u[i]);
+  offer(0, top0, n0, most0);
+  each_vec(x, base + kUnroll * chunk, lo, hi, [&](int j, const uint4 (&u)[kUnroll], int count) {
+    Top<LT> top[kUnroll];
+    const float all = take_vecs<LT, X>(acc, u, count, top, c, 0.f);
     thr = *shared_thr;
-#pragma unroll
-    for (int i = 0; i < kUnroll; ++i) acc.template push<LT>(u[i], top[i], c, 0.f);
-    offer((j - j0) / chunk, top);
+    offer((j - j0) / chunk, top, count, all);
   });
   // ---- the block's k best, sorted: every thread looks at its own candidates again
   bool fits = !__syncthreads_or(n > kCand || hi - base > 65536 * chunk);
   if (fits) {
-    const int b = cut_bin(s.bins, k);
-    thr = b > 1 ? fmaxf(*shared_thr, fmaf(b - 1.f, width, thr0)) : *shared_thr;
+    if (tid < 32) {
+      const int b = cut_bin(s.bins, k);
+      const float t = fmaf(b - 1.f, width, thr0);
+      if (tid == 0 && b > 1 && t > *shared_thr) *shared_thr = t;
+    }
+    __syncthreads();
+    thr = *shared_thr;
     for (int i = 0; i < n; ++i) {
       const uint32_t word = s.cand[i][tid];
       if (__uint_as_float(word & 0xffff0000u) < thr) continue;
@@ -786,16 +829,17 @@ __global__ void __launch_bounds__(kThreads) distill_fwd_kernel(DistillArgs a, fl
   Acc<X> acc;
   acc.init(-INFINITY, c1, c2);
   bool fresh = true;
-  each_vec(x, lo - misalign(x + lo), lo, hi, [&](int, const uint4 (&u)[kUnroll]) {
-    float top[kUnroll];
-#pragma unroll
-    for (int i = 0; i < kUnroll; ++i) top[i] = vec_max<LT>(u[i]);
+  each_vec(x, lo - misalign(x + lo), lo, hi, [&](int, const uint4 (&u)[kUnroll], int count) {
+    Top<LT> top[kUnroll];
     if (fresh) {                         // begin with the warp's maximum: later ones are rare
-      acc.init(warp_max_of(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))), c1, c2);
+      Top<LT> all = Top<LT>::of(u[0]);
+#pragma unroll
+      for (int i = 1; i < kUnroll; ++i)
+        if (i < count) all = Top<LT>::max(all, Top<LT>::of(u[i]));
+      acc.init(warp_max_of(all.scalar()), c1, c2);
       fresh = false;
     }
-#pragma unroll
-    for (int i = 0; i < kUnroll; ++i) acc.template push<LT>(u[i], top[i], c1, c2);
+    take_vecs<LT, X>(acc, u, count, top, c1, c2);
   });
   Stat st = stat_block<X>(acc.stat(), sh_stat, c1, c2);
   if (blocks > 1) {
