@@ -27,8 +27,9 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kUnroll = 4;                    // 16-byte vectors a thread has in flight
 constexpr int kMaxTop = 256;                  // longest list of alternatives
 constexpr int kMaxList = 1024;                // longest teacher's list
-constexpr int kCand = 24;                     // candidate vectors of a thread
-constexpr int kKeys = 2048;                   // candidate elements; a cluster's lists fit: kMaxSplit * kMaxTop
+constexpr int kCand = 2560;                   // candidates of a block
+constexpr int kKept = 1024;                   // of which this many may reach the last threshold
+constexpr int kKeys = 2048;                   // elements that do; a cluster's lists fit: kMaxSplit * kMaxTop
 constexpr int kBins = 256;
 constexpr int kMaxSplit = 8;                  // blocks (one cluster) a row is spread over when there are few rows
 constexpr int kMinPart = 4096;                // columns of such a part at least
@@ -362,25 +363,23 @@ __device__ __forceinline__ void each_vec(const LT* x, int from, int lo, int hi, 
   }
 }
 
-// Maxima of n vectors, one by one and together, and their sums.
-template <typename LT, int X>
-__device__ __forceinline__ float take_vecs(Acc<X>& acc, const uint4 (&u)[kUnroll], int n, Top<LT> (&top)[kUnroll], float c,
-                                           float c2) {
-  top[0] = Top<LT>::of(u[0]);
-  Top<LT> all = top[0];
+// The maximum of n vectors.
+template <typename LT>
+__device__ __forceinline__ float max_vecs(const uint4 (&u)[kUnroll], int n) {
+  Top<LT> all = Top<LT>::of(u[0]);
 #pragma unroll
-  for (int i = 1; i < kUnroll; ++i) {
-    if (i < n) {
-      top[i] = Top<LT>::of(u[i]);
-      all = Top<LT>::max(all, top[i]);
-    }
-  }
-  const float most = all.scalar();
+  for (int i = 1; i < kUnroll; ++i)
+    if (i < n) all = Top<LT>::max(all, Top<LT>::of(u[i]));
+  return all.scalar();
+}
+
+// Adds n vectors of the given maximum.
+template <typename LT, int X>
+__device__ __forceinline__ void add_vecs(Acc<X>& acc, const uint4 (&u)[kUnroll], int n, float most, float c, float c2) {
   if (most > acc.m) acc.raise(most, c, c2);
 #pragma unroll
   for (int i = 0; i < kUnroll; ++i)
     if (i < n) acc.template push<LT>(u[i], c, c2);
-  return most;
 }
 
 // ---- keys of candidates --------------------------------------------------------------------------------
@@ -479,26 +478,27 @@ struct TopArgs {
 
 // Selection state of a block.
 //
-// A candidate is a 16-byte vector whose largest element is not below a threshold that k elements of the block's part
-// are known to reach. The first threshold comes from the first iteration: the smallest over the warps of the
-// ceil(k / warps)-th largest of a warp's per-thread maxima (of the warps that have a whole vector per thread). From
-// then on the maxima of candidates are counted in bins of equal width above it, and in every iteration one warp moves
-// the threshold up to a bin below the lowest bin that k of them reach. Bin numbers (rounded to the nearest) and that
-// edge are computed with monotone roundings, so an element of such a bin is never below the edge. Every thread keeps
-// a list of its candidates (a few); at the end those that still reach the threshold are read again (from L2) and
-// their elements that do are sorted: little more than k.
+// A candidate is what a thread takes in one iteration (kUnroll vectors), when its largest element is not below a
+// threshold that k elements of the block's part are known to reach. The first threshold comes from the first iteration:
+// the smallest over the warps of the ceil(k / warps)-th largest of a warp's per-thread maxima (of the warps that have a
+// whole vector per thread). From then on the maxima of candidates are counted in bins of equal width above it, and in
+// every iteration one warp moves the threshold up to a bin below the lowest bin that k of them reach. Bin numbers
+// (rounded to the nearest) and that edge are computed with monotone roundings, so an element of such a bin is never
+// below the edge. At the end the candidates that still reach the threshold are read again (from L2), a vector per
+// thread, and their elements that do are sorted: little more than k. Every step is dense over the block's threads: the
+// kernel is bound by the instructions it issues, not by the memory.
 struct Select {
   unsigned long long keys[kKeys];
-  uint32_t cand[kCand][kThreads];        // largest element as bf16, rounded up | number of the thread's vector
+  uint32_t cand[kCand];                  // largest element as bf16, rounded up | iteration * kThreads + thread
+  uint16_t kept[kKept];
   int bins[kBins];
-  int n_keys;
+  int count, n_kept, n_keys;
   float thr;
   float warp_nth[kWarps], warp_max[kWarps];
   Stat stat[kWarps];
   Stat part;                   // this block's statistics, read by the cluster's first block
 };
 
-// The nearest bin, read from the low bits of a float that has no fraction left. NaN: the last one.
 __device__ __forceinline__ int bin_of(float x, float thr0, float inv_width) {
   return __float_as_int(fminf((x - thr0) * inv_width, static_cast<float>(kBins - 1)) + 8388608.f) & (kBins - 1);
 }
@@ -536,6 +536,7 @@ __device__ __forceinline__ int cut_bin(const volatile int* bins, int k) {
 template <typename LT>
 __device__ __noinline__ void select_in_order(Select& s, const LT* x, int lo, int hi, int k) {
   constexpr int limit = kKeys - kThreads;
+  static_assert(limit > kMaxTop, "");
   float thr = -INFINITY;
   bool any = true;                                   // no threshold yet
   __syncthreads();
@@ -565,36 +566,23 @@ __device__ __noinline__ void select_in_order(Select& s, const LT* x, int lo, int
   sort_keys(s.keys, s.n_keys);
 }
 
+// The k best of columns [lo, hi) into s.keys, sorted, and the statistics of the part. `base`: the first column of the
+// first vector.
 template <typename LT, int X>
-__global__ void __launch_bounds__(kThreads) top_fwd_kernel(TopArgs a) {
-  extern __shared__ unsigned char shared[];
-  Select& s = *reinterpret_cast<Select*>(shared);
-  cg::cluster_group cluster = cg::this_cluster();
-  const int blocks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
-  const int row = blockIdx.x / blocks, tid = threadIdx.x, lane = tid & 31;
-  const LT* x = static_cast<const LT*>(a.logits) + static_cast<long long>(row) * a.ld;
-  const float c = a.inv_temp * kLog2e;
-  const int k = a.k;
-  const int2 part = part_of(a.V, rank, blocks);
-  const int lo = part.x, hi = part.y;
+__device__ __forceinline__ Stat top_of_part(Select& s, const LT* x, int base, int lo, int hi, int k, float c) {
   constexpr int N = kVec<LT>, chunk = kChunk<LT>;
+  const int tid = threadIdx.x, lane = tid & 31;
   for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0;
-  if (tid == 0) s.n_keys = 0;
+  if (tid == 0) s.count = s.n_kept = s.n_keys = 0;
   // ---- first iteration: the first threshold
-  const int base = lo - misalign(x + lo);
-  const int j0 = base + tid * N;
   Acc<X> acc;
-  uint4 u0[kUnroll];
-  Top<LT> top0[kUnroll];
-  const int n0 = min(kUnroll, (hi - base + chunk - 1) / chunk);
+  uint4 u[kUnroll];
+  const int count = min(kUnroll, (hi - base + chunk - 1) / chunk);
 #pragma unroll
   for (int i = 0; i < kUnroll; ++i)
-    if (i < n0) u0[i] = load_vec(x, j0 + i * chunk, lo, hi, true);
-  Top<LT> all0 = Top<LT>::of(u0[0]);
-#pragma unroll
-  for (int i = 1; i < kUnroll; ++i)
-    if (i < n0) all0 = Top<LT>::max(all0, Top<LT>::of(u0[i]));
-  float v = all0.scalar();
+    if (i < count) u[i] = load_vec(x, base + tid * N + i * chunk, lo, hi, true);
+  const float most = max_vecs<LT>(u, count);
+  float v = most;
   v = v != v ? INFINITY : v;
   for (int size = 2; size <= 32; size <<= 1)
     for (int stride = size >> 1; stride > 0; stride >>= 1) {
@@ -611,54 +599,50 @@ __global__ void __launch_bounds__(kThreads) top_fwd_kernel(TopArgs a) {
     s.warp_max[tid >> 5] = warp_max;
   }
   acc.init(warp_max, c, 0.f);                                          // later maxima are rare
-  const float most0 = take_vecs<LT, X>(acc, u0, n0, top0, c, 0.f);
+  add_vecs<LT, X>(acc, u, count, most, c, 0.f);
   __syncthreads();
-  float thr0 = INFINITY, most = s.warp_max[0];
+  float thr0 = INFINITY, block_max = s.warp_max[0];
   for (int w = 0; w < kWarps; ++w) {
     if (w < whole) thr0 = fminf(thr0, s.warp_nth[w]);
-    most = fmaxf(most, s.warp_max[w]);
+    block_max = fmaxf(block_max, s.warp_max[w]);
   }
   if (nth_of > 32) thr0 = -INFINITY;
   // 64 bins up to the first iteration's maximum; any positive width is correct
-  float width = (most - thr0) * (1.f / 64.f);
+  float width = (block_max - thr0) * (1.f / 64.f);
   if (!(width > 1e-30f && width < 1e30f)) width = 1.f;
   const float inv_width = 1.f / width;
   if (tid == 0) s.thr = thr0;
   float thr = thr0;
   __syncthreads();
   volatile float* shared_thr = &s.thr;
-  int n = 0;                                       // candidates of this thread
-  auto offer = [&](int at, const Top<LT> (&top)[kUnroll], int count, float all) {   // `at`: number of the first vector
-    if (!(all < thr)) {
-#pragma unroll
-      for (int i = 0; i < kUnroll; ++i) {
-        if (i >= count) break;
-        const float t = top[i].scalar();
-        if (!(t < thr)) {
-          const uint32_t bits = __float_as_uint(t);
-          const uint32_t up = t >= 0.f ? (bits + 0xffffu) & 0xffff0000u : bits & 0xffff0000u;
-          if (n < kCand) s.cand[n][tid] = up | static_cast<uint32_t>(at + i);
-          ++n;
-          atomicAdd(&s.bins[bin_of(t, thr0, inv_width)], 1);
-        }
-      }
+  int it = 0;
+  auto offer = [&](float most) {
+    if (!(most < thr)) {
+      const uint32_t bits = __float_as_uint(most);
+      const uint32_t up = (bits + (most >= 0.f ? 0xffffu : 0u)) & 0xffff0000u;
+      const int pos = atomicAdd(&s.count, 1);
+      if (pos < kCand) s.cand[pos] = up | static_cast<uint32_t>(it * kThreads + tid);
+      atomicAdd(&s.bins[bin_of(most, thr0, inv_width)], 1);
     }
-    if (((at / kUnroll) & (kWarps - 1)) == tid >> 5) {
+    if ((it & (kWarps - 1)) == tid >> 5) {
       const int b = cut_bin(s.bins, k);
       const float t = fmaf(b - 1.f, width, thr0);
       if (lane == 0 && b > 1 && t > *shared_thr) *shared_thr = t;
       __syncwarp();
     }
+    ++it;
   };
-  offer(0, top0, n0, most0);
-  each_vec(x, base + kUnroll * chunk, lo, hi, [&](int j, const uint4 (&u)[kUnroll], int count) {
-    Top<LT> top[kUnroll];
-    const float all = take_vecs<LT, X>(acc, u, count, top, c, 0.f);
+  offer(most);
+  each_vec(x, base + kUnroll * chunk, lo, hi, [&](int, const uint4 (&w)[kUnroll], int n) {
     thr = *shared_thr;
-    offer((j - j0) / chunk, top, count, all);
+    const float t = max_vecs<LT>(w, n);
+    add_vecs<LT, X>(acc, w, n, t, c, 0.f);
+    offer(t);
   });
-  // ---- the block's k best, sorted: every thread looks at its own candidates again
-  bool fits = !__syncthreads_or(n > kCand || hi - base > 65536 * chunk);
+  __syncthreads();
+  // ---- the candidates' elements, sorted
+  const int n = s.count;
+  bool fits = n <= kCand && hi - base <= 65536 / kThreads * kUnroll * chunk;
   if (fits) {
     if (tid < 32) {
       const int b = cut_bin(s.bins, k);
@@ -667,12 +651,23 @@ __global__ void __launch_bounds__(kThreads) top_fwd_kernel(TopArgs a) {
     }
     __syncthreads();
     thr = *shared_thr;
-    for (int i = 0; i < n; ++i) {
-      const uint32_t word = s.cand[i][tid];
+    for (int i = tid; i < n; i += kThreads) {
+      const uint32_t word = s.cand[i];
       if (__uint_as_float(word & 0xffff0000u) < thr) continue;
-      const int j = j0 + static_cast<int>(word & 0xffffu) * chunk;
+      const int pos = atomicAdd(&s.n_kept, 1);
+      if (pos < kKept) s.kept[pos] = static_cast<uint16_t>(word);
+    }
+    __syncthreads();
+    fits = s.n_kept <= kKept;
+  }
+  if (fits) {
+    for (int i = tid; i < s.n_kept * kUnroll; i += kThreads) {
+      const int at = s.kept[i / kUnroll];
+      const int j = base + (at / kThreads * kUnroll + i % kUnroll) * chunk + at % kThreads * N;
+      const uint4 w = load_vec(x, j, lo, hi, true);
+      if (Top<LT>::of(w).scalar() < thr) continue;
       float z[N];
-      unpack(load_vec(x, j, lo, hi, true), z);
+      unpack(w, z);
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         if (!(z[e] < thr) && j + e >= lo && j + e < hi) {
@@ -688,12 +683,46 @@ __global__ void __launch_bounds__(kThreads) top_fwd_kernel(TopArgs a) {
     sort_keys(s.keys, s.n_keys);
   else
     select_in_order(s, x, lo, hi, k);
-  Stat st = stat_block<X>(acc.stat(), s.stat, c, 0.f);
-  // ---- over the cluster: the first block collects lists and statistics
-  if (blocks > 1) {
+  return stat_block<X>(acc.stat(), s.stat, c, 0.f);
+}
+
+template <typename LT, int X>
+__device__ __forceinline__ void write_row(const TopArgs& a, int row, const LT* x, const Stat& st, Stat* sh,
+                                          const unsigned long long* keys) {
+  const Row r = finish_row<LT, X>(st, x, a.V, sh, a.inv_temp * kLog2e, 0.f);
+  const int k = a.k;
+  for (int i = threadIdx.x; i < k; i += kThreads) {
+    const unsigned long long key = keys[i];
+    a.ids[static_cast<long long>(row) * k + i] = key_index(key);
+    a.top[static_cast<long long>(row) * k + i] = (key_value(key) - r.m) * a.inv_temp - r.ls;
+  }
+  if (threadIdx.x == 0) {
+    if (a.target) {
+      const long long t = a.targets[row];
+      a.target[row] = (t >= 0 && t < a.V) ? (to_f(x[t]) - r.m) * a.inv_temp - r.ls : 0.f;
+    }
+    if (a.entropy) a.entropy[row] = r.x;
+    a.stats[row] = make_float2(r.m, r.ls);
+  }
+}
+
+// A row per cluster of 1 .. kMaxSplit blocks.
+template <typename LT, int X>
+__global__ void __launch_bounds__(kThreads, X == kNone ? 5 : 4) top_fwd_kernel(TopArgs a) {
+  extern __shared__ __align__(16) unsigned char shared[];
+  Select& s = *reinterpret_cast<Select*>(shared);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int row = blockIdx.x / blocks, tid = threadIdx.x;
+  const LT* x = static_cast<const LT*>(a.logits) + static_cast<long long>(row) * a.ld;
+  const float c = a.inv_temp * kLog2e;
+  const int2 part = part_of(a.V, rank, blocks);
+  const int lo = part.x, hi = part.y, base = lo - misalign(x + lo);
+  Stat st = top_of_part<LT, X>(s, x, base, lo, hi, a.k, c);
+  if (blocks > 1) {                      // the first block collects lists and statistics
     if (tid == 0) {
       s.part = st;
-      s.n_keys = min(k, hi - lo);
+      s.n_keys = min(a.k, hi - lo);
     }
     cluster.sync();
     if (rank == 0) {
@@ -711,20 +740,7 @@ __global__ void __launch_bounds__(kThreads) top_fwd_kernel(TopArgs a) {
     cluster.sync();                      // the others' shared memory was read
     if (rank != 0) return;
   }
-  const Row r = finish_row<LT, X>(st, x, a.V, s.stat, c, 0.f);
-  for (int i = tid; i < k; i += kThreads) {
-    const unsigned long long key = s.keys[i];
-    a.ids[static_cast<long long>(row) * k + i] = key_index(key);
-    a.top[static_cast<long long>(row) * k + i] = (key_value(key) - r.m) * a.inv_temp - r.ls;
-  }
-  if (tid == 0) {
-    if (a.target) {
-      const long long t = a.targets[row];
-      a.target[row] = (t >= 0 && t < a.V) ? (to_f(x[t]) - r.m) * a.inv_temp - r.ls : 0.f;
-    }
-    if (a.entropy) a.entropy[row] = r.x;
-    a.stats[row] = make_float2(r.m, r.ls);
-  }
+  write_row<LT, X>(a, row, x, st, s.stat, s.keys);
 }
 
 // ---- forward: divergence from a teacher's list, cross entropy of a label ---------------------------------
@@ -830,16 +846,12 @@ __global__ void __launch_bounds__(kThreads) distill_fwd_kernel(DistillArgs a, fl
   acc.init(-INFINITY, c1, c2);
   bool fresh = true;
   each_vec(x, lo - misalign(x + lo), lo, hi, [&](int, const uint4 (&u)[kUnroll], int count) {
-    Top<LT> top[kUnroll];
+    const float most = max_vecs<LT>(u, count);
     if (fresh) {                         // begin with the warp's maximum: later ones are rare
-      Top<LT> all = Top<LT>::of(u[0]);
-#pragma unroll
-      for (int i = 1; i < kUnroll; ++i)
-        if (i < count) all = Top<LT>::max(all, Top<LT>::of(u[i]));
-      acc.init(warp_max_of(all.scalar()), c1, c2);
+      acc.init(warp_max_of(most), c1, c2);
       fresh = false;
     }
-    take_vecs<LT, X>(acc, u, count, top, c1, c2);
+    add_vecs<LT, X>(acc, u, count, most, c1, c2);
   });
   Stat st = stat_block<X>(acc.stat(), sh_stat, c1, c2);
   if (blocks > 1) {
@@ -1104,7 +1116,8 @@ extern "C" int tx_top_logprob_fwd(const void* logits, int logits_fp32, long long
   if (T <= 0) return 0;
   if (V < 1 || k < 1 || k > kMaxTop || k > V || V > 0x7fff0000) return 1;
   const TopArgs a{logits, ld, T, V, k, inv_temp, targets, ids, top, target, entropy, reinterpret_cast<float2*>(stats)};
-  const int n = split_of(T, V), bytes = sizeof(Select);
+  const int n = split_of(T, V);
+  const int bytes = sizeof(Select);
   if (logits_fp32)
     return entropy ? launch_rows<top_fwd_kernel<float, kEntropy>>(T, n, bytes, s, a)
                    : launch_rows<top_fwd_kernel<float, kNone>>(T, n, bytes, s, a);
