@@ -19,11 +19,11 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kSortThreads = 1024;
+constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kMaxDigits = 1024;              // 10 bits a pass
 constexpr int kSortCluster = 8;
-constexpr int kSortTile = 8;                  // pairs a lane has in flight
+constexpr int kSortTile = 16;                 // pairs a lane has in flight
 constexpr int kCountTokens = 4096;            // up to here every pair counts the pairs before it: T^2 / 2 comparisons
 constexpr int kCountThreads = 256;
 constexpr int kCountPer = 8;                  // threads per pair
@@ -32,7 +32,7 @@ struct SortArgs {
   const void* ids;
   int ids64;
   int T, V;
-  int passes, bits;           // digit width
+  int passes;
   int2* a;                    // [T]; the sorted pairs end up here
   int2* b;                    // [T]
   int* n_long;                // set to 0 here: length of the list of long runs
@@ -71,25 +71,29 @@ __global__ void __launch_bounds__(kCountThreads) count_sort_kernel(SortArgs s) {
 }
 
 // Every warp owns a contiguous part of its block's part of the pairs, which keeps each pass stable.
+template <int BITS>
 __global__ void __launch_bounds__(kSortThreads, 1) sort_ids_kernel(SortArgs s) {
-  extern __shared__ int hist[];                                    // [warps][digits]
+  extern __shared__ int hist[];                                    // [warps][digits], then lane masks of the same shape
   __shared__ int total[kMaxDigits];                                // of this block, read by the others
   __shared__ int base[kMaxDigits];
   __shared__ int warp_sums[kSortWarps];
   cg::cluster_group cluster = cg::this_cluster();
-  const int blocks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  constexpr int blocks = kSortCluster;
+  const int rank = static_cast<int>(cluster.block_rank());
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int digits = 1 << s.bits;
+  constexpr int digits = 1 << BITS;
   const int parts = blocks * kSortWarps;
   const int per = (s.T + parts - 1) / parts;
   const int lo = min(s.T, (rank * kSortWarps + warp) * per), hi = min(s.T, lo + per);
   int* mine = hist + warp * digits;
+  unsigned* masks = reinterpret_cast<unsigned*>(hist + kSortWarps * digits) + warp * digits;
+  for (int d = lane; d < digits; d += 32) masks[d] = 0;
   if (rank == 0 && tid == 0) *s.n_long = 0;
   for (int p = 0; p < s.passes; ++p) {
     // the last pass writes `a`
     int2* dst = ((s.passes - 1 - p) & 1) ? s.b : s.a;
     const int2* src = ((s.passes - 1 - p) & 1) ? s.a : s.b;
-    const int shift = p * s.bits;
+    const int shift = p * BITS;
     for (int d = lane; d < digits; d += 32) mine[d] = 0;
     __syncwarp();
     int2 pair[kSortTile];
@@ -103,69 +107,78 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_ids_kernel(SortArgs s) {
     for (int i0 = lo; i0 < hi; i0 += 32 * kSortTile) {
       load_tile(i0);
 #pragma unroll
-      for (int u = 0; u < kSortTile; ++u) {
-        const bool in = i0 + u * 32 + lane < hi;
-        const unsigned live = __ballot_sync(0xffffffffu, in);
-        if (in) {
-          const int d = (pair[u].x >> shift) & (digits - 1);
-          const unsigned same = __match_any_sync(live, d);
-          if ((same & ((1u << lane) - 1)) == 0) mine[d] += __popc(same);
-        }
-        __syncwarp();
-      }
+      for (int u = 0; u < kSortTile; ++u)
+        if (i0 + u * 32 + lane < hi) atomicAdd(&mine[(pair[u].x >> shift) & (digits - 1)], 1);
     }
     __syncthreads();
-    int sum = 0;
-    if (tid < digits) {
-      for (int w = 0; w < kSortWarps; ++w) {
-        const int n = hist[w * digits + tid];
-        hist[w * digits + tid] = sum;
-        sum += n;
+    // counts before each warp, this block's totals
+    constexpr int kPer = (digits + kSortThreads - 1) / kSortThreads;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const int d = tid + e * kSortThreads;
+      if (d < digits) {
+        int n[kSortWarps], sum = 0;
+#pragma unroll
+        for (int w = 0; w < kSortWarps; ++w) n[w] = hist[w * digits + d];
+#pragma unroll
+        for (int w = 0; w < kSortWarps; ++w) {
+          hist[w * digits + d] = sum;
+          sum += n[w];
+        }
+        total[d] = sum;
       }
-      total[tid] = sum;
     }
     cluster.sync();
-    int before = 0, all = 0;
-    if (tid < digits) {
-      for (int r = 0; r < blocks; ++r) {
-        const int n = cluster.map_shared_rank(total, r)[tid];
-        if (r < rank) before += n;
-        all += n;
+    int before[kPer], all[kPer], mass = 0;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      const int d = tid * kPer + e;
+      before[e] = all[e] = 0;
+      if (d < digits) {
+#pragma unroll
+        for (int r = 0; r < blocks; ++r) {
+          const int n = cluster.map_shared_rank(total, r)[d];
+          if (r < rank) before[e] += n;
+          all[e] += n;
+        }
       }
+      mass += all[e];
     }
-    int scan = all;                                                // inclusive over the digits
+    int scan = mass;                                               // inclusive over the threads
     for (int o = 1; o < 32; o <<= 1) {
       const int n = __shfl_up_sync(0xffffffffu, scan, o);
       if (lane >= o) scan += n;
     }
     if (lane == 31) warp_sums[warp] = scan;
     __syncthreads();
-    if (warp == 0) {
-      int v = warp_sums[lane];
-      for (int o = 1; o < 32; o <<= 1) {
-        const int n = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += n;
-      }
-      warp_sums[lane] = v;
+    int upto = scan - mass;
+    for (int w = 0; w < warp; ++w) upto += warp_sums[w];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      if (tid * kPer + e < digits) base[tid * kPer + e] = upto + before[e];
+      upto += all[e];
     }
-    __syncthreads();
-    if (tid < digits) base[tid] = scan - all + (warp ? warp_sums[warp - 1] : 0) + before;
     __syncthreads();
     for (int i0 = lo; i0 < hi; i0 += 32 * kSortTile) {
       if (hi - lo > 32 * kSortTile) load_tile(i0);                 // else the tile is still in the registers
 #pragma unroll
       for (int u = 0; u < kSortTile; ++u) {
+        if (i0 + u * 32 >= hi) break;
         const bool in = i0 + u * 32 + lane < hi;
-        const unsigned live = __ballot_sync(0xffffffffu, in);
-        unsigned same = 0;
-        int d = 0;
-        if (in) {
-          d = (pair[u].x >> shift) & (digits - 1);
-          same = __match_any_sync(live, d);
-          dst[base[d] + mine[d] + __popc(same & ((1u << lane) - 1))] = pair[u];
-        }
+        // lanes with this lane's digit: every lane sets its bit in the digit's word (votes and matches take longer)
+        const int d = (pair[u].x >> shift) & (digits - 1);
+        if (in) atomicOr(&masks[d], 1u << lane);
         __syncwarp();
-        if (in && (same & ((1u << lane) - 1)) == 0) mine[d] += __popc(same);
+        const unsigned same = in ? masks[d] : 0, below = same & ((1u << lane) - 1);
+        const int at = in ? base[d] + mine[d] + __popc(below) : 0;
+        __syncwarp();
+        if (in) {
+          dst[at] = pair[u];
+          if (below == 0) {
+            mine[d] += __popc(same);
+            masks[d] = 0;
+          }
+        }
         __syncwarp();
       }
     }
@@ -214,6 +227,7 @@ __device__ __forceinline__ void store_row(__nv_bfloat16* dst, const float (&v)[8
 
 constexpr int kMaxChunk = 32;
 constexpr int kMinChunk = 4;
+constexpr int kRows = 8;             // rows of dout a thread has in flight
 
 // Block (chunk, column tile); a thread owns 8 columns. A run that crosses into the next chunk and ends there belongs to
 // the chunk where it begins; one that covers a whole chunk or more is long.
@@ -255,14 +269,14 @@ __global__ void __launch_bounds__(256) sum_runs_kernel(GradArgs g) {
   }
   if (col >= g.D) return;
   float acc[8] = {};
-  for (int i0 = begin; i0 < end; i0 += 4) {
-    uint4 v[4];
+  for (int i0 = begin; i0 < end; i0 += kRows) {
+    uint4 v[kRows];
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < kRows; ++u)
       if (i0 + u < end)
         v[u] = *reinterpret_cast<const uint4*>(g.dout + static_cast<long long>(run[i0 + u].y) * g.D + col);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kRows; ++u) {
       const int i = i0 + u;
       if (i >= end) break;
       const int id = run[i].x;
@@ -303,6 +317,7 @@ __global__ void __launch_bounds__(8 * kJoinGroups) join_runs_kernel(GradArgs g) 
     const int id = g.pairs[run.y * g.chunk].x;
     float acc[8] = {};
     if (col < g.D) {
+#pragma unroll 4
       for (int i = part * per; i < min(count, (part + 1) * per); ++i) {
         const float4* p = reinterpret_cast<const float4*>(g.partial + (2ll * (run.x + i) + (i == 0 ? 1 : 0)) * g.D + col);
         const float4 x = p[0], y = p[1];
@@ -341,6 +356,30 @@ int launch_grad(const GradArgs& g, cudaStream_t s) {
   return cudaGetLastError() == cudaSuccess ? 0 : 400;
 }
 
+template <int BITS>
+int launch_sort(const SortArgs& so, cudaStream_t s) {
+  const int bytes = 2 * kSortWarps * (1 << BITS) * 4;
+  static txh::DeviceFlag flag;                                     // one per width
+  if (!flag.cur()) {
+    if (cudaFuncSetAttribute(sort_ids_kernel<BITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+      return 401;
+    flag.cur() = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(kSortCluster);
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = kSortCluster;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, sort_ids_kernel<BITS>, so) == cudaSuccess ? 0 : 402;
+}
+
 }  // namespace
 
 // Bytes of workspace for T tokens of D columns (16-byte aligned): two lists of pairs, the list of long runs and its
@@ -361,7 +400,7 @@ extern "C" int tx_embedding_grad(const void* ids, int ids64, const void* dout, v
   int2* b = a + (T + 1ll) / 2 * 2;
   int2* long_runs = b + (T + 1ll) / 2 * 2;
   int* n_long = reinterpret_cast<int*>(long_runs + (chunks + 1) / 2 * 2);
-  SortArgs so{ids, ids64, T, V, 1, 1, a, b, n_long};
+  SortArgs so{ids, ids64, T, V, 1, a, b, n_long};
   const GradArgs g{a, static_cast<const __nv_bfloat16*>(dout), reinterpret_cast<float*>(n_long + 4), long_runs, n_long,
                    grad, T, V, D, chunk_of(T), scale, reinterpret_cast<uintptr_t>(grad) % 16 == 0};
   if (T <= kCountTokens) {
@@ -372,27 +411,8 @@ extern "C" int tx_embedding_grad(const void* ids, int ids64, const void* dout, v
   int bits = 1;
   while ((V >> bits) != 0) ++bits;                                 // V itself marks ids outside
   so.passes = (bits + 9) / 10;
-  so.bits = (bits + so.passes - 1) / so.passes;
-  const int bytes = kSortWarps * (1 << so.bits) * 4;
-  static txh::DeviceFlag flag;
-  if (!flag.cur()) {
-    if (cudaFuncSetAttribute(sort_ids_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             kSortWarps * kMaxDigits * 4) != cudaSuccess) return 401;
-    flag.cur() = true;
-  }
-  const int blocks = kSortCluster;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(blocks);
-  cfg.blockDim = dim3(kSortThreads);
-  cfg.dynamicSmemBytes = bytes;
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = blocks;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, sort_ids_kernel, so) != cudaSuccess) return 402;
+  const int width = (bits + so.passes - 1) / so.passes;
+  const int rc = width > 9 ? launch_sort<10>(so, s) : (width > 8 ? launch_sort<9>(so, s) : launch_sort<8>(so, s));
+  if (rc) return rc;
   return grad_bf16 ? launch_grad<__nv_bfloat16>(g, s) : launch_grad<float>(g, s);
 }
