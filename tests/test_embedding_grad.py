@@ -46,9 +46,9 @@ def check(ids, D, V, scale, grad_dtype, seed=0):
   ids = ids.cuda()
   dout = torch.randn(ids.numel(), D, generator=g, device="cuda").to(bf16)
   base = torch.randn(V, D, generator=g, device="cuda") if grad_dtype == torch.float32 else torch.zeros(V, D, device="cuda", dtype=bf16)
-  grad = base.clone()
+  fresh = lambda: base.clone() if grad_dtype == torch.float32 else torch.full_like(base, 7.0)   # noqa: E731
+  grad, again = fresh(), fresh()                                         # a bf16 gradient is written whole
   kernels.embedding_bwd(ids, dout, grad, scale)
-  again = base.clone()
   kernels.embedding_bwd(ids, dout, again, scale)
   assert torch.equal(grad, again)
   total, mag, n = sums64(ids, dout, V, scale)
@@ -81,6 +81,7 @@ def test_long_lists_and_large_tables(kernel_lib):
   check(id_list("tail", 20_000, 1_048_577), 8, 1_048_577, 1.0, bf16)       # three passes of the sort
   check(id_list("padded", 5000, 100), 4104, 100, 1.0, torch.float32)       # several column tiles
   check(id_list("one", 0, 10), 8, 10, 1.0, torch.float32)
+  check(id_list("one", 0, 10), 8, 10, 1.0, bf16)
   for T in (5, 40, 700, 4096, 9000, 20_000):                               # runs that end on and around chunk borders
     for length in (1, 3, 4, 5, 8, 9, 15, 16, 31, 32, 33, 63, 64, 65, 97):
       check(torch.arange(T) // length, 8, T, 1.0, torch.float32)

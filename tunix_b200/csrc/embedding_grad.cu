@@ -6,7 +6,9 @@
 // memory and whose per-block totals are read through distributed shared memory. (2) Blocks walk `chunk` sorted positions
 // each. A run of equal ids is summed by the block where it begins, also a little into the next chunk; a run that covers
 // a whole chunk (a frequent token, the padding id) is summed by every block it touches, into fp32 partial sums.
-// (3) The partial sums of such a run are added in order. dout is read once and every present row of the table is
+// (3) The partial sums of such a run are added in order. A new gradient is cleared while the
+// ids are sorted.
+// dout is read once and every present row of the table is
 // touched once. Ids outside the vocabulary sort behind all others and are left out.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -14,6 +16,7 @@
 #include <stdint.h>
 
 #include "tx_host.h"
+#include "tx_ptx.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -23,6 +26,7 @@ constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kMaxDigits = 1024;              // 10 bits a pass
 constexpr int kSortCluster = 8;
+constexpr int kClearThreads = 512;
 constexpr int kSortTile = 16;                 // pairs a lane has in flight
 constexpr int kCountTokens = 4096;            // up to here every pair counts the pairs before it: T^2 / 2 comparisons
 constexpr int kCountThreads = 256;
@@ -36,7 +40,25 @@ struct SortArgs {
   int2* a;                    // [T]; the sorted pairs end up here
   int2* b;                    // [T]
   int* n_long;                // set to 0 here: length of the list of long runs
+  uint4* zero;                // a new gradient (n_zero vectors) that is cleared meanwhile, or none
+  long long n_zero;
+  int sort_blocks;            // blocks behind these clear (0: all of them)
 };
+
+__device__ __forceinline__ void clear_part(const SortArgs& s) {
+  constexpr int kTile = 16;                                        // stores a thread has in flight
+  const long long tile = static_cast<long long>(kTile) * blockDim.x, step = (gridDim.x - s.sort_blocks) * tile;
+  const uint4 none = make_uint4(0, 0, 0, 0);
+  for (long long at = (blockIdx.x - s.sort_blocks) * tile + threadIdx.x; at < s.n_zero; at += step) {
+    uint4* p = s.zero + at;
+    if (at + (kTile - 1) * blockDim.x < s.n_zero) {
+#pragma unroll
+      for (int i = 0; i < kTile; ++i) p[i * blockDim.x] = none;
+    } else {
+      for (long long i = at; i < s.n_zero; i += blockDim.x) s.zero[i] = none;
+    }
+  }
+}
 
 // Ids outside the vocabulary become V.
 __device__ __forceinline__ int id_at(const SortArgs& s, int i) {
@@ -52,6 +74,10 @@ __device__ __forceinline__ int2 sort_load(const SortArgs& s, const int2* src, in
 __global__ void __launch_bounds__(kCountThreads) count_sort_kernel(SortArgs s) {
   __shared__ int4 ids4[kCountTokens / 4];
   int* ids = reinterpret_cast<int*>(ids4);
+  if (static_cast<int>(blockIdx.x) >= s.sort_blocks) {
+    clear_part(s);
+    return;
+  }
   const int padded = (s.T + 3) / 4 * 4;
   for (int i = threadIdx.x; i < padded; i += kCountThreads) ids[i] = i < s.T ? id_at(s, i) : 0x7fffffff;
   if (blockIdx.x == 0 && threadIdx.x == 0) *s.n_long = 0;
@@ -88,6 +114,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_ids_kernel(SortArgs s) {
   int* mine = hist + warp * digits;
   unsigned* masks = reinterpret_cast<unsigned*>(hist + kSortWarps * digits) + warp * digits;
   for (int d = lane; d < digits; d += 32) masks[d] = 0;
+  tx::griddep_launch_dependents();
   if (rank == 0 && tid == 0) *s.n_long = 0;
   for (int p = 0; p < s.passes; ++p) {
     // the last pass writes `a`
@@ -186,6 +213,12 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_ids_kernel(SortArgs s) {
   }
 }
 
+// Clears a new gradient on the SMs that the sort in front of it leaves free, and ends after it.
+__global__ void __launch_bounds__(kClearThreads) clear_kernel(SortArgs s) {
+  clear_part(s);
+  tx::griddep_wait();
+}
+
 struct GradArgs {
   const int2* pairs;          // [T] sorted
   const __nv_bfloat16* dout;  // [T, D]
@@ -232,7 +265,7 @@ constexpr int kRows = 8;             // rows of dout a thread has in flight
 // Block (chunk, column tile); a thread owns 8 columns. A run that crosses into the next chunk and ends there belongs to
 // the chunk where it begins; one that covers a whole chunk or more is long.
 template <typename GT>
-__global__ void __launch_bounds__(256) sum_runs_kernel(GradArgs g) {
+__global__ void __launch_bounds__(256, 4) sum_runs_kernel(GradArgs g) {
   __shared__ int2 window[3 * kMaxChunk + 2];                       // the chunk before with one more, this one, the next with one more
   const int size = g.chunk, lo = blockIdx.x * size, n = min(size, g.T - lo);
   for (int i = threadIdx.x; i < 3 * size + 2; i += blockDim.x) {
@@ -269,24 +302,36 @@ __global__ void __launch_bounds__(256) sum_runs_kernel(GradArgs g) {
   }
   if (col >= g.D) return;
   float acc[8] = {};
+  auto row = [&](int i) { return *reinterpret_cast<const uint4*>(g.dout + static_cast<long long>(run[i].y) * g.D + col); };
+  auto add = [&](uint4 v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      acc[2 * e] += __uint_as_float(w[e] << 16);
+      acc[2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u);
+    }
+  };
   for (int i0 = begin; i0 < end; i0 += kRows) {
     uint4 v[kRows];
+    const int id0 = run[i0].x;
+    if (id0 >= g.V) return;                                        // only ids outside the vocabulary follow
+    if (i0 + kRows < end && run[i0 + kRows].x == id0) {            // in the middle of a run
+#pragma unroll
+      for (int u = 0; u < kRows; ++u) v[u] = row(i0 + u);
+#pragma unroll
+      for (int u = 0; u < kRows; ++u) add(v[u]);
+      continue;
+    }
 #pragma unroll
     for (int u = 0; u < kRows; ++u)
-      if (i0 + u < end)
-        v[u] = *reinterpret_cast<const uint4*>(g.dout + static_cast<long long>(run[i0 + u].y) * g.D + col);
+      if (i0 + u < end) v[u] = row(i0 + u);
 #pragma unroll
     for (int u = 0; u < kRows; ++u) {
       const int i = i0 + u;
       if (i >= end) break;
       const int id = run[i].x;
-      if (id >= g.V) return;                                       // only ids outside the vocabulary follow
-      const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        acc[2 * e] += __uint_as_float(w[e] << 16);
-        acc[2 * e + 1] += __uint_as_float(w[e] & 0xffff0000u);
-      }
+      if (id >= g.V) return;
+      add(v[u]);
       if (i + 1 < end && run[i + 1].x == id) continue;
       const bool in = long_in && id == head, on = long_out && id == tail;
       if (in || on) {
@@ -357,7 +402,7 @@ int launch_grad(const GradArgs& g, cudaStream_t s) {
 }
 
 template <int BITS>
-int launch_sort(const SortArgs& so, cudaStream_t s) {
+int launch_sort(SortArgs so, cudaStream_t s) {
   const int bytes = 2 * kSortWarps * (1 << BITS) * 4;
   static txh::DeviceFlag flag;                                     // one per width
   if (!flag.cur()) {
@@ -377,7 +422,15 @@ int launch_sort(const SortArgs& so, cudaStream_t s) {
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sort_ids_kernel<BITS>, so) == cudaSuccess ? 0 : 402;
+  if (cudaLaunchKernelEx(&cfg, sort_ids_kernel<BITS>, so) != cudaSuccess) return 402;
+  if (so.n_zero == 0) return 0;
+  const long long tiles = (so.n_zero + 16 * kClearThreads - 1) / (16 * kClearThreads);
+  cfg.gridDim = dim3(static_cast<unsigned>(min(tiles, 4ll * txh::sm_count())));
+  cfg.blockDim = dim3(kClearThreads);
+  cfg.dynamicSmemBytes = 0;
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  return cudaLaunchKernelEx(&cfg, clear_kernel, so) == cudaSuccess ? 0 : 404;
 }
 
 }  // namespace
@@ -390,22 +443,32 @@ extern "C" long long tx_embedding_grad_workspace(int T, int D) {
 }
 
 // ids int64 or int32 [T], dout bf16 [T, D] with D a multiple of 8. grad_bf16 == 0: grad is fp32 and added to; else it
-// is bf16 and the present rows are overwritten (the caller has zeroed the others).
+// is bf16 and written whole.
 extern "C" int tx_embedding_grad(const void* ids, int ids64, const void* dout, void* grad, int grad_bf16, int T, int D,
                                  int V, float scale, void* workspace, cudaStream_t s) {
   if (D % 8 || D <= 0 || V <= 0 || V > 0x3fffffff) return 1;
-  if (T <= 0) return 0;
+  if (T <= 0) return grad_bf16 && cudaMemsetAsync(grad, 0, 2ll * V * D, s) != cudaSuccess ? 403 : 0;
   const long long chunks = (T + chunk_of(T) - 1) / chunk_of(T);
   int2* a = static_cast<int2*>(workspace);
   int2* b = a + (T + 1ll) / 2 * 2;
   int2* long_runs = b + (T + 1ll) / 2 * 2;
   int* n_long = reinterpret_cast<int*>(long_runs + (chunks + 1) / 2 * 2);
-  SortArgs so{ids, ids64, T, V, 1, a, b, n_long};
+  SortArgs so{ids, ids64, T, V, 1, a, b, n_long, nullptr, 0, 0};
+  if (grad_bf16) {
+    if (reinterpret_cast<uintptr_t>(grad) % 16 == 0) {
+      so.zero = static_cast<uint4*>(grad);
+      so.n_zero = static_cast<long long>(V) * D / 8;
+    } else if (cudaMemsetAsync(grad, 0, 2ll * V * D, s) != cudaSuccess) {
+      return 403;
+    }
+  }
   const GradArgs g{a, static_cast<const __nv_bfloat16*>(dout), reinterpret_cast<float*>(n_long + 4), long_runs, n_long,
                    grad, T, V, D, chunk_of(T), scale, reinterpret_cast<uintptr_t>(grad) % 16 == 0};
   if (T <= kCountTokens) {
     const int per = kCountThreads / kCountPer;
-    count_sort_kernel<<<(T + per - 1) / per, kCountThreads, 0, s>>>(so);
+    so.sort_blocks = (T + per - 1) / per;
+    const long long clear = (so.n_zero + 8 * kCountThreads - 1) / (8 * kCountThreads);
+    count_sort_kernel<<<so.sort_blocks + static_cast<int>(min(clear, 8ll * txh::sm_count())), kCountThreads, 0, s>>>(so);
     return grad_bf16 ? launch_grad<__nv_bfloat16>(g, s) : launch_grad<float>(g, s);
   }
   int bits = 1;

@@ -279,8 +279,7 @@ class _EmbeddingFn(torch.autograd.Function):
     if mg is not None:
       kernels.embedding_bwd(ids, dout, mg, ctx.scale)
       return None, None, None
-    V, D = ctx.shape                    # zeroed as 32-bit words: twice the rate of the 16-bit fill
-    g = torch.zeros((V, D // 2), dtype=torch.float32, device=dout.device).view(dout.dtype)
+    g = torch.empty(ctx.shape, dtype=dout.dtype, device=dout.device)
     kernels.embedding_bwd(ids, dout, g, ctx.scale)
     return None, g, None
 

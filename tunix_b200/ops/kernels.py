@@ -162,7 +162,7 @@ def embedding_fwd(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) ->
 
 def embedding_bwd(ids: torch.Tensor, dout: torch.Tensor, grad_table: torch.Tensor, scale: float = 1.0) -> None:
   """Sums scale * dout [T, D] (bf16) over the positions of every id, in a fixed order. grad_table [V, D] fp32 is added
-  to; a bf16 one (zeroed by the caller) gets the rows that occur. Ids outside the vocabulary are left out."""
+  to; a bf16 one is written whole, rows that do not occur are zero. Ids outside the vocabulary are left out."""
   ids = ids.reshape(-1)
   if ids.dtype not in (torch.int32, torch.int64):
     ids = ids.to(torch.int64)
