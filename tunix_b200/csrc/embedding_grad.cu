@@ -42,21 +42,16 @@ struct SortArgs {
   int* n_long;                // set to 0 here: length of the list of long runs
   uint4* zero;                // a new gradient (n_zero vectors) that is cleared meanwhile, or none
   long long n_zero;
-  int sort_blocks;            // blocks behind these clear (0: all of them)
+  int sort_blocks;            // of the counting sort; blocks behind these clear
 };
 
-__device__ __forceinline__ void clear_part(const SortArgs& s) {
-  constexpr int kTile = 16;                                        // stores a thread has in flight
-  const long long tile = static_cast<long long>(kTile) * blockDim.x, step = (gridDim.x - s.sort_blocks) * tile;
-  const uint4 none = make_uint4(0, 0, 0, 0);
-  for (long long at = (blockIdx.x - s.sort_blocks) * tile + threadIdx.x; at < s.n_zero; at += step) {
-    uint4* p = s.zero + at;
-    if (at + (kTile - 1) * blockDim.x < s.n_zero) {
-#pragma unroll
-      for (int i = 0; i < kTile; ++i) p[i * blockDim.x] = none;
-    } else {
-      for (long long i = at; i < s.n_zero; i += blockDim.x) s.zero[i] = none;
-    }
+// One block's tile. Tiles of 16 KB whose blocks end at once: 7.4 TB/s, where a few blocks per SM that loop over them
+// write 6.1 TB/s.
+constexpr int kClearTile = 1024;
+__device__ __forceinline__ void clear_tile(const SortArgs& s, long long tile) {
+  for (int i = threadIdx.x; i < kClearTile; i += blockDim.x) {
+    const long long at = tile * kClearTile + i;
+    if (at < s.n_zero) s.zero[at] = make_uint4(0, 0, 0, 0);
   }
 }
 
@@ -75,7 +70,7 @@ __global__ void __launch_bounds__(kCountThreads) count_sort_kernel(SortArgs s) {
   __shared__ int4 ids4[kCountTokens / 4];
   int* ids = reinterpret_cast<int*>(ids4);
   if (static_cast<int>(blockIdx.x) >= s.sort_blocks) {
-    clear_part(s);
+    clear_tile(s, blockIdx.x - s.sort_blocks);
     return;
   }
   const int padded = (s.T + 3) / 4 * 4;
@@ -213,10 +208,10 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_ids_kernel(SortArgs s) {
   }
 }
 
-// Clears a new gradient on the SMs that the sort in front of it leaves free, and ends after it.
+// Clears a new gradient on the SMs that the sort in front of it leaves free; its last block ends after the sort.
 __global__ void __launch_bounds__(kClearThreads) clear_kernel(SortArgs s) {
-  clear_part(s);
-  tx::griddep_wait();
+  clear_tile(s, blockIdx.x);
+  if (blockIdx.x == gridDim.x - 1) tx::griddep_wait();
 }
 
 struct GradArgs {
@@ -424,8 +419,7 @@ int launch_sort(SortArgs so, cudaStream_t s) {
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, sort_ids_kernel<BITS>, so) != cudaSuccess) return 402;
   if (so.n_zero == 0) return 0;
-  const long long tiles = (so.n_zero + 16 * kClearThreads - 1) / (16 * kClearThreads);
-  cfg.gridDim = dim3(static_cast<unsigned>(min(tiles, 4ll * txh::sm_count())));
+  cfg.gridDim = dim3(static_cast<unsigned>((so.n_zero + kClearTile - 1) / kClearTile));
   cfg.blockDim = dim3(kClearThreads);
   cfg.dynamicSmemBytes = 0;
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -467,8 +461,8 @@ extern "C" int tx_embedding_grad(const void* ids, int ids64, const void* dout, v
   if (T <= kCountTokens) {
     const int per = kCountThreads / kCountPer;
     so.sort_blocks = (T + per - 1) / per;
-    const long long clear = (so.n_zero + 8 * kCountThreads - 1) / (8 * kCountThreads);
-    count_sort_kernel<<<so.sort_blocks + static_cast<int>(min(clear, 8ll * txh::sm_count())), kCountThreads, 0, s>>>(so);
+    const unsigned clear = static_cast<unsigned>((so.n_zero + kClearTile - 1) / kClearTile);
+    count_sort_kernel<<<so.sort_blocks + clear, kCountThreads, 0, s>>>(so);
     return grad_bf16 ? launch_grad<__nv_bfloat16>(g, s) : launch_grad<float>(g, s);
   }
   int bits = 1;

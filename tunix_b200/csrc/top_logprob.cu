@@ -33,6 +33,7 @@ constexpr int kKeys = 2048;                   // elements that do; a cluster's l
 constexpr int kBins = 256;
 constexpr int kMaxSplit = 8;                  // blocks (one cluster) a row is spread over when there are few rows
 constexpr int kMinPart = 4096;                // columns of such a part at least
+constexpr int kBwdPart = 32768;               // columns a block of the backward pass takes at most
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFloor = -1e37f;              // lowest running maximum
 
@@ -153,6 +154,17 @@ __device__ __forceinline__ uint4 load_vec(const T* row, int j, int lo, int hi, b
 #pragma unroll
   for (int i = 0; i < kVec<T>; ++i) z[i] = (j + i >= lo && j + i < hi) ? to_f(row[j + i]) : -INFINITY;
   return pack(z);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_vec(T* row, int j, int lo, int hi, const float (&z)[kVec<T>]) {
+  if (j >= lo && j + kVec<T> <= hi) {
+    *reinterpret_cast<uint4*>(row + j) = pack(z);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec<T>; ++i)
+      if (j + i >= lo && j + i < hi) from_f(z[i], row + j + i);
+  }
 }
 
 // Columns of a row that block `rank` of `blocks` takes: equal parts, cut at multiples of 8 from the first one.
@@ -891,6 +903,10 @@ struct BwdArgs {
 
 // d_j = A p_j (temperature) + B p_j (temperature 1) - G p_j (log p_j + H), then the listed columns get their own
 // terms on top: they are computed from the same fp32 value and rounded once, by the thread of the first occurrence.
+//
+// A block has a part of kBwdPart columns: the blocks at work at a time then cover few rows from end to end, which the
+// memory takes 4 to 8 % faster than a block per row (4096 x 128256 bf16: 325 us, against 354 us for whole rows and
+// 392 us for parts of 8192, whose lists cost more). Without a dense term the gradient was cleared before.
 template <typename LT, int DENSE>   // bit 0: temperature, bit 1: temperature 1, bit 2: entropy
 __global__ void __launch_bounds__(kThreads) top_bwd_kernel(BwdArgs a) {
   __shared__ __align__(16) int sh_id[kMaxList];
@@ -1002,15 +1018,15 @@ __global__ void __launch_bounds__(kThreads) top_bwd_kernel(BwdArgs a) {
     return r;
   };
   // ---- the whole part
-  for (int at = from; at < hi; at += kUnroll * chunk) {
-    const int j = at + tid * N;
-    if (DENSE && at != from) load(j);
+  if (DENSE) {
+    for (int at = from; at < hi; at += kUnroll * chunk) {
+      const int j = at + tid * N;
+      if (at != from) load(j);
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-      const int ji = j + i * chunk;
-      if (ji >= hi) break;
-      float z[N];
-      if (DENSE) {
+      for (int i = 0; i < kUnroll; ++i) {
+        const int ji = j + i * chunk;
+        if (ji >= hi) break;
+        float z[N];
         unpack(u[i], z);
 #pragma unroll
         for (int e = 0; e < N; e += 2) {
@@ -1018,16 +1034,7 @@ __global__ void __launch_bounds__(kThreads) top_bwd_kernel(BwdArgs a) {
           z[e] = r.x;
           z[e + 1] = r.y;
         }
-      } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) z[e] = 0.f;
-      }
-      if (ji >= lo && ji + N <= hi) {
-        *reinterpret_cast<uint4*>(dx + ji) = pack(z);
-      } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e)
-          if (ji + e >= lo && ji + e < hi) from_f(z[e], dx + ji + e);
+        store_vec(dx, ji, lo, hi, z);
       }
     }
   }
@@ -1094,10 +1101,32 @@ int launch_rows(int T, int blocks, int bytes, cudaStream_t s, Args... args) {
   return cudaLaunchKernelEx(&cfg, Kernel, args...) == cudaSuccess ? 0 : 400;
 }
 
+// n 16-byte vectors. Blocks of 16 KB that end at once: 7.4 TB/s, where 1184 blocks that loop over the same tiles write
+// 6.1 TB/s (1.24 GB).
+constexpr int kClearThreads = 512, kClearVecs = 2;
+__global__ void __launch_bounds__(kClearThreads) clear_kernel(uint4* p, long long n) {
+  const long long at = blockIdx.x * static_cast<long long>(kClearThreads * kClearVecs) + threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < kClearVecs; ++i)
+    if (at + i * kClearThreads < n) p[at + i * kClearThreads] = make_uint4(0, 0, 0, 0);
+}
+
 template <typename LT>
 int launch_bwd(BwdArgs a, int dense, cudaStream_t s) {
+  // few rows: more and smaller parts, so that every SM has some
   const int want = 8 * txh::sm_count(), most = (a.V + kMinPart - 1) / kMinPart;
-  a.blocks = min(most, a.T >= want ? 1 : (want + a.T - 1) / a.T);
+  a.blocks = max((a.V + kBwdPart - 1) / kBwdPart, min(most, (want + a.T - 1) / a.T));
+  if (dense == 0) {
+    a.blocks = 1;
+    const long long bytes = ((a.T - 1) * a.ldd + a.V) * static_cast<long long>(sizeof(LT));
+    const long long n = reinterpret_cast<uintptr_t>(a.dx) % 16 == 0 && a.ldd == a.V ? bytes / 16 : 0;
+    if (n > 0)
+      clear_kernel<<<static_cast<unsigned>((n + kClearThreads * kClearVecs - 1) / (kClearThreads * kClearVecs)), kClearThreads, 0, s>>>(
+          static_cast<uint4*>(a.dx), n);
+    if (bytes > n * 16 && cudaMemset2DAsync(static_cast<char*>(a.dx) + n * 16, n ? bytes - n * 16 : a.ldd * sizeof(LT), 0,
+                                            n ? bytes - n * 16 : a.V * sizeof(LT), n ? 1 : a.T, s) != cudaSuccess)
+      return 403;
+  }
 #define TX_BWD(D) case D: top_bwd_kernel<LT, D><<<a.T * a.blocks, kThreads, 0, s>>>(a); break
   switch (dense) {
     TX_BWD(0); TX_BWD(1); TX_BWD(2); TX_BWD(3); TX_BWD(5);
