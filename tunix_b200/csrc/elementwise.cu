@@ -92,7 +92,8 @@ __global__ void glu_bwd_kernel(const __nv_bfloat16* __restrict__ gu, const __nv_
 }
 
 // out[t, :] = table[ids[t], :] * scale
-__global__ void embedding_fwd_kernel(const int* __restrict__ ids, const __nv_bfloat16* __restrict__ table,
+template <typename IdT>
+__global__ void embedding_fwd_kernel(const IdT* __restrict__ ids, const __nv_bfloat16* __restrict__ table,
                                      __nv_bfloat16* __restrict__ out, long long T, int D, int V, float scale) {
   const int dv = D / 8;
   const long long total = T * dv;
@@ -100,7 +101,7 @@ __global__ void embedding_fwd_kernel(const int* __restrict__ ids, const __nv_bfl
        i += static_cast<long long>(gridDim.x) * blockDim.x) {
     const long long t = i / dv;
     const int c = static_cast<int>(i - t * dv) * 8;
-    int id = ids[t];
+    IdT id = ids[t];
     TX_DEBUG_CHECK(id >= 0 && id < V, TX_DBG_TOKEN_ID, id, V);
     id = id < 0 ? 0 : (id >= V ? V - 1 : id);
     float v[8];
@@ -266,12 +267,18 @@ extern "C" int tx_glu_bwd(const void* gu, const void* dout, void* dgu, long long
   return TX_OK();
 }
 
-extern "C" int tx_embedding_fwd(const int* ids, const void* table, void* out, long long T, int D, int V,
+// ids int64 or int32 [T]
+extern "C" int tx_embedding_fwd(const void* ids, int ids64, const void* table, void* out, long long T, int D, int V,
                                 float scale, cudaStream_t s) {
   if (D % 8) return 1;
   if (T <= 0) return 0;
-  embedding_fwd_kernel<<<grid_for(T * (D / 8), 256), 256, 0, s>>>(ids, (const __nv_bfloat16*)table,
-                                                                  (__nv_bfloat16*)out, T, D, V, scale);
+  const int g = grid_for(T * (D / 8), 256);
+  if (ids64)
+    embedding_fwd_kernel<<<g, 256, 0, s>>>((const long long*)ids, (const __nv_bfloat16*)table, (__nv_bfloat16*)out, T, D,
+                                           V, scale);
+  else
+    embedding_fwd_kernel<<<g, 256, 0, s>>>((const int*)ids, (const __nv_bfloat16*)table, (__nv_bfloat16*)out, T, D, V,
+                                           scale);
   return TX_OK();
 }
 

@@ -45,7 +45,7 @@ def _declare(lib):
       "tx_qknorm_rope_bwd": [P, P, P, P, P, P, P, P, P, L, I, I, I, I, L, L, L, F, F, I, P, P],
       "tx_glu_fwd": [P, P, L, I, I, P],
       "tx_glu_bwd": [P, P, P, L, I, I, P],
-      "tx_embedding_fwd": [P, P, P, L, I, I, F, P],
+      "tx_embedding_fwd": [P, I, P, P, L, I, I, F, P],
       "tx_embedding_grad": [P, I, P, P, I, I, I, I, F, P, P],
       "tx_adamw": [P, P, P, P, P, L, F, F, F, F, F, F, F, P, I, P],
       "tx_sumsq_partials": [],

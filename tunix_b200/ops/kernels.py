@@ -151,22 +151,29 @@ def glu_bwd(gu: torch.Tensor, dout: torch.Tensor, gelu: bool) -> torch.Tensor:
   return dgu
 
 
+def _flat_ids(ids: torch.Tensor) -> torch.Tensor:
+  """ids as the kernels read them: one contiguous dimension, int64 or int32."""
+  if ids.dim() != 1:
+    ids = ids.reshape(-1)
+  if ids.dtype not in (torch.int64, torch.int32):
+    ids = ids.to(torch.int64)
+  return ids if ids.is_contiguous() else ids.contiguous()
+
+
 def embedding_fwd(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
-  ids32 = ids.reshape(-1).to(torch.int32)
+  ids = _flat_ids(ids)
+  T = ids.numel()
   V, D = table.shape
-  out = torch.empty((ids32.numel(), D), dtype=table.dtype, device=table.device)
-  _lib.check_rc(_lib.require().tx_embedding_fwd(ids32.data_ptr(), table.data_ptr(), out.data_ptr(), ids32.numel(),
-                                                D, V, float(scale), _lib.stream_ptr()), "tx_embedding_fwd")
+  out = torch.empty((T, D), dtype=table.dtype, device=table.device)
+  _lib.check_rc(_lib.require().tx_embedding_fwd(ids.data_ptr(), ids.dtype == torch.int64, table.data_ptr(),
+                                                out.data_ptr(), T, D, V, scale, _lib.stream_ptr()), "tx_embedding_fwd")
   return out
 
 
 def embedding_bwd(ids: torch.Tensor, dout: torch.Tensor, grad_table: torch.Tensor, scale: float = 1.0) -> None:
   """Sums scale * dout [T, D] (bf16) over the positions of every id, in a fixed order. grad_table [V, D] fp32 is added
   to; a bf16 one is written whole, rows that do not occur are zero. Ids outside the vocabulary are left out."""
-  ids = ids.reshape(-1)
-  if ids.dtype not in (torch.int32, torch.int64):
-    ids = ids.to(torch.int64)
-  ids = ids.contiguous()
+  ids = _flat_ids(ids)
   T = ids.numel()
   V, D = grad_table.shape
   assert dout.dtype == bf16 and dout.is_contiguous() and dout.numel() == T * D and grad_table.is_contiguous()
@@ -175,9 +182,9 @@ def embedding_bwd(ids: torch.Tensor, dout: torch.Tensor, grad_table: torch.Tenso
     dout = dout.clone()
   lib = _lib.require()
   work = torch.empty(lib.tx_embedding_grad_workspace(T, D), dtype=torch.uint8, device=dout.device)
-  _lib.check_rc(lib.tx_embedding_grad(ids.data_ptr(), int(ids.dtype == torch.int64), dout.data_ptr(),
-                                      grad_table.data_ptr(), int(grad_table.dtype == bf16), T, D, V, float(scale),
-                                      work.data_ptr(), _lib.stream_ptr()), "tx_embedding_grad")
+  _lib.check_rc(lib.tx_embedding_grad(ids.data_ptr(), ids.dtype == torch.int64, dout.data_ptr(), grad_table.data_ptr(),
+                                      grad_table.dtype == bf16, T, D, V, scale, work.data_ptr(), _lib.stream_ptr()),
+                "tx_embedding_grad")
 
 
 def adamw_step(master, m, v, grad, param_bf16, *, lr, beta1, beta2, eps, weight_decay, step: int,
