@@ -1,0 +1,208 @@
+"""Distillation from a teacher's best tokens as a user runs it: `LogitStrategy` with a top-k or a stored list, the
+trainer around it, and a step from the token embedding to the table's gradient; captured and on two streams."""
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from tunix_b200 import optim
+from tunix_b200.common.configs import TrainingConfig
+from tunix_b200.distillation import DistillationTrainer, TrainingInput, strategies
+from tunix_b200.models.transformer import ModelConfig, Transformer
+from tunix_b200.ops import functional
+from tunix_b200.sft import utils as sft_utils
+
+bf16, f64 = torch.bfloat16, torch.float64
+DEVICES = [pytest.param("cpu"), pytest.param("cuda", marks=pytest.mark.gpu)]
+U = 2.0 ** -24
+
+
+def strategy(**kw):
+  return strategies.LogitStrategy(lambda m, **i: None, lambda m, **i: None, lambda **i: None, **kw)
+
+
+def loss64(s, t, labels, k, tau, alpha):
+  """The strategy's loss in 64 bits for integer or one-hot labels, the gradients of its two parts and a bound of the
+  terms these are made of."""
+  s = s.detach().to(f64).requires_grad_()
+  t = t.detach().to(f64)
+  rows = s[..., 0].numel()
+  tk, idx = torch.topk(t, k, dim=-1)
+  lq = F.log_softmax(tk / tau, -1)
+  lp = F.log_softmax(s.gather(-1, idx) / tau, -1)
+  soft = alpha * (lq.exp() * (lq - lp)).sum(-1).mean() * tau * tau
+  lps = F.log_softmax(s, -1)
+  hot = F.one_hot(labels, s.shape[-1]).to(f64) if labels.ndim == 2 else labels.to(f64)
+  hard = (1 - alpha) * -(lps * hot).sum(-1).mean()
+  terms = ((1 - alpha) * (lps.exp() + hot) / rows).scatter_add(-1, idx, alpha * tau * (lq.exp() + lp.exp()) / rows)
+  return (soft + hard).detach(), torch.autograd.grad(soft, s)[0], torch.autograd.grad(hard, s)[0], terms.detach()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("one_hot", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, bf16])
+def test_strategy_over_logits_and_over_a_list(device, one_hot, dtype):
+  B, T, V, k, tau, alpha = 2, 9, 700, 12, 2.0, 0.6
+  g = torch.Generator().manual_seed(0)
+  # distinct teacher values in either type: no ties at the k-th place
+  t = torch.stack([torch.randperm(V, generator=g) for _ in range(B * T)]).view(B, T, V).float().to(device).mul(0.0625).to(dtype)
+  if dtype == bf16:
+    t = (torch.stack([torch.randperm(V, generator=g) for _ in range(B * T)]).view(B, T, V) % 256).float().to(device)
+    t = torch.where(t > 128, t, torch.zeros_like(t)).mul(0.0625)
+    rank = torch.argsort(torch.rand(B, T, V, generator=g), -1)[..., :k].to(device)
+    t.scatter_(-1, rank, (torch.arange(k, device=device) + 20.0).expand(B, T, k))
+    t = t.to(bf16)
+  s = (torch.randn(B, T, V, generator=g) * 2).to(device).to(dtype)
+  ids = torch.randint(0, V, (B, T), generator=g).to(device)
+  labels = F.one_hot(ids, V).float() if one_hot else ids
+  want, g_soft, g_hard, terms = loss64(s, t, labels, k, tau, alpha)
+  strat = strategy(temperature=tau, alpha=alpha, distill_top_k=k)
+  listed = functional.top_logprobs(t, k + 5, ids)
+  # fp32 throughout: log-probabilities of at most 64 in size off by 16 roundings each, means of 18 of them
+  tol = 64 * 16 * U * (tau * tau + 1)
+  for teacher in (t, listed):
+    leaf = s.clone().requires_grad_()
+    loss, m = strat.compute_loss(leaf, teacher, labels)
+    assert abs(float(loss.detach()) - float(want)) <= tol
+    assert set(m) == {"distill/soft_loss", "distill/hard_loss", "distill/kl_div", "distill/teacher_loss"}
+    assert float(m["distill/teacher_loss"]) == pytest.approx(float(-F.log_softmax(t.double(), -1).gather(-1, ids[..., None]).mean()), abs=tol)
+    grad, = torch.autograd.grad(loss, leaf)
+    # one-hot labels: the two parts arrive separately, each rounded to the logits' type, and their sum is rounded; an
+    # exponent of at most 64 in size off by 8 roundings and 2^-22 of an exponential is 1024 U of a term
+    half = torch.finfo(dtype).eps / 2
+    near = (grad.to(f64) - (g_soft + g_hard)).abs() - half * (1 + half) * (g_soft.abs() + g_hard.abs() + (g_soft + g_hard).abs()) \
+        - 1024 * U * terms
+    assert float(near.max()) <= 0
+
+
+def test_a_list_without_targets_has_no_teacher_loss():
+  t, s = torch.randn(2, 3, 40), torch.randn(2, 3, 40)
+  _, m = strategy(distill_top_k=4).compute_loss(s, functional.top_logprobs(t, 4), torch.zeros(2, 3, dtype=torch.long))
+  assert "distill/teacher_loss" not in m and math.isfinite(float(m["distill/soft_loss"]))
+  # without a top-k of its own the strategy takes the whole list
+  whole, _ = strategy(alpha=1.0).compute_loss(s, functional.top_logprobs(t, 4), torch.zeros(2, 3, dtype=torch.long))
+  cut, _ = strategy(alpha=1.0, distill_top_k=4).compute_loss(s, t, torch.zeros(2, 3, dtype=torch.long))
+  assert float(whole) == pytest.approx(float(cut), rel=1e-5)
+
+
+V_MODEL = 512
+
+
+def tiny(layers, width, seed, device, dtype):
+  cfg = ModelConfig(num_layers=layers, vocab_size=V_MODEL, embed_dim=width, hidden_dim=2 * width, num_heads=2,
+                    head_dim=64, num_kv_heads=1, dtype=dtype, weight_tying=True, embed_scale=True)
+  return Transformer(cfg, device=device).init_weights(seed=seed, scale=0.05)
+
+
+def forward_logits(m, input_tokens, input_mask):
+  pos = sft_utils.build_positions_from_mask(input_mask)
+  return m(input_tokens, pos, None, sft_utils.make_causal_attn_mask(input_mask))[0]
+
+
+def teacher_list(m, input_tokens, input_mask):
+  return functional.top_logprobs(forward_logits(m, input_tokens, input_mask), 16, torch.roll(input_tokens, -1, 1))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("stored", [False, True])
+def test_trainer(device, stored):
+  dtype = bf16 if device == "cuda" else torch.float32
+  strat = strategies.LogitStrategy(forward_logits, teacher_list if stored else forward_logits,
+                                   lambda input_tokens, input_mask: torch.roll(input_tokens, -1, 1), temperature=2.0,
+                                   alpha=0.7, distill_top_k=16)
+  tr = DistillationTrainer(tiny(1, 128, 0, device, dtype), tiny(2, 256, 1, device, dtype), strat, optim.adamw(1e-3),
+                           TrainingConfig(eval_every_n_steps=100, max_steps=3, pbar_description=None))
+  g = torch.Generator().manual_seed(0)
+  before = tr.model.embedder.input_embedding.detach().clone()
+  tr.train([TrainingInput(torch.randint(1, V_MODEL, (2, 24), generator=g), torch.ones(2, 24, dtype=torch.long)) for _ in range(3)])
+  for name in ("distill/soft_loss", "distill/hard_loss", "distill/kl_div", "distill/teacher_loss"):
+    h = tr.metrics_logger.get_metric_history("", name, "train")
+    assert len(h) == 3 and all(math.isfinite(v) for v in h)
+  assert not torch.equal(before, tr.model.embedder.input_embedding.detach())
+  tr.close()
+
+
+def step(table, ids, t_logits, labels, k, tau):
+  """Token embedding -> tied head -> distillation from the teacher's list -> gradient of the table (both uses)."""
+  h = functional.embedding(ids, table, 1.5)
+  logits = h @ table.t()
+  with torch.no_grad():
+    top = functional.top_logprobs(t_logits, k, labels, temperature=tau)
+  terms = functional.top_distill_loss(logits, top.ids, top.top, labels, temperature=tau, normalize="full")
+  loss = (0.7 * terms.kl + 0.3 * terms.nll).mean()
+  return loss, torch.autograd.grad(loss, table)[0], top
+
+
+@pytest.mark.gpu
+def test_chain_against_64_bits(kernel_lib):
+  V, D, T, k, tau = 2003, 64, 300, 20, 1.3
+  g = torch.Generator().manual_seed(0)
+  table = (torch.randn(V, D, generator=g) * 0.3).to(bf16).cuda().requires_grad_()
+  ids = torch.randint(0, 40, (T,), generator=g).cuda()
+  labels = torch.randint(0, V, (T,), generator=g).cuda()
+  t_logits = (torch.randn(T, V, generator=g) * 2).cuda()
+  loss, grad, top = step(table, ids, t_logits, labels, k, tau)
+
+  tb = table.detach().to(f64).requires_grad_()
+  h = tb[ids] * 1.5
+  h = h + (h.detach().to(bf16).to(f64) - h.detach())                # rounded where the operators round
+  logits = h @ tb.t()
+  logits = logits + (logits.detach().to(bf16).to(f64) - logits.detach())
+  t = F.log_softmax(t_logits.to(f64) / tau, -1)
+  tt, at = torch.topk(t, k, -1)
+  lp = F.log_softmax(logits / tau, -1).gather(-1, at)
+  kl = (tt.exp() * (tt - lp)).sum(-1)
+  nll = -F.log_softmax(logits, -1).gather(-1, labels[:, None])[:, 0]
+  want = (0.7 * kl + 0.3 * nll).mean()
+  want_grad, = torch.autograd.grad(want, tb)
+  assert torch.equal(top.ids, at)
+  # a logit that lies within its product's fp32 error of a border rounds to the other side: half a step of 2^-8
+  assert abs(float(loss.detach()) - float(want.detach())) <= 2.0 ** -8 * float(logits.detach().abs().max())
+  # the gradients of the logits, of the hidden state and of each use of the table are rounded to bf16 (2^-8 each), a
+  # logit on a border moves its probability by at most half a step of its size
+  rel = float((grad.to(f64) - want_grad).norm() / want_grad.norm())
+  assert rel <= 4 * 2.0 ** -8 + 2.0 ** -8 * float(logits.detach().abs().max())
+
+
+@pytest.mark.gpu
+def test_captured_step_and_two_streams(kernel_lib):
+  V, D, T, k, tau = 5000, 64, 400, 20, 1.3
+  g = torch.Generator().manual_seed(0)
+  table = torch.nn.Parameter((torch.randn(V, D, generator=g) * 0.3).to(bf16).cuda())
+  inputs = [(torch.randint(0, 40, (T,), generator=g).cuda(), (torch.randn(T, V, generator=g) * 2).cuda(),
+             torch.randint(0, V, (T,), generator=g).cuda()) for _ in range(2)]
+
+  def run(i):
+    loss, grad, top = step(table, i[0], i[1], i[2], k, tau)
+    return loss.detach(), grad, top.ids, top.top, top.target
+
+  static = [x.clone() for x in inputs[0]]
+  side = torch.cuda.Stream()
+  side.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(side):
+    for _ in range(2):
+      run(static)
+  torch.cuda.current_stream().wait_stream(side)
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    captured = run(static)
+  want = [[x.clone() for x in run(i)] for i in inputs]
+  torch.cuda.synchronize()
+  for which in (0, 1, 0):
+    for dst, src in zip(static, inputs[which]):
+      dst.copy_(src)
+    graph.replay()
+    for a, b in zip(captured, want[which]):
+      assert torch.equal(a, b)
+  torch.cuda.synchronize()
+  streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+  for n, s in enumerate(streams):
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+      got.append([run(inputs[n]) for _ in range(4)])
+  graph.replay()
+  torch.cuda.synchronize()
+  for n in range(2):
+    for r in got[n]:
+      assert all(torch.equal(a, b) for a, b in zip(r, want[n]))

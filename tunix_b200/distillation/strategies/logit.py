@@ -1,11 +1,17 @@
 """Logit distillation: alpha * tau^2 * KL(teacher || student) at temperature tau plus
 (1 - alpha) * cross entropy, with optional restriction to the teacher's top-k logits
-(tunix/distillation/strategies/logit.py:28-169)."""
+(tunix/distillation/strategies/logit.py:28-169).
+
+With a top-k the GPU runs two operators instead of passes over [.., V] in fp32: `top_logprobs` makes the teacher's list
+(and its loss on integer labels) and `top_distill_loss` reads the student's logits once. A teacher's list may also stand
+in the place of its logits: a `teacher_forward_fn` that returns `ops.functional.TopLogprobs`, computed on the spot or
+stored earlier, keeps k numbers per token instead of V."""
 from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
 
+from ...ops import functional, kernels
 from .base_strategy import BaseStrategy, softmax_cross_entropy
 
 
@@ -22,7 +28,32 @@ class LogitStrategy(BaseStrategy):
   def compute_eval_loss(self, student_output, labels):
     return softmax_cross_entropy(student_output, labels).mean(), {}
 
+  def _compute_listed_loss(self, student_output, teacher_output, labels):
+    V = student_output.shape[-1]
+    ids = labels.long() if not labels.is_floating_point() and labels.ndim == student_output.ndim - 1 else None
+    if isinstance(teacher_output, functional.TopLogprobs):
+      top = teacher_output
+      teacher = None if top.target is None else -top.target.mean()
+    else:
+      with torch.no_grad():
+        top = functional.top_logprobs(teacher_output.detach(), self.distill_top_k, ids)
+        teacher = -top.target.mean() if ids is not None else softmax_cross_entropy(teacher_output, labels).mean()
+    k = min(top.ids.shape[-1], self.distill_top_k or V)
+    terms = functional.top_distill_loss(student_output, top.ids[..., :k], top.top.detach()[..., :k], ids, self.temperature)
+    soft = (terms.kl * self.temperature ** 2).mean()
+    hard = terms.nll.mean() if ids is not None else softmax_cross_entropy(student_output, labels).mean()
+    loss = self.alpha * soft + (1.0 - self.alpha) * hard
+    metrics = {"distill/soft_loss": soft.detach(), "distill/hard_loss": hard.detach(),
+               "distill/kl_div": terms.kl.mean().detach()}
+    if teacher is not None:
+      metrics["distill/teacher_loss"] = teacher.detach()
+    return loss, metrics
+
   def compute_loss(self, student_output, teacher_output, labels):
+    if isinstance(teacher_output, functional.TopLogprobs) or (
+        student_output.is_cuda and 0 < self.distill_top_k <= min(kernels.MAX_TOP_K, teacher_output.shape[-1])
+        and {student_output.dtype, teacher_output.dtype} <= {torch.float32, torch.bfloat16}):
+      return self._compute_listed_loss(student_output, teacher_output, labels)
     s, t = student_output.float(), teacher_output.float()
     sk, tk = s, t
     if self.distill_top_k > 0:
