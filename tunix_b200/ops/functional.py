@@ -289,7 +289,10 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> tor
   fp32 sums rounded once, straight into `main_grad` where the table has one."""
   if _use_kernels(table) and table.shape[1] % 8 == 0:
     flat = ids if ids.dim() == 1 else ids.reshape(-1)
-    out = _EmbeddingFn.apply(flat, table, scale)
+    if table.requires_grad and torch.is_grad_enabled():
+      out = _EmbeddingFn.apply(flat, table, scale)
+    else:
+      out = kernels.embedding_fwd(flat, table, scale)
     return out if ids.dim() == 1 else out.view(*ids.shape, table.shape[1])
   return ref.embedding(ids, table, scale)
 
@@ -474,22 +477,22 @@ class _TopDistillFn(torch.autograd.Function):
     return dx, None, None, None, None, None
 
 
-def _check_rows(name: str, logits: torch.Tensor, temperature: float, **indexed) -> None:
-  """Arguments that `top_logprobs` and `top_distill_loss` share: floating logits [..., V], a positive temperature,
-  integer tensors on the logits' device."""
+def _check_rows(name: str, logits: torch.Tensor, temperature: float) -> None:
+  """Arguments that `top_logprobs` and `top_distill_loss` share: floating logits [..., V], a positive temperature."""
   if logits.dim() < 1 or not logits.is_floating_point():
     raise ValueError(f"{name}: logits must be a floating tensor [..., V], got {logits.dtype} {tuple(logits.shape)}")
-  if not (temperature > 0 and math.isfinite(temperature)):
+  if not 0.0 < temperature < math.inf:
     raise ValueError(f"{name}: temperature must be positive and finite, got {temperature}")
-  for what, (t, shape) in indexed.items():
-    if t is None:
-      continue
-    if t.dtype not in (torch.int32, torch.int64):
-      raise ValueError(f"{name}: {what} must be int32 or int64, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
-      raise ValueError(f"{name}: {what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    if t.device != logits.device:
-      raise ValueError(f"{name}: {what} is on {t.device}, the logits on {logits.device}")
+
+
+def _check_index(name: str, what: str, t: torch.Tensor, shape, logits: torch.Tensor) -> None:
+  """An integer tensor of this shape on the logits' device."""
+  if t.dtype != torch.int64 and t.dtype != torch.int32:
+    raise ValueError(f"{name}: {what} must be int32 or int64, got {t.dtype}")
+  if t.shape != shape:
+    raise ValueError(f"{name}: {what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+  if t.device != logits.device:
+    raise ValueError(f"{name}: {what} is on {t.device}, the logits on {logits.device}")
 
 
 def _rows(name: str, logits: torch.Tensor) -> Optional[torch.Tensor]:
@@ -525,9 +528,10 @@ def top_logprobs(logits: torch.Tensor, k: int, targets: Optional[torch.Tensor] =
   is ignored (0, no gradient). Logits of -inf are masked out; a row that has nothing else gets log-probabilities of
   -inf, entropy 0 and no gradient. fp32 and bf16 logits on the GPU, rows of any alignment and stride, take one
   kernel in each direction; there `k` is at most 256."""
-  V = logits.shape[-1] if logits.dim() else 0
-  lead = logits.shape[:-1]
-  _check_rows("top_logprobs", logits, temperature, targets=(targets, lead))
+  _check_rows("top_logprobs", logits, temperature)
+  V, lead = logits.shape[-1], logits.shape[:-1]
+  if targets is not None:
+    _check_index("top_logprobs", "targets", targets, lead, logits)
   k = int(k)
   if not 1 <= k <= V:
     raise ValueError(f"top_logprobs: k must be between 1 and the vocabulary's {V}, got {k}")
@@ -538,7 +542,10 @@ def top_logprobs(logits: torch.Tensor, k: int, targets: Optional[torch.Tensor] =
   else:
     if k > kernels.MAX_TOP_K:
       raise ValueError(f"top_logprobs: k is at most {kernels.MAX_TOP_K} on the GPU, got {k}")
-    ids, top, target, ent = _TopLogprobsFn.apply(x2, k, tg, 1.0 / float(temperature), bool(want_entropy))
+    if x2.requires_grad and torch.is_grad_enabled():
+      ids, top, target, ent = _TopLogprobsFn.apply(x2, k, tg, 1.0 / float(temperature), bool(want_entropy))
+    else:
+      ids, top, target, ent, _ = kernels.top_logprobs_fwd(x2, k, tg, 1.0 / float(temperature), bool(want_entropy))
   return TopLogprobs(_lead(ids, *lead, k), _lead(top, *lead, k), _lead(target, *lead), _lead(ent, *lead))
 
 
@@ -558,15 +565,17 @@ def top_distill_loss(logits: torch.Tensor, top_ids: torch.Tensor, top_values: to
   ignored; an entry of probability 0 adds nothing. A row without a usable entry (no id left, teacher's values all
   -inf, student's logits there all -inf) has divergence 0 and no gradient, a row of -inf also no cross entropy.
   fp32 and bf16 logits on the GPU take one kernel in each direction; there the list has at most 1024 entries."""
-  lead = logits.shape[:-1]
-  V = logits.shape[-1] if logits.dim() else 0
+  _check_rows("top_distill_loss", logits, temperature)
+  V, lead = logits.shape[-1], logits.shape[:-1]
   k = top_ids.shape[-1] if top_ids.dim() else 0
-  _check_rows("top_distill_loss", logits, temperature, top_ids=(top_ids, (*lead, k)), labels=(labels, lead))
+  _check_index("top_distill_loss", "top_ids", top_ids, (*lead, k), logits)
+  if labels is not None:
+    _check_index("top_distill_loss", "labels", labels, lead, logits)
   if normalize not in ("top", "full"):
     raise ValueError(f"top_distill_loss: normalize must be 'top' or 'full', got {normalize!r}")
   if k < 1 or V < 1:
     raise ValueError(f"top_distill_loss: needs a list of at least one entry and a vocabulary, got k={k}, V={V}")
-  if tuple(top_values.shape) != tuple(top_ids.shape) or not top_values.is_floating_point():
+  if top_values.shape != top_ids.shape or not top_values.is_floating_point():
     raise ValueError(f"top_distill_loss: top_values must be floating and shaped like top_ids {tuple(top_ids.shape)}, "
                      f"got {top_values.dtype} {tuple(top_values.shape)}")
   if top_values.device != logits.device:
@@ -581,6 +590,11 @@ def top_distill_loss(logits: torch.Tensor, top_ids: torch.Tensor, top_values: to
   else:
     if k > kernels.MAX_TOP_LIST:
       raise ValueError(f"top_distill_loss: the list has at most {kernels.MAX_TOP_LIST} entries on the GPU, got {k}")
-    values = top_values.detach().reshape(-1, k).float().contiguous()
-    kl, nll = _TopDistillFn.apply(x2, ids, values, tg, 1.0 / float(temperature), full)
+    values = top_values
+    if values.dtype != torch.float32 or values.dim() != 2 or values.requires_grad or not values.is_contiguous():
+      values = values.detach().reshape(-1, k).float().contiguous()
+    if x2.requires_grad and torch.is_grad_enabled():
+      kl, nll = _TopDistillFn.apply(x2, ids, values, tg, 1.0 / float(temperature), full)
+    else:
+      kl, nll, _ = kernels.top_distill_fwd(x2, ids, values, tg, 1.0 / float(temperature), full)
   return DistillLoss(_lead(kl, *lead), _lead(nll, *lead))
