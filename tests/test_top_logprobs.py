@@ -500,3 +500,13 @@ def test_refusals_of_the_kernels():
     F.top_distill_loss(x, ids, ids.float())
   with pytest.raises(ValueError, match="on cpu"):
     F.top_logprobs(x, 3, torch.zeros(2, dtype=torch.long))
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused():
+  x = torch.randn(3, 500, device="cuda", requires_grad=True)
+  ids, values = make_list(x, 4)
+  for out in (F.top_logprobs(x, 4).top, F.top_distill_loss(x, ids, values).kl):
+    g, = torch.autograd.grad(out.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="no second derivative"):
+      g.sum().backward()

@@ -1123,14 +1123,20 @@ int launch_rows(int T, int blocks, int bytes, cudaStream_t s, Args... args) {
   return cudaLaunchKernelEx(&cfg, Kernel, args...) == cudaSuccess ? 0 : 400;
 }
 
-// n 16-byte vectors. Blocks of 16 KB that end at once: 7.4 TB/s, where 1184 blocks that loop over the same tiles write
-// 6.1 TB/s (1.24 GB).
+// n bytes (a multiple of 2) from a 16-byte boundary. Blocks of 16 KB that end at once: 7.4 TB/s, where 1184 blocks that
+// loop over the same tiles write 6.1 TB/s (1.24 GB).
 constexpr int kClearThreads = 512, kClearVecs = 2;
-__global__ void __launch_bounds__(kClearThreads) clear_kernel(uint4* p, long long n) {
+__global__ void __launch_bounds__(kClearThreads) clear_kernel(unsigned char* p, long long n) {
   const long long at = blockIdx.x * static_cast<long long>(kClearThreads * kClearVecs) + threadIdx.x;
 #pragma unroll
-  for (int i = 0; i < kClearVecs; ++i)
-    if (at + i * kClearThreads < n) p[at + i * kClearThreads] = make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < kClearVecs; ++i) {
+    const long long byte = (at + i * kClearThreads) * 16;
+    if (byte + 16 <= n) {
+      *reinterpret_cast<uint4*>(p + byte) = make_uint4(0, 0, 0, 0);
+    } else {
+      for (long long b = byte; b < n; b += 2) *reinterpret_cast<uint16_t*>(p + b) = 0;
+    }
+  }
 }
 
 template <typename LT>
@@ -1140,14 +1146,9 @@ int launch_bwd(BwdArgs a, int dense, cudaStream_t s) {
   a.blocks = max((a.V + kBwdPart - 1) / kBwdPart, min(most, (want + a.T - 1) / a.T));
   if (dense == 0) {
     a.blocks = 1;
-    const long long bytes = ((a.T - 1) * a.ldd + a.V) * static_cast<long long>(sizeof(LT));
-    const long long n = reinterpret_cast<uintptr_t>(a.dx) % 16 == 0 && a.ldd == a.V ? bytes / 16 : 0;
-    if (n > 0)
-      clear_kernel<<<static_cast<unsigned>((n + kClearThreads * kClearVecs - 1) / (kClearThreads * kClearVecs)), kClearThreads, 0, s>>>(
-          static_cast<uint4*>(a.dx), n);
-    if (bytes > n * 16 && cudaMemset2DAsync(static_cast<char*>(a.dx) + n * 16, n ? bytes - n * 16 : a.ldd * sizeof(LT), 0,
-                                            n ? bytes - n * 16 : a.V * sizeof(LT), n ? 1 : a.T, s) != cudaSuccess)
-      return 403;
+    const long long bytes = a.T * a.ldd * static_cast<long long>(sizeof(LT)), tile = 16 * kClearThreads * kClearVecs;
+    clear_kernel<<<static_cast<unsigned>((bytes + tile - 1) / tile), kClearThreads, 0, s>>>(
+        static_cast<unsigned char*>(a.dx), bytes);
   }
 #define TX_BWD(D) case D: top_bwd_kernel<LT, D><<<a.T * a.blocks, kThreads, 0, s>>>(a); break
   switch (dense) {
@@ -1198,29 +1199,30 @@ extern "C" int tx_top_distill_fwd(const void* logits, int logits_fp32, long long
                      : launch_rows<distill_fwd_kernel<__nv_bfloat16, kNone>>(T, n, 0, s, a, c1, c);
 }
 
-// Gradient of tx_top_logprob_fwd: g_top or null, g_target with targets or null, g_entropy with entropy or null.
+// Gradient of tx_top_logprob_fwd: g_top or null, g_target with targets or null, g_entropy with entropy or null. dx is
+// [T, V], dense, from a 16-byte boundary.
 extern "C" int tx_top_logprob_bwd(const void* logits, int logits_fp32, long long ld, int T, int V, int k,
                                   float inv_temp, const long long* ids, const float* g_top, const long long* targets,
                                   const float* g_target, const float* g_entropy, const float* entropy,
-                                  const float* stats, void* dx, long long ldd, cudaStream_t s) {
+                                  const float* stats, void* dx, cudaStream_t s) {
   if (T <= 0) return 0;
   if (V < 1 || k < 1 || k > kMaxTop || V > 0x7fff0000) return 1;
   const BwdArgs a{logits, ld, T, V, k, kScore, inv_temp, ids, g_top, targets, nullptr, g_target, g_entropy, entropy,
-                  stats, dx, ldd, 1, 0};
+                  stats, dx, V, 1, 0};
   const int dense = g_entropy ? 5 : 1;
   return logits_fp32 ? launch_bwd<float>(a, dense, s) : launch_bwd<__nv_bfloat16>(a, dense, s);
 }
 
-// Gradient of tx_top_distill_fwd; g_kl or g_nll may be null.
+// Gradient of tx_top_distill_fwd; g_kl or g_nll may be null. dx as above.
 extern "C" int tx_top_distill_bwd(const void* logits, int logits_fp32, long long ld, int T, int V, int k,
                                   float inv_temp, int full, const long long* ids, const float* values,
                                   const long long* labels, const float* g_kl, const float* g_nll, const float* stats,
-                                  void* dx, long long ldd, cudaStream_t s) {
+                                  void* dx, cudaStream_t s) {
   if (T <= 0) return 0;
   if (V < 1 || k < 1 || k > kMaxList || V > 0x7fff0000) return 1;
   const int both = full && g_kl && g_nll && inv_temp == 1.f;
   const BwdArgs a{logits, ld, T, V, k, full ? kFull : kListed, inv_temp, ids, values, labels, g_kl, g_nll, nullptr,
-                  nullptr, stats, dx, ldd, 1, both};
+                  nullptr, stats, dx, V, 1, both};
   const int dense = (full && g_kl ? 1 : 0) | (g_nll && !both ? 2 : 0);
   return logits_fp32 ? launch_bwd<float>(a, dense, s) : launch_bwd<__nv_bfloat16>(a, dense, s);
 }

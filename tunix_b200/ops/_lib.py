@@ -82,9 +82,9 @@ def _declare(lib):
       "tx_logprob_fwd": [P, I, L, P, P, P, P, I, I, F, F, P],
       "tx_logprob_bwd": [P, I, L, P, P, P, P, P, P, L, I, I, I, F, F, P],
       "tx_top_logprob_fwd": [P, I, L, I, I, I, F, P, P, P, P, P, P, P],
-      "tx_top_logprob_bwd": [P, I, L, I, I, I, F, P, P, P, P, P, P, P, P, L, P],
+      "tx_top_logprob_bwd": [P, I, L, I, I, I, F, P, P, P, P, P, P, P, P, P],
       "tx_top_distill_fwd": [P, I, L, I, I, I, F, I, P, P, P, P, P, P, P],
-      "tx_top_distill_bwd": [P, I, L, I, I, I, F, I, P, P, P, P, P, P, P, L, P],
+      "tx_top_distill_bwd": [P, I, L, I, I, I, F, I, P, P, P, P, P, P, P, P],
   }
   for name, argtypes in sigs.items():
     fn = getattr(lib, name, None)

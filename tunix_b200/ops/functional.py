@@ -434,47 +434,53 @@ def _grad32(g: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
   return g.float().contiguous()
 
 
+def _once(dx: torch.Tensor) -> torch.Tensor:
+  """A gradient that cannot be differentiated again: where a graph of the backward pass is built, an error is put
+  behind it (the softmax's own derivative would silently be missing)."""
+  if not torch.is_grad_enabled():
+    return dx
+  error = torch._C._functions.DelayedError(b"top_logprobs and top_distill_loss have no second derivative", 1)
+  return error(dx.detach().requires_grad_())
+
+
 class _TopLogprobsFn(torch.autograd.Function):
 
   @staticmethod
   def forward(ctx, x2, k, targets, inv_temp, want_entropy):
-    ids, top, target, ent, stats = kernels.top_logprobs_fwd(x2, k, targets, inv_temp, want_entropy)
-    ctx.save_for_backward(x2, ids, targets, stats, ent)
+    ids, top, target, ent, ctx.stats = kernels.top_logprobs_fwd(x2, k, targets, inv_temp, want_entropy)
+    ctx.save_for_backward(x2, ids, targets, ent)
     ctx.inv_temp = inv_temp
     ctx.mark_non_differentiable(ids)
     ctx.set_materialize_grads(False)
     return ids, top, target, ent
 
   @staticmethod
-  @torch.autograd.function.once_differentiable
   def backward(ctx, _, g_top, g_target, g_ent):
-    x2, ids, targets, stats, ent = ctx.saved_tensors
+    x2, ids, targets, ent = ctx.saved_tensors
     if g_top is None and g_target is None and g_ent is None:
       return None, None, None, None, None
-    dx = kernels.top_logprobs_bwd(x2, ids, targets, stats, ent, _grad32(g_top), _grad32(g_target), _grad32(g_ent),
+    dx = kernels.top_logprobs_bwd(x2, ids, targets, ctx.stats, ent, _grad32(g_top), _grad32(g_target), _grad32(g_ent),
                                   ctx.inv_temp)
-    return dx, None, None, None, None
+    return _once(dx), None, None, None, None
 
 
 class _TopDistillFn(torch.autograd.Function):
 
   @staticmethod
   def forward(ctx, x2, ids, values, labels, inv_temp, full):
-    kl, nll, stats = kernels.top_distill_fwd(x2, ids, values, labels, inv_temp, full)
-    ctx.save_for_backward(x2, ids, values, labels, stats)
+    kl, nll, ctx.stats = kernels.top_distill_fwd(x2, ids, values, labels, inv_temp, full)
+    ctx.save_for_backward(x2, ids, values, labels)
     ctx.cfg = (inv_temp, full)
     ctx.set_materialize_grads(False)
     return kl, nll
 
   @staticmethod
-  @torch.autograd.function.once_differentiable
   def backward(ctx, g_kl, g_nll):
-    x2, ids, values, labels, stats = ctx.saved_tensors
-    inv_temp, full = ctx.cfg
+    x2, ids, values, labels = ctx.saved_tensors
     if g_kl is None and g_nll is None:
       return None, None, None, None, None, None
-    dx = kernels.top_distill_bwd(x2, ids, values, labels, stats, _grad32(g_kl), _grad32(g_nll), inv_temp, full)
-    return dx, None, None, None, None, None
+    dx = kernels.top_distill_bwd(x2, ids, values, labels, ctx.stats, _grad32(g_kl), _grad32(g_nll), *ctx.cfg)
+    return _once(dx), None, None, None, None, None
 
 
 def _check_rows(name: str, logits: torch.Tensor, temperature: float) -> None:

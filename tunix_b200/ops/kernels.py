@@ -295,7 +295,7 @@ def top_logprobs_bwd(logits, ids, targets, stats, entropy, g_top, g_target, g_en
   _lib.check_rc(_lib.require().tx_top_logprob_bwd(
       logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0), T, V, ids.shape[1], float(inv_temp),
       ids.data_ptr(), _p(g_top), _p(targets), _p(g_target), _p(g_entropy), _p(entropy), stats.data_ptr(),
-      dx.data_ptr(), V, _lib.stream_ptr()), "tx_top_logprob_bwd")
+      dx.data_ptr(), _lib.stream_ptr()), "tx_top_logprob_bwd")
   return dx
 
 
@@ -323,7 +323,7 @@ def top_distill_bwd(logits, ids, values, labels, stats, g_kl, g_nll, inv_temp: f
   _lib.check_rc(_lib.require().tx_top_distill_bwd(
       logits.data_ptr(), int(logits.dtype == torch.float32), logits.stride(0), T, V, ids.shape[1], float(inv_temp),
       int(full), ids.data_ptr(), values.data_ptr(), _p(labels), _p(g_kl), _p(g_nll), stats.data_ptr(), dx.data_ptr(),
-      V, _lib.stream_ptr()), "tx_top_distill_bwd")
+      _lib.stream_ptr()), "tx_top_distill_bwd")
   return dx
 
 
