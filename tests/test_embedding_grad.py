@@ -163,3 +163,28 @@ def test_captured_backward_and_two_streams(kernel_lib):
   torch.cuda.synchronize()
   assert torch.equal(captured, second)
   assert all(torch.equal(r, second) for rs in results for r in rs)
+
+
+@pytest.mark.gpu
+def test_tables_and_batches_beyond_32_bits(kernel_lib):
+  from tunix_b200.ops import kernels
+  V, D = 600_000, 4096                                                   # 2.5e9 elements of the table
+  ids = torch.tensor([V - 1, 5, V - 1, V - 2], device="cuda")
+  dout = torch.randn(4, D, device="cuda").to(bf16)
+  grad = torch.empty(V, D, device="cuda", dtype=bf16)
+  kernels.embedding_bwd(ids, dout, grad)
+  assert torch.equal(grad[V - 1], (dout[0].float() + dout[2].float()).to(bf16))
+  assert torch.equal(grad[V - 2], dout[3]) and torch.equal(grad[5], dout[1])
+  assert int((grad != 0).any(1).sum()) == 3
+  assert torch.equal(kernels.embedding_fwd(ids, grad), grad[ids])
+  del grad
+  T, V = 600_000, 7                                                      # 2.5e9 elements of the batch
+  ids = torch.full((T,), 3, device="cuda")
+  ids[-2:] = 6
+  dout = torch.zeros(T, D, device="cuda", dtype=bf16)
+  dout[::1000] = 1.0
+  dout[-2:] = torch.randn(2, D, device="cuda").to(bf16)
+  grad = torch.zeros(V, D, device="cuda")
+  kernels.embedding_bwd(ids, dout, grad)
+  assert torch.equal(grad[6], dout[-2].float() + dout[-1].float())
+  assert float((grad[3] - T / 1000).abs().max()) == 0.0                  # 600 ones: exact in fp32

@@ -287,7 +287,7 @@ def test_top_logprobs(device, dtype, T, V, k, tau, entropy):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("V,k", [(6, 3), (300, 40), (5000, 256), (20011, 33)])
+@pytest.mark.parametrize("V,k", [(6, 3), (300, 40), (5000, 256), (20011, 33), (140001, 200)])
 def test_top_logprobs_of_odd_rows(device, dtype, V, k):
   x = odd_rows(V, dtype, device)
   targets = torch.arange(x.shape[0], device=device) % V
@@ -510,3 +510,60 @@ def test_second_derivatives_are_refused():
     g, = torch.autograd.grad(out.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="no second derivative"):
       g.sum().backward()
+
+
+@pytest.mark.gpu
+def test_blocks_of_logits_beyond_32_bits():
+  """Rows behind the 2^31st element of a block, and their gradients."""
+  T, V, k = 17000, 131072, 10
+  x = torch.zeros(T, V, device="cuda", dtype=torch.bfloat16)
+  x[-4:] = make_logits(4, V, torch.bfloat16, "cuda")
+  x.requires_grad_()
+  last = x.detach()[-4:]
+  targets = torch.arange(T, device="cuda")
+  got = F.top_logprobs(x, k, targets)
+  want = score64(last, k, targets[-4:], 1.0, torch.ones(4, k, device="cuda"))
+  assert torch.equal(got.ids[-4:], want["ids"])
+  close(got.top[-4:], want["top"], lp_tol(last, 1.0).gather(1, want["ids"]), "top")
+  assert torch.equal(got.ids[0], torch.arange(k, device="cuda"))
+  g, = torch.autograd.grad(got.top, x, torch.ones(T, k, device="cuda"))
+  tol = (k + 2) * p_tol(last, 1.0) + (k + 8) * U * (1 + log_softmax64(last.to(f64)).exp()) \
+      + 2.0 ** -8 * want["grad"].abs() * (1 + 2 ** -6) + 2.0 ** -130
+  close(g[-4:], want["grad"], tol, "gradient")
+  del got, g
+  ids, values = make_list(last, k)
+  ids, values = ids.repeat(T // 4, 1), values.repeat(T // 4, 1)
+  loss = F.top_distill_loss(x, ids, values, None, temperature=2.0)
+  g, = torch.autograd.grad(loss.kl.sum(), x)
+  alone = distill64(last, ids[-4:], values[-4:], None, 2.0, False, torch.ones(4))
+  assert float((loss.kl[-4:].detach().to(f64) - alone["kl"]).abs().max()) <= 1e-4
+  assert float((g[-4:].to(f64) - alone["grad"]).abs().max()) <= 2.0 ** -8
+  assert int((g[0] != 0).sum()) <= k and int((g[T // 2] != 0).sum()) <= k
+
+
+@pytest.mark.gpu
+def test_another_device_than_the_process_is_refused(monkeypatch):
+  from tunix_b200.ops import _lib
+  x = torch.randn(2, 100, device="cuda")
+  ids, values = make_list(x, 3)
+  monkeypatch.setattr(_lib, "bind_thread", lambda: 1)
+  with pytest.raises(ValueError, match="this process drives cuda:1"):
+    F.top_logprobs(x, 3)
+  with pytest.raises(ValueError, match="this process drives cuda:1"):
+    F.top_distill_loss(x, ids, values)
+
+
+@pytest.mark.gpu
+def test_repeated_calls_agree_to_the_bit():
+  """Candidates are collected in any order; what is reported does not depend on it."""
+  x = make_logits(40, 50000, torch.bfloat16, "cuda")
+  targets = torch.arange(40, device="cuda")
+  first = F.top_logprobs(x, 64, targets, want_entropy=True)
+  many = x.repeat(20, 1)                           # another number of blocks per row
+  other = F.top_logprobs(many, 64, targets.repeat(20), want_entropy=True)
+  for _ in range(5):
+    again = F.top_logprobs(x, 64, targets, want_entropy=True)
+    more = F.top_logprobs(many, 64, targets.repeat(20), want_entropy=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    assert all(torch.equal(a, b) for a, b in zip(other, more))
+  assert torch.equal(first.ids, other.ids[:40])
