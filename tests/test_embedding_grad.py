@@ -102,6 +102,26 @@ def test_buffer_at_an_odd_offset(kernel_lib):
     kernels.embedding_bwd(ids, dout, flat[off:off + 40 * 32].view(40, 32))
     assert torch.equal(flat[off:off + 40 * 32].view(40, 32), want)
     assert float(flat[:off].abs().sum()) == 0 and float(flat[off + 40 * 32:].abs().sum()) == 0
+  small = torch.full((40 * 32 + 9,), 3.0, device="cuda", dtype=bf16)
+  kernels.embedding_bwd(ids, dout, small[3:3 + 40 * 32].view(40, 32))
+  assert torch.equal(small[3:3 + 40 * 32].view(40, 32), want.to(bf16))
+  assert bool((small[:3] == 3).all()) and bool((small[3 + 40 * 32:] == 3).all())
+
+
+@pytest.mark.gpu
+def test_tables_that_the_kernels_do_not_take(kernel_lib):
+  """Views of wider tables and tables at odd offsets get the plain statement, ids on the host an error."""
+  ids = id_list("padded", 50, 30).cuda()
+  wide = torch.randn(30, 48, device="cuda").to(bf16)
+  flat = torch.randn(30 * 32 + 1, device="cuda").to(bf16)
+  for table in (wide[:, :32], flat[1:].view(30, 32)):
+    leaf = table.detach().requires_grad_()
+    out = F.embedding(ids, leaf, 2.0)
+    assert torch.equal(out, (table[ids].float() * 2.0).to(bf16))
+    out.float().sum().backward()
+    assert leaf.grad.shape == (30, 32)
+  with pytest.raises(ValueError, match="ids are on cpu"):
+    F.embedding(ids.cpu(), wide.contiguous())
 
 
 @pytest.mark.parametrize("device", DEVICES)

@@ -461,7 +461,7 @@ def test_refusals(device):
   for k in (0, -1, 41):
     with pytest.raises(ValueError, match="k must be between"):
       F.top_logprobs(x, k)
-  for bad in (0.0, -1.0, math.inf, math.nan):
+  for bad in (0.0, -1.0, 1e-19, 1e19, math.inf, math.nan):
     with pytest.raises(ValueError, match="temperature"):
       F.top_logprobs(x, 3, temperature=bad)
     with pytest.raises(ValueError, match="temperature"):
@@ -567,3 +567,20 @@ def test_repeated_calls_agree_to_the_bit():
     assert all(torch.equal(a, b) for a, b in zip(first, again))
     assert all(torch.equal(a, b) for a, b in zip(other, more))
   assert torch.equal(first.ids, other.ids[:40])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("tau", [1e-18, 1e-6, 1e-3, 1e3, 1e18])
+def test_extreme_temperatures(device, tau):
+  """Cold: one token takes everything (the smallest temperatures leave the range in which sums are taken in one pass).
+  Hot: all tokens are alike."""
+  x = make_logits(3, 6000, torch.float32, device)
+  x[:, 77] = x.amax(1) + 1.0                                       # a clear best token
+  got = F.top_logprobs(x, 5, torch.zeros(3, dtype=torch.long, device=device), temperature=tau, want_entropy=True)
+  want = score64(x, 5, torch.zeros(3, dtype=torch.long, device=device), tau)
+  assert torch.equal(got.ids, want["ids"])
+  close(got.top, want["top"], lp_tol(x, tau).gather(1, want["ids"]), "top")
+  close(got.target, want["target"], lp_tol(x, tau)[:, 0], "target")
+  p, lp = log_softmax64(x.to(f64) / tau).exp(), log_softmax64(x.to(f64) / tau)
+  size = torch.where(p > 0, p * lp.abs(), torch.zeros_like(p)).sum(1) + math.log(6001)
+  close(got.entropy, want["entropy"], 4 * lse_tol(x, tau) * (1 + size) + U * 100 * size, "entropy")

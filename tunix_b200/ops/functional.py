@@ -287,7 +287,9 @@ class _EmbeddingFn(torch.autograd.Function):
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
   """Rows of `table` [V, D] times `scale`. The table's gradient is summed by sorted tokens: repeatable to the bit,
   fp32 sums rounded once, straight into `main_grad` where the table has one."""
-  if _use_kernels(table) and table.shape[1] % 8 == 0:
+  if _use_kernels(table) and table.shape[1] % 8 == 0 and table.is_contiguous() and table.data_ptr() % 16 == 0:
+    if not ids.is_cuda:
+      raise ValueError(f"embedding: ids are on {ids.device}, the table on {table.device}")
     flat = ids if ids.dim() == 1 else ids.reshape(-1)
     if table.requires_grad and torch.is_grad_enabled():
       out = _EmbeddingFn.apply(flat, table, scale)
@@ -487,8 +489,8 @@ def _check_rows(name: str, logits: torch.Tensor, temperature: float) -> None:
   """Arguments that `top_logprobs` and `top_distill_loss` share: floating logits [..., V], a positive temperature."""
   if logits.dim() < 1 or not logits.is_floating_point():
     raise ValueError(f"{name}: logits must be a floating tensor [..., V], got {logits.dtype} {tuple(logits.shape)}")
-  if not 0.0 < temperature < math.inf:
-    raise ValueError(f"{name}: temperature must be positive and finite, got {temperature}")
+  if not 1e-18 <= temperature <= 1e18:       # its inverse and products with logits stay within fp32
+    raise ValueError(f"{name}: temperature must be positive and finite (1e-18 to 1e18), got {temperature}")
 
 
 def _check_index(name: str, what: str, t: torch.Tensor, shape, logits: torch.Tensor) -> None:

@@ -177,7 +177,7 @@ def embedding_bwd(ids: torch.Tensor, dout: torch.Tensor, grad_table: torch.Tenso
   T = ids.numel()
   V, D = grad_table.shape
   assert dout.dtype == bf16 and dout.is_contiguous() and dout.numel() == T * D and grad_table.is_contiguous()
-  assert grad_table.dtype in (bf16, torch.float32)
+  assert grad_table.dtype in (bf16, torch.float32) and T < 2 ** 31 and ids.is_cuda
   if dout.data_ptr() % 16:
     dout = dout.clone()
   lib = _lib.require()
