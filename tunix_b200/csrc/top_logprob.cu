@@ -4,12 +4,13 @@
 //    values by the lowest id) and the entropy of softmax(x * inv_temp), in one pass over the row.
 //  * tx_top_distill_fwd: per row the divergence from a teacher's list of (id, value) pairs and the cross entropy of
 //    a label, in one pass over the student's row (none at all when only the listed entries matter).
-//  * tx_top_bwd: the gradient of either with respect to the row, one read and one write.
+//  * tx_top_logprob_bwd, tx_top_distill_bwd: the gradient of either with respect to the row, one read and one write
+//    (one write alone where the dense part of the gradient is zero).
 //
 // With m = max x, d_j = x_j - m and c = inv_temp * log2(e):  s = sum 2^(d_j c),  log p_j = d_j inv_temp - ln s.
-// Everything is kept relative to m, so log-probabilities do not lose the bits of a large log-sum-exp, and the
-// running maximum starts at the lowest finite float: a row of -inf sums to 0 instead of to NaN (it is reported as
-// an empty row: ln s is stored as +inf, log-probabilities are -inf, losses and gradients 0).
+// What is reported is kept relative to m, so log-probabilities do not lose the bits of a large log-sum-exp. Sums,
+// maxima and the list's statistics are fp32. A row of -inf is an empty row: ln s is stored as +inf, log-probabilities
+// are -inf, losses and gradients 0.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -699,8 +700,8 @@ __device__ __forceinline__ Stat top_of_part(Select& s, const LT* x, int base, in
     block_max = fmaxf(block_max, s.warp_max[w]);
   }
   if (nth_of > 32) thr0 = -INFINITY;
-  // 64 bins up to the first iteration's maximum; any positive width is correct
-  float width = (block_max - thr0) * (1.f / 64.f);
+  // 128 bins up to the first iteration's maximum; any positive width is correct
+  float width = (block_max - thr0) * (1.f / 128.f);
   if (!(width > 1e-30f && width < 1e30f)) width = 1.f;
   const float inv_width = 1.f / width;
   if (tid == 0) s.thr = thr0;
@@ -781,6 +782,13 @@ __device__ __forceinline__ Stat top_of_part(Select& s, const LT* x, int base, in
 }
 
 // A row per cluster of 1 .. kMaxSplit blocks, each with a part of the columns.
+//
+// Bound by instructions: unpacking, the multiply-add, the exponential and the sum are about 45 per 16-byte vector and
+// warp, of which the special function unit's 8 cycles for each of 8 exponentials are the longest part; the selection
+// adds a quarter of that at k = 64. Five blocks of 256 threads per SM hide one row's serial parts (first threshold, last
+// sort) behind the others' streaming; a ring of asynchronous copies with two blocks per SM instead measured 649 us where
+// this took 415 us. 8192 x 128256 bf16, k = 64: 388 us (5.4 TB/s), k = 1: 344 us; 2047 x 151936 fp32 with entropy, k = 8:
+// 212 us (5.9 TB/s). Under the power cap of a long run the clock falls and these times grow by up to a tenth.
 template <typename LT, int X>
 __global__ void __launch_bounds__(kThreads, X == kNone ? 5 : 4) top_fwd_kernel(TopArgs a) {
   extern __shared__ __align__(16) unsigned char shared[];
@@ -932,7 +940,8 @@ __global__ void __launch_bounds__(kThreads) distill_list_kernel(DistillArgs a) {
   distill_list(a, row, static_cast<const LT*>(a.logits) + static_cast<long long>(row) * a.ld, -FLT_MAX, INFINITY, INFINITY);
 }
 
-// X: kNone (one softmax sum of the row, scale c1 in the exponent) or kSecond (c1 and c2).
+// X: kNone (one softmax sum of the row, scale c1 in the exponent) or kSecond (c1 and c2). One sum is bound by memory
+// (4096 x 128256 bf16: 165 us, 6.4 TB/s), two by the exponentials (4096 x 151936 bf16: 266 us, 4.7 TB/s).
 template <typename LT, int X>
 __global__ void __launch_bounds__(kThreads) distill_fwd_kernel(DistillArgs a, float c1, float c2) {
   __shared__ Stat sh_stat[kWarps];
@@ -992,6 +1001,9 @@ struct BwdArgs {
 
 // d_j = A p_j (temperature) + B p_j (temperature 1) - G p_j (log p_j + H), then the listed columns get their own
 // terms on top: they are computed from the same fp32 value and rounded once, by the thread of the first occurrence.
+//
+// Bound by memory: 4096 x 151936 bf16 with both temperatures 393 us (6.3 TB/s), 1000 x 262144 bf16 with entropy 173 us
+// (6.1 TB/s), soft part alone on 2048 x 151936 fp32 186 us (6.7 TB/s written).
 //
 // A block has a part of kBwdPart columns: the blocks at work at a time then cover few rows from end to end, which the
 // memory takes 4 to 8 % faster than a block per row (4096 x 128256 bf16: 325 us, against 354 us for whole rows and
@@ -1161,7 +1173,8 @@ __global__ void __launch_bounds__(kThreads) top_bwd_kernel(BwdArgs a) {
   }
 }
 
-// Blocks per row of a forward pass: one while the rows fill the GPU, else up to kMaxSplit.
+// Blocks per row of a forward pass: one while the rows fill the GPU, else up to kMaxSplit. One row of 262144 fp32 takes
+// 17 us on eight blocks, eight rows of 151936 bf16 17 us.
 int split_of(int T, int V) {
   int n = 1;
   while (n < kMaxSplit && 2ll * n * T <= 4ll * txh::sm_count() && V / (2 * n) >= kMinPart) n *= 2;
