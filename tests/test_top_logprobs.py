@@ -277,6 +277,7 @@ def eps(dtype):
 @pytest.mark.parametrize("T,V,k,tau,entropy", [
     (1, 1, 1, 1.0, True), (3, 7, 7, 0.5, True), (5, 257, 17, 1.0, False), (2, 256, 256, 2.0, True),
     (4, 1000, 64, 1.0, True), (3, 4097, 256, 1.3, True), (7, 9001, 5, 0.7, False), (2, 32003, 100, 1.0, True),
+    (3, 70001, 256, 1.0, True), (2, 200003, 3, 0.9, True),
 ])
 def test_top_logprobs(device, dtype, T, V, k, tau, entropy):
   x = make_logits(T, V, dtype, device, seed=V)

@@ -33,7 +33,7 @@ constexpr int kKept = 1024;                   // of which this many may reach th
 constexpr int kKeys = 2048;                   // elements that do
 constexpr int kBins = 256;
 constexpr int kMaxSplit = 8;                  // blocks (one cluster) a row is spread over when there are few rows
-constexpr int kMinPart = 4096;                // columns of such a part at least
+constexpr int kMinPart = 4096;                // columns of a part of the backward pass at least
 constexpr int kBwdPart = 32768;               // columns a block of the backward pass takes at most
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFloor = -1e37f;              // lowest running maximum
@@ -438,18 +438,19 @@ __device__ __forceinline__ unsigned long long shfl_key(unsigned long long k, int
   return (static_cast<unsigned long long>(hi) << 32) | lo;
 }
 
-// Sorts n keys (all different) in shared memory from high to low. All threads call it. Short lists: two threads count
-// how many keys are above theirs. Longer ones: bitonic (slots n .. P-1 are filled with 0, P the next power of 2); up to
+// Sorts n keys (all different) in shared memory from high to low. All threads call it. Short lists: four or two threads
+// count how many keys are above theirs. Longer ones: bitonic (slots n .. P-1 are filled with 0, P the next power of 2); up to
 // one key per thread stays in a register and strides below a warp are shuffles.
 __device__ __forceinline__ void sort_keys(unsigned long long* keys, int n) {
   if (n <= kThreads / 2) {
-    const int i = threadIdx.x >> 1;
+    const int per = n <= kThreads / 4 ? 4 : 2, i = threadIdx.x / per, sub = threadIdx.x % per;
     const unsigned long long key = i < n ? keys[i] : 0;
     int above = 0;
-    for (int j = threadIdx.x & 1; j < n; j += 2) above += keys[j] > key;
+    for (int j = sub; j < n; j += per) above += keys[j] > key;
     above += __shfl_xor_sync(0xffffffffu, above, 1);
+    if (per == 4) above += __shfl_xor_sync(0xffffffffu, above, 2);
     __syncthreads();
-    if (i < n && (threadIdx.x & 1) == 0) keys[above] = key;
+    if (i < n && sub == 0) keys[above] = key;
     __syncthreads();
     return;
   }
@@ -811,23 +812,33 @@ __global__ void __launch_bounds__(kThreads, X == kNone ? 5 : 4) top_fwd_kernel(T
     cluster.sync();
     // Every block takes in all parts, in the same order, and counts for its own keys those above them in the others'
     // sorted lists: binary searches through distributed shared memory, side by side.
-    st = cluster.map_shared_rank(&s, 0)->part;
-    for (int r = 1; r < blocks; ++r) stat_merge<X>(st, cluster.map_shared_rank(&s, r)->part, c, 0.f);
+    Stat parts[kMaxSplit];
+    int l[kMaxSplit], h[kMaxSplit];
+#pragma unroll
+    for (int r = 0; r < kMaxSplit; ++r) {
+      const Select* o = cluster.map_shared_rank(&s, r < blocks ? r : 0);
+      parts[r] = o->part;
+      l[r] = 0;
+      h[r] = r < blocks ? o->n_keys : 0;
+    }
+    st = parts[0];
+#pragma unroll
+    for (int r = 1; r < kMaxSplit; ++r)
+      if (r < blocks) stat_merge<X>(st, parts[r], c, 0.f);
     at = k;
     if (tid < mine) {
       const unsigned long long key = s.keys[tid];
-      int l[kMaxSplit], h[kMaxSplit];
+      for (int span = 1; span <= k; span *= 2) {                       // loads of all lists first, without branches
+        unsigned long long v[kMaxSplit];
 #pragma unroll
-      for (int r = 0; r < kMaxSplit; ++r) {
-        l[r] = 0;
-        h[r] = r < blocks ? cluster.map_shared_rank(&s, r)->n_keys : 0;
-      }
-      for (int span = kMaxTop; span > 0; span >>= 1) {
+        for (int r = 0; r < kMaxSplit; ++r)
+          v[r] = cluster.map_shared_rank(&s, r < blocks ? r : 0)->keys[(l[r] + h[r]) / 2];
 #pragma unroll
         for (int r = 0; r < kMaxSplit; ++r) {
-          if (l[r] >= h[r]) continue;
           const int mid = (l[r] + h[r]) / 2;
-          if (cluster.map_shared_rank(&s, r)->keys[mid] > key) l[r] = mid + 1; else h[r] = mid;
+          const bool more = l[r] < h[r], above = v[r] > key;
+          l[r] = more && above ? mid + 1 : l[r];
+          h[r] = more && !above ? mid : h[r];
         }
       }
       at = 0;
@@ -967,8 +978,14 @@ __global__ void __launch_bounds__(kThreads) distill_fwd_kernel(DistillArgs a, fl
   if (blocks > 1) {
     if (tid == 0) sh_part = st;
     cluster.sync();
-    if (rank == 0)
-      for (int r = 1; r < blocks; ++r) stat_merge<X>(st, *cluster.map_shared_rank(&sh_part, r), c1, c2);
+    if (rank == 0) {
+      Stat parts[kMaxSplit];
+#pragma unroll
+      for (int r = 1; r < kMaxSplit; ++r) parts[r] = *cluster.map_shared_rank(&sh_part, r < blocks ? r : 0);
+#pragma unroll
+      for (int r = 1; r < kMaxSplit; ++r)
+        if (r < blocks) stat_merge<X>(st, parts[r], c1, c2);
+    }
     cluster.sync();
     if (rank != 0) return;
   }
@@ -1173,11 +1190,14 @@ __global__ void __launch_bounds__(kThreads) top_bwd_kernel(BwdArgs a) {
   }
 }
 
-// Blocks per row of a forward pass: one while the rows fill the GPU, else up to kMaxSplit. One row of 262144 fp32 takes
-// 17 us on eight blocks, eight rows of 151936 bf16 17 us.
-int split_of(int T, int V) {
+// Blocks per row of a forward pass: up to kMaxSplit while all of them are at most three per SM and each has `least`
+// bytes of the row. Measured on rows of 151936 bf16 with k = 20 (us with 1, 2, 4, 8 blocks): one row 16.5, 13.5, 10.6,
+// 10.4; 32 rows 17.2, 13.6, 11.2, 12.4; 64 rows 17.3, 13.8, 13.0, 15.9; 148 rows 17.7, 16.5, 19.1, 20.9; 200 rows 21.7,
+// 19.8, 19.9, 20.9; rows of 32000: 64 rows 8.7, 9.4, 9.1, 10.5. Without a selection less is enough (one row 12.3, 9.3,
+// 6.8, 5.9).
+int split_of(int T, long long bytes, int least) {
   int n = 1;
-  while (n < kMaxSplit && 2ll * n * T <= 4ll * txh::sm_count() && V / (2 * n) >= kMinPart) n *= 2;
+  while (n < kMaxSplit && 2ll * n * T <= 3ll * txh::sm_count() && bytes / (2 * n) >= least) n *= 2;
   return n;
 }
 
@@ -1248,7 +1268,7 @@ extern "C" int tx_top_logprob_fwd(const void* logits, int logits_fp32, long long
   if (T <= 0) return 0;
   if (V < 1 || k < 1 || k > kMaxTop || k > V || V > 0x7fff0000) return 1;
   const TopArgs a{logits, ld, T, V, k, inv_temp, targets, ids, top, target, entropy, reinterpret_cast<float2*>(stats)};
-  const int n = split_of(T, V);
+  const int n = split_of(T, V * (logits_fp32 ? 4ll : 2ll), 65536);
   const int bytes = sizeof(Select);
   if (logits_fp32)
     return entropy ? launch_rows<top_fwd_kernel<float, kEntropy>>(T, n, bytes, s, a)
@@ -1265,7 +1285,7 @@ extern "C" int tx_top_distill_fwd(const void* logits, int logits_fp32, long long
   if (V < 1 || k < 1 || k > kMaxList || V > 0x7fff0000) return 1;
   const DistillArgs a{logits, ld, T, V, k, inv_temp, full, ids, values, labels, kl, nll, stats};
   const float c = inv_temp * kLog2e, c1 = nll ? kLog2e : c;
-  const int n = split_of(T, V);
+  const int n = split_of(T, V * (logits_fp32 ? 4ll : 2ll), 32768);
   if (!nll && !full) {
     const int grid = (T + kWarps - 1) / kWarps;
     if (logits_fp32) distill_list_kernel<float><<<grid, kThreads, 0, s>>>(a);
