@@ -30,7 +30,9 @@ constexpr int kMaxDigits = 1024;              // 10 bits a pass
 constexpr int kSortCluster = 8;
 constexpr int kClearThreads = 512;
 constexpr int kSortTile = 16;                 // pairs a lane has in flight
-constexpr int kCountTokens = 4096;            // up to here every pair counts the pairs before it: T^2 / 2 comparisons
+// Up to here every pair counts the pairs before it, from there on the radix sort (whole gradient of 64 columns, us:
+// 512 tokens 6.9 and 12.8; 4096 tokens 12.4 and 13.8; 8192 tokens 28.8 and 16.6).
+constexpr int kCountTokens = 4096;
 constexpr int kCountThreads = 256;
 constexpr int kCountPer = 8;                  // threads per pair
 
