@@ -376,6 +376,18 @@ __device__ __forceinline__ Row finish_row(const Stat& a, const LT* x, int V, Sta
   return r;
 }
 
+// Asks for what the warp reads in the iteration that begins at element `at`, 128 bytes per lane, so that its loads find
+// it in L2: a block's threads wait for each other only at a row's ends, but each has only one iteration's loads in
+// flight. One iteration ahead 8192 x 128256 bf16 with k = 64 takes 360 us, two 366 us, four 374 us, none 388 us; bulk
+// prefetches of 512 bytes 375 us. Backward 4096 x 151936 bf16 with both temperatures 385 us, 393 us without.
+template <typename LT>
+__device__ __forceinline__ void ask_ahead(const LT* x, int at, int hi) {
+  constexpr int line = 128 / sizeof(LT);                     // a warp's vectors side by side are four lines
+  const int lane = threadIdx.x & 31;
+  const int j = at + (threadIdx.x >> 5) * 4 * line + lane / 4 * kChunk<LT> + lane % 4 * line;
+  if (lane < 4 * kUnroll && j < hi) asm volatile("prefetch.global.L2 [%0];" ::"l"(x + j));
+}
+
 // The block's vectors of columns [lo, hi) from element `from` on, kUnroll per thread at a time: fn(first element of the
 // thread, vectors, how many of them begin inside; the last may reach out and is then filled with -inf).
 template <typename LT, typename Fn>
@@ -385,6 +397,7 @@ __device__ __forceinline__ void each_vec(const LT* x, int from, int lo, int hi, 
   uint4 u[kUnroll];
   for (; at >= lo && at + step <= hi; at += step) {
     const int j = at + threadIdx.x * kVec<LT>;
+    ask_ahead(x, at + step, hi);
 #pragma unroll
     for (int i = 0; i < kUnroll; ++i) u[i] = *reinterpret_cast<const uint4*>(x + j + i * kChunk<LT>);
     fn(j, u, kUnroll);
@@ -671,6 +684,7 @@ __device__ __forceinline__ Stat top_of_part(Select& s, const LT* x, int base, in
   // ---- first iteration: the first threshold
   Acc<X> acc;
   uint4 u[kUnroll];
+  ask_ahead(x, base + kUnroll * chunk, hi);
   const int count = min(kUnroll, (hi - base + chunk - 1) / chunk);
 #pragma unroll
   for (int i = 0; i < kUnroll; ++i)
@@ -788,8 +802,9 @@ __device__ __forceinline__ Stat top_of_part(Select& s, const LT* x, int base, in
 // warp, of which the special function unit's 8 cycles for each of 8 exponentials are the longest part; the selection
 // adds a quarter of that at k = 64. Five blocks of 256 threads per SM hide one row's serial parts (first threshold, last
 // sort) behind the others' streaming; a ring of asynchronous copies with two blocks per SM instead measured 649 us where
-// this took 415 us. 8192 x 128256 bf16, k = 64: 388 us (5.4 TB/s), k = 1: 344 us; 2047 x 151936 fp32 with entropy, k = 8:
-// 212 us (5.9 TB/s). Under the power cap of a long run the clock falls and these times grow by up to a tenth.
+// this took 415 us, blocks for half a row 557 us, six blocks with 40 registers 390 us where five took 361 us. 8192 x
+// 128256 bf16, k = 64: 361 us (5.8 TB/s), k = 1: 321 us (6.5 TB/s), k = 256: 478 us; 2047 x 151936 fp32 with entropy, k
+// = 8: 202 us (6.2 TB/s). Under the power cap of a long run the clock falls and these times grow by up to a tenth.
 template <typename LT, int X>
 __global__ void __launch_bounds__(kThreads, X == kNone ? 5 : 4) top_fwd_kernel(TopArgs a) {
   extern __shared__ __align__(16) unsigned char shared[];
@@ -952,7 +967,7 @@ __global__ void __launch_bounds__(kThreads) distill_list_kernel(DistillArgs a) {
 }
 
 // X: kNone (one softmax sum of the row, scale c1 in the exponent) or kSecond (c1 and c2). One sum is bound by memory
-// (4096 x 128256 bf16: 165 us, 6.4 TB/s), two by the exponentials (4096 x 151936 bf16: 266 us, 4.7 TB/s).
+// (4096 x 128256 bf16: 162 us, 6.5 TB/s), two by the exponentials (4096 x 151936 bf16: 266 us, 4.7 TB/s).
 template <typename LT, int X>
 __global__ void __launch_bounds__(kThreads) distill_fwd_kernel(DistillArgs a, float c1, float c2) {
   __shared__ Stat sh_stat[kWarps];
@@ -1019,8 +1034,8 @@ struct BwdArgs {
 // d_j = A p_j (temperature) + B p_j (temperature 1) - G p_j (log p_j + H), then the listed columns get their own
 // terms on top: they are computed from the same fp32 value and rounded once, by the thread of the first occurrence.
 //
-// Bound by memory: 4096 x 151936 bf16 with both temperatures 393 us (6.3 TB/s), 1000 x 262144 bf16 with entropy 173 us
-// (6.1 TB/s), soft part alone on 2048 x 151936 fp32 186 us (6.7 TB/s written).
+// Bound by memory: 4096 x 151936 bf16 with both temperatures 385 us (6.5 TB/s), 1000 x 262144 bf16 with entropy 163 us
+// (6.4 TB/s), soft part alone on 2048 x 151936 fp32 186 us (6.7 TB/s written).
 //
 // A block has a part of kBwdPart columns: the blocks at work at a time then cover few rows from end to end, which the
 // memory takes 4 to 8 % faster than a block per row (4096 x 128256 bf16: 325 us, against 354 us for whole rows and
@@ -1045,6 +1060,7 @@ __global__ void __launch_bounds__(kThreads) top_bwd_kernel(BwdArgs a) {
     for (int i = 0; i < kUnroll; ++i)
       if (j + i * chunk < hi) u[i] = load_vec(x, j + i * chunk, lo, hi, aligned);
   };
+  if (DENSE && aligned) ask_ahead(x, from + kUnroll * chunk, hi);
   if (DENSE) load(from + tid * N);                 // on their way while the list is looked at
   const float* st = a.stats + static_cast<long long>(row) * (mode == kScore ? 2 : kDistillStats);
   const float m = st[0], ls1 = st[1], lst = mode == kScore ? st[1] : st[2];
@@ -1139,6 +1155,7 @@ __global__ void __launch_bounds__(kThreads) top_bwd_kernel(BwdArgs a) {
   if (DENSE) {
     for (int at = from; at < hi; at += kUnroll * chunk) {
       const int j = at + tid * N;
+      if (at != from && aligned) ask_ahead(x, at + kUnroll * chunk, hi);
       if (at != from) load(j);
 #pragma unroll
       for (int i = 0; i < kUnroll; ++i) {
