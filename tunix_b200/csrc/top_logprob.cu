@@ -133,6 +133,13 @@ __device__ __forceinline__ uint4 pack(const float (&z)[8]) {
   for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(z[2 * i], z[2 * i + 1]);
   return u;
 }
+// Element e of a vector.
+template <typename T>
+__device__ __forceinline__ float element(uint4 u, int e) {
+  const int word = sizeof(T) == 2 ? e / 2 : e;
+  const uint32_t v = word < 2 ? (word == 0 ? u.x : u.y) : (word == 2 ? u.z : u.w);
+  return __uint_as_float(sizeof(T) == 4 ? v : (e & 1 ? v & 0xffff0000u : v << 16));
+}
 // Maxima of vectors, kept packed for bf16: `scalar` is the one number.
 template <typename T>
 struct Top;
@@ -289,24 +296,26 @@ __device__ __forceinline__ float warp_sum_of(float v) {
   return v;
 }
 
-// Leaves the block's statistics in every thread: the maximum first, then sums relative to it. `sh` holds kWarps entries.
+// The block's statistics in every thread, the maximum first, then sums relative to it. Between the steps, and before `sh`
+// (kWarps entries) is used again, the block synchronises.
+__device__ __forceinline__ void stat_max(const Stat& a, Stat* sh) {
+  const float m = warp_max_of(a.m);
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5].m = m;
+}
 template <int X>
-__device__ __forceinline__ Stat stat_block(Stat a, Stat* sh, float c, float c2) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const float wm = warp_max_of(a.m);
-  __syncthreads();
-  if (lane == 0) sh[warp].m = wm;
-  __syncthreads();
+__device__ __forceinline__ void stat_sums(Stat& a, Stat* sh, float c, float c2) {
   float m = sh[0].m;
   for (int w = 1; w < kWarps; ++w) m = fmaxf(m, sh[w].m);
   if (a.m != m) stat_raise<X>(a, m, c, c2);
   a.s = warp_sum_of(a.s);
   if (X != kNone) a.t = warp_sum_of(a.t);
-  if (lane == 0) {
-    sh[warp].s = a.s;
-    sh[warp].t = a.t;
+  if ((threadIdx.x & 31) == 0) {
+    sh[threadIdx.x >> 5].s = a.s;
+    sh[threadIdx.x >> 5].t = a.t;
   }
-  __syncthreads();
+}
+template <int X>
+__device__ __forceinline__ Stat stat_all(Stat a, const Stat* sh) {
   a.s = a.t = 0.f;
   for (int w = 0; w < kWarps; ++w) {
     a.s += sh[w].s;
@@ -459,7 +468,7 @@ __device__ __forceinline__ void sort_keys(unsigned long long* keys, int n) {
     const int per = n <= kThreads / 4 ? 4 : 2, i = threadIdx.x / per, sub = threadIdx.x % per;
     const unsigned long long key = i < n ? keys[i] : 0;
     int above = 0;
-    for (int j = sub; j < n; j += per) above += keys[j] > key;
+    for (int j = sub; i < n && j < n; j += per) above += keys[j] > key;
     above += __shfl_xor_sync(0xffffffffu, above, 1);
     if (per == 4) above += __shfl_xor_sync(0xffffffffu, above, 2);
     __syncthreads();
@@ -525,17 +534,49 @@ struct TopArgs {
   float2* stats;               // [T]: m, ln s
 };
 
+// The row's target and its logit.
+struct Given {
+  long long at;
+  float value;
+};
+
+// Numbers in the order of floats; a NaN counts as +inf.
+__device__ __forceinline__ uint32_t order_of(float x) {
+  const uint32_t b = __float_as_uint(x != x ? INFINITY : x);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float of_order(uint32_t o) {
+  return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+
+// The n-th largest number of a warp (1 <= n <= 32), neither 0 nor ~0 among them, from the nearer end: the extreme one is
+// taken away until it is that one's turn (8192 x 32000 bf16 with k = 20: 129 us, 135 us with a sort of the warp; with k =
+// 64, eight rounds, both are the same).
+__device__ __forceinline__ uint32_t nth_largest(uint32_t v, int n) {
+  const bool down = n <= 16;
+  int left = down ? n : 33 - n;
+  if (!down) v = ~v;
+  uint32_t top;
+  while (true) {
+    top = __reduce_max_sync(0xffffffffu, v);
+    left -= __popc(__ballot_sync(0xffffffffu, v == top));
+    if (left <= 0) break;
+    if (v == top) v = 0;
+  }
+  return down ? top : ~top;
+}
+
 // Selection state of a block.
 //
 // A candidate is what a thread takes in one iteration (kUnroll vectors), when its largest element is not below a
 // threshold that k elements of the block's part are known to reach. The first threshold comes from the first iteration:
 // the smallest over the warps of the ceil(k / warps)-th largest of a warp's per-thread maxima (of the warps that have a
 // whole vector per thread). From then on the maxima of candidates are counted in bins of equal width above it, and in
-// every iteration one warp moves the threshold up to a bin below the lowest bin that k of them reach. Bin numbers
+// every other iteration one warp moves the threshold up to a bin below the lowest bin that k of them reach. Bin numbers
 // (rounded to the nearest) and that edge are computed with monotone roundings, so an element of such a bin is never
 // below the edge. At the end the candidates that still reach the threshold are read again (from L2), a vector per
-// thread, and their elements that do are sorted: little more than k. Every step is dense over the block's threads: the
-// kernel is bound by the instructions it issues, not by the memory.
+// thread, and their elements that do are sorted: little more than k. Every step is dense over the block's threads: for
+// all but the smallest k the kernel is bound by the instructions it issues, not by the memory.
 struct Select {
   unsigned long long keys[kKeys];
   union {
@@ -621,7 +662,7 @@ __device__ __noinline__ void select_in_order(Select& s, const LT* x, int lo, int
 
 // Sorts the first k of n keys from high to low with the bins they were counted in: a key goes behind the keys of higher
 // bins, its place among those of its own (a few, as long as few elements are equal) is counted. All threads call it.
-// 8192 rows of 8000 with k = 200: 191 us, 277 us with a bitonic sort.
+// 8192 rows of 8000 with k = 200 (before the steps around it became shorter): 191 us, 277 us with a bitonic sort.
 __device__ __forceinline__ void sort_binned(Select& s, int n, int k, float thr0, float inv_width) {
   const int tid = threadIdx.x;
   if (n <= kThreads / 4) {                                   // counting all of them is less
@@ -676,7 +717,8 @@ __device__ __forceinline__ void sort_binned(Select& s, int n, int k, float thr0,
 // The k best of columns [lo, hi) into s.keys, sorted, and the statistics of the part. `base`: the first column of the
 // first vector.
 template <typename LT, int X>
-__device__ __forceinline__ Stat top_of_part(Select& s, const LT* x, int base, int lo, int hi, int k, float c) {
+__device__ __forceinline__ Stat top_of_part(Select& s, const LT* x, int base, int lo, int hi, int k, float c,
+                                            const long long* targets, int V, Given& given) {
   constexpr int N = kVec<LT>, chunk = kChunk<LT>;
   const int tid = threadIdx.x, lane = tid & 31;
   for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0;
@@ -690,18 +732,11 @@ __device__ __forceinline__ Stat top_of_part(Select& s, const LT* x, int base, in
   for (int i = 0; i < kUnroll; ++i)
     if (i < count) u[i] = load_vec(x, base + tid * N + i * chunk, lo, hi, true);
   const float most = max_vecs<LT>(u, count);
-  float v = most;
-  v = v != v ? INFINITY : v;
-  for (int size = 2; size <= 32; size <<= 1)
-    for (int stride = size >> 1; stride > 0; stride >>= 1) {
-      const float o = __shfl_xor_sync(0xffffffffu, v, stride);
-      const bool larger = ((lane & stride) == 0) == ((lane & size) == 0);
-      v = larger ? fmaxf(v, o) : fminf(v, o);
-    }
   const int whole = min(kWarps, max(0, hi - base) / (32 * N));
   const int nth_of = whole ? (k + whole - 1) / whole : 33;             // more than a warp's threads: no threshold
-  const float nth = __shfl_sync(0xffffffffu, v, min(nth_of, 32) - 1);
-  const float warp_max = __shfl_sync(0xffffffffu, v, 0);
+  const uint32_t order = order_of(most);
+  const float warp_max = of_order(__reduce_max_sync(0xffffffffu, order));
+  const float nth = of_order(nth_largest(order, min(nth_of, 32)));
   if (lane == 0) {
     s.warp_nth[tid >> 5] = nth;
     s.warp_max[tid >> 5] = warp_max;
@@ -732,7 +767,7 @@ __device__ __forceinline__ Stat top_of_part(Select& s, const LT* x, int base, in
       if (pos < kCand) s.cand[pos] = up | static_cast<uint32_t>(it * kThreads + tid);
       atomicAdd(&s.bins[bin_of(most, thr0, inv_width)], 1);
     }
-    if ((it & (kWarps - 1)) == tid >> 5) {
+    if ((it & 1) && ((it >> 1) & (kWarps - 1)) == tid >> 5) {
       const int b = cut_bin(s.bins, k);
       const float t = fmaf(b - 1.f, width, thr0);
       if (lane == 0 && b > 1 && t > *shared_thr) *shared_thr = t;
@@ -747,7 +782,11 @@ __device__ __forceinline__ Stat top_of_part(Select& s, const LT* x, int base, in
     add_vecs<LT, X>(acc, w, n, t, c, 0.f);
     offer(t);
   });
+  Stat st = acc.stat();
+  stat_max(st, s.stat);
   __syncthreads();
+  if (tid == 0 && targets) given.at = *targets;              // the loads come back while the candidates are sorted
+  stat_sums<X>(st, s.stat, c, 0.f);
   // ---- the candidates' elements, sorted
   const int n = s.count;
   bool fits = n <= kCand && hi - base <= 65536 / kThreads * kUnroll * chunk;
@@ -769,6 +808,7 @@ __device__ __forceinline__ Stat top_of_part(Select& s, const LT* x, int base, in
     __syncthreads();
     fits = s.n_kept <= kKept;
   }
+  if (given.at >= 0 && given.at < V) given.value = to_f(x[given.at]);
   if (fits) {
     for (int i = tid; i < s.n_kept * kUnroll; i += kThreads) {
       const int at = s.kept[i / kUnroll];
@@ -777,13 +817,16 @@ __device__ __forceinline__ Stat top_of_part(Select& s, const LT* x, int base, in
       if (Top<LT>::of(w).scalar() < thr) continue;
       float z[N];
       unpack(w, z);
+      unsigned above = 0;                                    // its elements that reach the threshold, usually one
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        if (!(z[e] < thr) && j + e >= lo && j + e < hi) {
-          const int pos = atomicAdd(&s.n_keys, 1);
-          if (pos < kKeys) s.keys[pos] = key_of(z[e], j + e);
-          atomicAdd(&s.bins[bin_of(z[e], thr0, inv_width)], 1);
-        }
+      for (int e = 0; e < N; ++e) above |= !(z[e] < thr) && j + e >= lo && j + e < hi ? 1u << e : 0u;
+      int pos = atomicAdd(&s.n_keys, __popc(above));
+      for (; above; above &= above - 1) {
+        const int e = __ffs(above) - 1;
+        const float v = element<LT>(w, e);
+        if (pos < kKeys) s.keys[pos] = key_of(v, j + e);
+        ++pos;
+        atomicAdd(&s.bins[bin_of(v, thr0, inv_width)], 1);
       }
     }
     __syncthreads();
@@ -793,18 +836,19 @@ __device__ __forceinline__ Stat top_of_part(Select& s, const LT* x, int base, in
     sort_binned(s, s.n_keys, k, thr0, inv_width);
   else
     select_in_order(s, x, lo, hi, k);
-  return stat_block<X>(acc.stat(), s.stat, c, 0.f);
+  return stat_all<X>(st, s.stat);
 }
 
 // A row per cluster of 1 .. kMaxSplit blocks, each with a part of the columns.
 //
-// Bound by instructions: unpacking, the multiply-add, the exponential and the sum are about 45 per 16-byte vector and
-// warp, of which the special function unit's 8 cycles for each of 8 exponentials are the longest part; the selection
-// adds a quarter of that at k = 64. Five blocks of 256 threads per SM hide one row's serial parts (first threshold, last
-// sort) behind the others' streaming; a ring of asynchronous copies with two blocks per SM instead measured 649 us where
-// this took 415 us, blocks for half a row 557 us, six blocks with 40 registers 390 us where five took 361 us. 8192 x
-// 128256 bf16, k = 64: 361 us (5.8 TB/s), k = 1: 321 us (6.5 TB/s), k = 256: 478 us; 2047 x 151936 fp32 with entropy, k
-// = 8: 202 us (6.2 TB/s). Under the power cap of a long run the clock falls and these times grow by up to a tenth.
+// Long rows with small k are bound by memory (8192 x 128256 bf16, k = 1: 312 us, 6.7 TB/s), with larger k by the
+// instructions of the selection, a fifth on top of those of the sums at k = 64 (349 us, 6.0 TB/s; k = 256: 430 us). Five
+// blocks of 256 threads per SM hide one row's serial parts (first threshold, last sort) behind the others' streaming.
+// Short rows are mostly those parts: 8192 x 32000, k = 20: 130 us, 4.0 TB/s (blocks of 128 threads take 113 us there, but
+// 357 us where this takes 349 us). Tried at 8192 x 128256, k = 64: a ring of asynchronous copies with two blocks per SM
+// 649 us where this took 415 us, two blocks per row 557 us and six blocks with 40 registers 390 us where it took 361 us.
+// 2047 x 151936 fp32 with entropy, k = 8: 198 us (6.3 TB/s). Under the power cap of a long run the clock falls and these
+// times grow by up to a tenth.
 template <typename LT, int X>
 __global__ void __launch_bounds__(kThreads, X == kNone ? 5 : 4) top_fwd_kernel(TopArgs a) {
   extern __shared__ __align__(16) unsigned char shared[];
@@ -816,7 +860,8 @@ __global__ void __launch_bounds__(kThreads, X == kNone ? 5 : 4) top_fwd_kernel(T
   const float c = a.inv_temp * kLog2e;
   const int2 part = part_of(a.V, rank, blocks);
   const int lo = part.x, hi = part.y, base = lo - misalign(x + lo);
-  Stat st = top_of_part<LT, X>(s, x, base, lo, hi, k, c);
+  Given given{-1, 0.f};
+  Stat st = top_of_part<LT, X>(s, x, base, lo, hi, k, c, a.target && rank == 0 ? a.targets + row : nullptr, a.V, given);
   int at = tid;                          // place of this thread's key among the k best of the row
   if (blocks > 1) {
     const int mine = min(k, hi - lo);
@@ -869,10 +914,7 @@ __global__ void __launch_bounds__(kThreads, X == kNone ? 5 : 4) top_fwd_kernel(T
     a.top[static_cast<long long>(row) * k + at] = (key_value(key) - r.m) * a.inv_temp - r.ls;
   }
   if (tid == 0 && rank == 0) {
-    if (a.target) {
-      const long long t = a.targets[row];
-      a.target[row] = (t >= 0 && t < a.V) ? (to_f(x[t]) - r.m) * a.inv_temp - r.ls : 0.f;
-    }
+    if (a.target) a.target[row] = given.at >= 0 && given.at < a.V ? (given.value - r.m) * a.inv_temp - r.ls : 0.f;
     if (a.entropy) a.entropy[row] = r.x;
     a.stats[row] = make_float2(r.m, r.ls);
   }
@@ -989,7 +1031,12 @@ __global__ void __launch_bounds__(kThreads) distill_fwd_kernel(DistillArgs a, fl
     }
     add_vecs<LT, X>(acc, u, count, most, c1, c2);
   });
-  Stat st = stat_block<X>(acc.stat(), sh_stat, c1, c2);
+  Stat st = acc.stat();
+  stat_max(st, sh_stat);
+  __syncthreads();
+  stat_sums<X>(st, sh_stat, c1, c2);
+  __syncthreads();
+  st = stat_all<X>(st, sh_stat);
   if (blocks > 1) {
     if (tid == 0) sh_part = st;
     cluster.sync();
