@@ -36,6 +36,7 @@ constexpr int kMaxSplit = 8;                  // blocks (one cluster) a row is s
 constexpr int kMinPart = 4096;                // columns of a part of the backward pass at least
 constexpr int kBwdPart = 32768;               // columns a block of the backward pass takes at most
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr double kLog2eFine = 1.4426950408889634;
 constexpr float kFloor = -1e37f;              // lowest running maximum
 
 __device__ __forceinline__ float ex2(float x) {
@@ -328,9 +329,21 @@ __device__ __forceinline__ Stat stat_all(Stat a, const Stat* sh) {
 struct Row {
   float m, ls;      // maximum, ln sum exp((x - m) at the scale)
   float x;          // kEntropy: the entropy; kSecond: ln of the sum at the scale c2
+  bool careful;     // from differences to the true maximum: there is no sum 2^(x c - M)
 };
 
 __device__ __forceinline__ float log_sum(float s) { return s == 0.f ? INFINITY : logf(s); }
+
+// ln s of a positive, finite and normal s: the logarithm's argument is brought near 1, where its rounding is small.
+__device__ __forceinline__ double log_fine(float s) {
+  const int b = __float_as_int(s), e = (b - 0x3f400000) >> 23;       // s / 2^e is in [0.75, 1.5)
+  return fma(static_cast<double>(e), 0.69314718055994531, static_cast<double>(logf(__int_as_float(b - (e << 23)))));
+}
+// ln sum exp((x - m) at the scale), from s = sum 2^(x c - M) with M rounded.
+__device__ __forceinline__ double log_fine(float s, float m, float c) {
+  return fma(-0.69314718055994531, fma(static_cast<double>(m), static_cast<double>(c), -static_cast<double>(scaled_max(m, c))),
+             log_fine(s));
+}
 
 // Row statistics from differences to the true maximum, by the whole block over the whole row.
 template <typename LT, int X>
@@ -363,7 +376,7 @@ __device__ __noinline__ Row careful_row(const LT* x, int V, Stat* sh, float c, f
     s += sh[w].s;
     t += sh[w].t;
   }
-  Row r{m, log_sum(s), 0.f};
+  Row r{m, log_sum(s), 0.f, true};
   if (X == kEntropy) r.x = s == 0.f ? 0.f : r.ls - kLn2 * (t / s);
   if (X == kSecond) r.x = log_sum(t);
   return r;
@@ -376,6 +389,7 @@ __device__ __forceinline__ Row finish_row(const Stat& a, const LT* x, int V, Sta
   if (!(a.s > 0.5f && a.s < INFINITY && (X != kSecond || (a.t > 0.5f && a.t < INFINITY))))
     return careful_row<LT, X>(x, V, sh, c, c2);
   Row r;
+  r.careful = false;
   r.m = a.m;
   const float ln = logf(a.s);
   r.ls = fmaf(-kLn2, fmaf(a.m, c, -scaled_max(a.m, c)), ln);          // M - m c, exactly
@@ -925,7 +939,7 @@ struct DistillArgs {
   const void* logits;
   long long ld;
   int T, V, k;
-  float inv_temp;
+  double inv_temp;
   int full;                    // 0: both sides normalised over the list, 1: over the vocabulary
   const long long* ids;        // [T, k]; an id outside the vocabulary is an absent entry
   const float* values;         // [T, k]
@@ -940,8 +954,10 @@ struct DistillArgs {
 constexpr int kDistillStats = 8;
 
 // The list of one row, by one warp; writes the row's outputs. ls1, ls2: ln s at temperature 1 and at the temperature.
+// A divergence is a sum of differences of log-probabilities that can be much smaller than these: they are formed in 64
+// bits, a few operations per entry, where roundings in 32 bits were 2e-6 of the result and more.
 template <typename LT>
-__device__ __forceinline__ void distill_list(const DistillArgs& a, int row, const LT* x, float m, float ls1, float ls2) {
+__device__ __forceinline__ void distill_list(const DistillArgs& a, int row, const LT* x, float m, float ls1, double ls2) {
   const int lane = threadIdx.x & 31, V = a.V, k = a.k;
   const long long* ids = a.ids + static_cast<long long>(row) * k;
   const float* values = a.values + static_cast<long long>(row) * k;
@@ -953,13 +969,13 @@ __device__ __forceinline__ void distill_list(const DistillArgs& a, int row, cons
       const float t = values[i], q = expf(t);
       mass += q;
       if (q == 0.f) continue;
-      kl += q * (t - ((to_f(x[id]) - m) * a.inv_temp - ls2));
+      kl += q * static_cast<float>(t - ((static_cast<double>(to_f(x[id])) - m) * a.inv_temp - ls2));
     }
     mass = warp_sum_of(mass);
     kl = warp_sum_of(kl);
     if (ls2 == INFINITY) kl = 0.f;
   } else {
-    const float c = a.inv_temp * kLog2e;
+    const float c = static_cast<float>(a.inv_temp * kLog2eFine);
     float st = 0.f, sx = 0.f;
     for (int i = lane; i < k; i += 32) {
       const long long id = ids[i];
@@ -975,15 +991,19 @@ __device__ __forceinline__ void distill_list(const DistillArgs& a, int row, cons
       st += ex2((values[i] - mt) * c);
       sx += ex2((to_f(x[id]) - mx) * c);
     }
-    lt = log_sum(warp_sum_of(st));
-    lx = log_sum(warp_sum_of(sx));
+    st = warp_sum_of(st);
+    sx = warp_sum_of(sx);
+    lt = log_sum(st);
+    lx = log_sum(sx);
+    const bool usable = st > 0.5f && st < INFINITY && sx > 0.5f && sx < INFINITY;      // a maximum alone counts 1
+    const double both = usable ? log_fine(sx) - log_fine(st) : static_cast<double>(lx) - lt;
     for (int i = lane; i < k; i += 32) {
       const long long id = ids[i];
       if (id < 0 || id >= V) continue;
-      const float lq = (values[i] - mt) * a.inv_temp - lt;
-      const float q = expf(lq);
+      const double t = static_cast<double>(values[i]) - mt, s = static_cast<double>(to_f(x[id])) - mx;
+      const float q = expf(static_cast<float>(t * a.inv_temp) - lt);
       if (q == 0.f) continue;
-      kl += q * (lq - ((to_f(x[id]) - mx) * a.inv_temp - lx));
+      kl += q * static_cast<float>((t - s) * a.inv_temp + both);
     }
     kl = warp_sum_of(kl);
     if (lt == INFINITY || lx == INFINITY) kl = 0.f;
@@ -995,7 +1015,7 @@ __device__ __forceinline__ void distill_list(const DistillArgs& a, int row, cons
       a.nll[row] = (t >= 0 && t < V && ls1 != INFINITY) ? ls1 - (to_f(x[t]) - m) : 0.f;
     }
     float4* out = reinterpret_cast<float4*>(a.stats + static_cast<long long>(row) * kDistillStats);
-    out[0] = make_float4(m, ls1, ls2, mass);
+    out[0] = make_float4(m, ls1, static_cast<float>(ls2), mass);
     out[1] = make_float4(mt, lt, mx, lx);
   }
 }
@@ -1053,7 +1073,11 @@ __global__ void __launch_bounds__(kThreads) distill_fwd_kernel(DistillArgs a, fl
   }
   const Row r = finish_row<LT, X>(st, x, a.V, sh_stat, c1, c2);
   // With one sum both logarithms are the same number and only the one that is asked for gets used.
-  if (tid < 32) distill_list(a, row, x, r.m, r.ls, X == kSecond ? r.x : r.ls);
+  if (tid < 32) {
+    const float rough = X == kSecond ? r.x : r.ls;
+    distill_list(a, row, x, r.m, r.ls,
+                 r.careful ? rough : (X == kSecond ? log_fine(st.t, st.m, c2) : log_fine(st.s, st.m, c1)));
+  }
 }
 
 // ---- backward -------------------------------------------------------------------------------------------
@@ -1343,12 +1367,12 @@ extern "C" int tx_top_logprob_fwd(const void* logits, int logits_fp32, long long
 
 // 1 <= k <= 1024; stats [T, 8].
 extern "C" int tx_top_distill_fwd(const void* logits, int logits_fp32, long long ld, int T, int V, int k,
-                                  float inv_temp, int full, const long long* ids, const float* values,
+                                  double inv_temp, int full, const long long* ids, const float* values,
                                   const long long* labels, float* kl, float* nll, float* stats, cudaStream_t s) {
   if (T <= 0) return 0;
   if (V < 1 || k < 1 || k > kMaxList || V > 0x7fff0000) return 1;
   const DistillArgs a{logits, ld, T, V, k, inv_temp, full, ids, values, labels, kl, nll, stats};
-  const float c = inv_temp * kLog2e, c1 = nll ? kLog2e : c;
+  const float c = static_cast<float>(inv_temp * kLog2eFine), c1 = nll ? kLog2e : c;
   const int n = split_of(T, V * (logits_fp32 ? 4ll : 2ll), 32768);
   if (!nll && !full) {
     const int grid = (T + kWarps - 1) / kWarps;
@@ -1356,7 +1380,7 @@ extern "C" int tx_top_distill_fwd(const void* logits, int logits_fp32, long long
     else             distill_list_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(a);
     return cudaGetLastError() == cudaSuccess ? 0 : 400;
   }
-  if (nll && full && inv_temp != 1.f)
+  if (nll && full && inv_temp != 1.0)
     return logits_fp32 ? launch_rows<distill_fwd_kernel<float, kSecond>>(T, n, 0, s, a, c1, c)
                        : launch_rows<distill_fwd_kernel<__nv_bfloat16, kSecond>>(T, n, 0, s, a, c1, c);
   return logits_fp32 ? launch_rows<distill_fwd_kernel<float, kNone>>(T, n, 0, s, a, c1, c)

@@ -35,7 +35,7 @@ def available() -> bool:
 
 
 def _declare(lib):
-  P, I, L, F = c_void_p, c_int, c_ll, c_float
+  P, I, L, F, D = c_void_p, c_int, c_ll, c_float, ctypes.c_double
   sigs = {
       "tx_gemm_bf16": [P, P, P, I, I, I, L, L, L, I, I, I, I, F, P, I, P],
       "tx_rmsnorm_fwd": [P, P, P, P, P, P, I, I, F, F, P],
@@ -83,7 +83,7 @@ def _declare(lib):
       "tx_logprob_bwd": [P, I, L, P, P, P, P, P, P, L, I, I, I, F, F, P],
       "tx_top_logprob_fwd": [P, I, L, I, I, I, F, P, P, P, P, P, P, P],
       "tx_top_logprob_bwd": [P, I, L, I, I, I, F, P, P, P, P, P, P, P, P, P],
-      "tx_top_distill_fwd": [P, I, L, I, I, I, F, I, P, P, P, P, P, P, P],
+      "tx_top_distill_fwd": [P, I, L, I, I, I, D, I, P, P, P, P, P, P, P],
       "tx_top_distill_bwd": [P, I, L, I, I, I, F, I, P, P, P, P, P, P, P, P],
   }
   for name, argtypes in sigs.items():
