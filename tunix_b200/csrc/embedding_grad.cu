@@ -10,8 +10,12 @@
 // token cannot keep a block busy alone. (3) The partial sums of such a run are added in order. dout is read once and
 // every present row of the table is touched once. Ids outside the vocabulary sort behind all others and are left out.
 //
-// 16384 tokens x 4096 into an fp32 buffer: 97 us (134 MB of dout and 115 MB of rows read and written: 3.8 TB/s).
-// 65536 x 1152, half of them one id, new table of 262144 rows: 151 us, of which 82 us write the table (604 MB).
+// Blocks of (2) and (3) are launched before their predecessor ends and wait for it on the device (with plain launches 4
+// and 5 us more in the two cases below, 1 us of 7 for 512 tokens). Fetching a part of dout into L2 while the ids are sorted
+// gained nothing.
+//
+// 16384 tokens x 4096 into an fp32 buffer: 96 us (134 MB of dout and 115 MB of rows read and written: 3.8 TB/s).
+// 65536 x 1152, half of them one id, new table of 262144 rows: 145 us, of which 82 us write the table (604 MB).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -267,6 +271,7 @@ template <typename GT>
 __global__ void __launch_bounds__(256, 4) sum_runs_kernel(GradArgs g) {
   __shared__ int2 window[3 * kMaxChunk + 2];                       // the chunk before with one more, this one, the next with one more
   const int size = g.chunk, lo = blockIdx.x * size, n = min(size, g.T - lo);
+  tx::griddep_wait();
   for (int i = threadIdx.x; i < 3 * size + 2; i += blockDim.x) {
     const int at = lo - size - 1 + i;
     window[i] = (at >= 0 && at < g.T) ? g.pairs[at] : make_int2(-1, 0);
@@ -352,6 +357,7 @@ constexpr int kJoinGroups = 32;      // chunks of a long run are summed in this 
 template <typename GT>
 __global__ void __launch_bounds__(8 * kJoinGroups) join_runs_kernel(GradArgs g) {
   __shared__ float sh[kJoinGroups][8][8];
+  tx::griddep_wait();
   const int tiles = (g.D + 63) / 64, items = *g.n_long * tiles;
   const int tx = threadIdx.x & 7, part = threadIdx.x >> 3;
   for (int item = blockIdx.x; item < items; item += gridDim.x) {
@@ -392,12 +398,22 @@ template <typename GT>
 int launch_grad(const GradArgs& g, cudaStream_t s) {
   const int chunks = (g.T + g.chunk - 1) / g.chunk;
   const int threads = min(256, (g.D / 8 + 31) / 32 * 32);
-  sum_runs_kernel<GT><<<dim3(chunks, (g.D / 8 + threads - 1) / threads), threads, 0, s>>>(g);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(chunks, (g.D / 8 + threads - 1) / threads);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, sum_runs_kernel<GT>, g) != cudaSuccess) return 405;
   if (chunks < 2) return cudaGetLastError() == cudaSuccess ? 0 : 400;        // a long run covers a chunk behind its first
   const long long most = static_cast<long long>(chunks) * ((g.D + 63) / 64);
   const int grid = static_cast<int>(min(most, 4ll * txh::sm_count()));
-  join_runs_kernel<GT><<<grid, 8 * kJoinGroups, 0, s>>>(g);
-  return cudaGetLastError() == cudaSuccess ? 0 : 400;
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(8 * kJoinGroups);
+  return cudaLaunchKernelEx(&cfg, join_runs_kernel<GT>, g) == cudaSuccess ? 0 : 406;
 }
 
 template <int BITS>
