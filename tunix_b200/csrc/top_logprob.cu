@@ -402,7 +402,9 @@ __device__ __forceinline__ Row finish_row(const Stat& a, const LT* x, int V, Sta
 // Asks for what the warp reads in the iteration that begins at element `at`, 128 bytes per lane, so that its loads find
 // it in L2: a block's threads wait for each other only at a row's ends, but each has only one iteration's loads in
 // flight. One iteration ahead 8192 x 128256 bf16 with k = 64 takes 360 us, two 366 us, four 374 us, none 388 us; bulk
-// prefetches of 512 bytes 375 us. Backward 4096 x 151936 bf16 with both temperatures 385 us, 393 us without.
+// prefetches of 512 bytes 375 us. In the backward pass it pays where an element takes two terms (1000 x 262144 bf16 with
+// entropy: 163 us, 172 us without); with one, 4096 x 128256 takes 323 us instead of 326 us for itself, but 340 us instead
+// of 333 us in long runs under the power cap.
 template <typename LT>
 __device__ __forceinline__ void ask_ahead(const LT* x, int at, int hi) {
   constexpr int line = 128 / sizeof(LT);                     // a warp's vectors side by side are four lines
@@ -1131,7 +1133,8 @@ __global__ void __launch_bounds__(kThreads) top_bwd_kernel(BwdArgs a) {
     for (int i = 0; i < kUnroll; ++i)
       if (j + i * chunk < hi) u[i] = load_vec(x, j + i * chunk, lo, hi, aligned);
   };
-  if (DENSE && aligned) ask_ahead(x, from + kUnroll * chunk, hi);
+  const bool ahead = (DENSE == 3 || DENSE == 5) && aligned;
+  if (ahead) ask_ahead(x, from + kUnroll * chunk, hi);
   if (DENSE) load(from + tid * N);                 // on their way while the list is looked at
   const float* st = a.stats + static_cast<long long>(row) * (mode == kScore ? 2 : kDistillStats);
   const float m = st[0], ls1 = st[1], lst = mode == kScore ? st[1] : st[2];
@@ -1226,7 +1229,7 @@ __global__ void __launch_bounds__(kThreads) top_bwd_kernel(BwdArgs a) {
   if (DENSE) {
     for (int at = from; at < hi; at += kUnroll * chunk) {
       const int j = at + tid * N;
-      if (at != from && aligned) ask_ahead(x, at + kUnroll * chunk, hi);
+      if (ahead && at != from) ask_ahead(x, at + kUnroll * chunk, hi);
       if (at != from) load(j);
 #pragma unroll
       for (int i = 0; i < kUnroll; ++i) {
