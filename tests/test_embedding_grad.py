@@ -124,6 +124,19 @@ def test_tables_that_the_kernels_do_not_take(kernel_lib):
     F.embedding(ids.cpu(), wide.contiguous())
 
 
+@pytest.mark.gpu
+def test_other_devices_and_buffers_are_refused(kernel_lib, monkeypatch):
+  from tunix_b200.ops import _lib
+  ids = id_list("padded", 50, 30).cuda()
+  table = torch.randn(30, 32, device="cuda").to(bf16).requires_grad_()
+  table.main_grad = torch.zeros(30, 32, device="cuda", dtype=bf16)
+  with pytest.raises(ValueError, match="main_grad must be fp32"):
+    F.embedding(ids, table).sum().backward()
+  monkeypatch.setattr(_lib, "bind_thread", lambda: 1)
+  with pytest.raises(ValueError, match="this process drives cuda:1"):
+    F.embedding(ids, table)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("main_grad", [False, True])
 def test_gradient_through_the_lookup(device, main_grad):

@@ -277,6 +277,8 @@ class _EmbeddingFn(torch.autograd.Function):
     mg = _main_grad(ctx.holder)
     dout = dout.contiguous()
     if mg is not None:
+      if mg.dtype != torch.float32:
+        raise ValueError(f"embedding: main_grad must be fp32 to be added to, got {mg.dtype}")
       kernels.embedding_bwd(ids, dout, mg, ctx.scale)
       return None, None, None
     g = torch.empty(ctx.shape, dtype=dout.dtype, device=dout.device)
@@ -288,8 +290,10 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> tor
   """Rows of `table` [V, D] times `scale`. The table's gradient is summed by sorted tokens: repeatable to the bit,
   fp32 sums rounded once, straight into `main_grad` where the table has one."""
   if _use_kernels(table) and table.shape[1] % 8 == 0 and table.is_contiguous() and table.data_ptr() % 16 == 0:
-    if not ids.is_cuda:
-      raise ValueError(f"embedding: ids are on {ids.device}, the table on {table.device}")
+    home = _lib.bind_thread()
+    if ids.get_device() != home or table.get_device() != home:
+      raise ValueError(f"embedding: ids are on {ids.device}, the table on {table.device}, "
+                       f"this process drives cuda:{home}")
     flat = ids if ids.dim() == 1 else ids.reshape(-1)
     if table.requires_grad and torch.is_grad_enabled():
       out = _EmbeddingFn.apply(flat, table, scale)
