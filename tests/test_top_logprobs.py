@@ -555,6 +555,15 @@ def test_another_device_than_the_process_is_refused(monkeypatch):
 
 
 @pytest.mark.gpu
+def test_more_rows_than_31_bits_are_refused():
+  x = torch.zeros(1, 1, device="cuda").expand(2 ** 31, 1)                  # no memory behind it
+  with pytest.raises(ValueError, match="31 bits"):
+    F.top_logprobs(x, 1)
+  with pytest.raises(ValueError, match="31 bits"):
+    F.top_distill_loss(x, torch.zeros(1, 1, dtype=torch.int64, device="cuda").expand(2 ** 31, 1), x)
+
+
+@pytest.mark.gpu
 def test_repeated_calls_agree_to_the_bit():
   """Candidates are collected in any order; what is reported does not depend on it."""
   x = make_logits(40, 50000, torch.bfloat16, "cuda")

@@ -1,18 +1,19 @@
 // Gradient of an embedding table, summed by sorted tokens: grad[v, :] (+)= scale * sum over the positions t with
 // ids[t] == v of dout[t, :], every sum in fp32, in one fixed order and without atomics.
 //
-// Launches. (1) The pairs (id, position) are sorted by id, equal ids by position. Few tokens: every pair counts the pairs
-// before it. More: one cluster, a radix sort from the low digit up whose per-warp digit counts live in shared memory and
-// whose per-block totals are read through distributed shared memory (12 us for 16384 tokens, 27 us for 65536: latency of
-// its few steps). A new gradient is cleared while the ids are sorted. (2) Blocks walk `chunk` sorted positions each. A
-// run of equal ids is summed by the block where it begins, also a little into the next chunk; a run that covers a whole
-// chunk (a frequent token, the padding id) is summed by every block it touches, into fp32 partial sums, so that one
-// token cannot keep a block busy alone. (3) The partial sums of such a run are added in order. dout is read once and
-// every present row of the table is touched once. Ids outside the vocabulary sort behind all others and are left out.
+// Launches. (1) The pairs (id, position) are sorted by id, equal ids by position. Few tokens: every pair counts the
+// pairs before it. More: one cluster, a radix sort from the low digit up whose per-warp digit counts live in shared
+// memory and whose per-block totals are read through distributed shared memory (12 us for 16384 tokens, 27 us for
+// 65536: latency of its few steps). A new gradient is cleared while the ids are sorted. (2) Blocks walk `chunk` sorted
+// positions each. A run of equal ids is summed by the block where it begins, also a little into the next chunk; a run
+// that covers a whole chunk (a frequent token, the padding id) is summed by every block it touches, into fp32 partial
+// sums, so that one token cannot keep a block busy alone. (3) The partial sums of such a run are added in order. dout
+// is read once and every present row of the table is touched once. Ids outside the vocabulary sort behind all others
+// and are left out.
 //
 // Blocks of (2) and (3) are launched before their predecessor ends and wait for it on the device (with plain launches 4
-// and 5 us more in the two cases below, 1 us of 7 for 512 tokens). Fetching a part of dout into L2 while the ids are sorted
-// gained nothing.
+// and 5 us more in the two cases below, 1 us of 7 for 512 tokens). Fetching a part of dout into L2 while the ids are
+// sorted gained nothing.
 //
 // 16384 tokens x 4096 into an fp32 buffer: 96 us (134 MB of dout and 115 MB of rows read and written: 3.8 TB/s).
 // 65536 x 1152, half of them one id, new table of 262144 rows: 145 us, of which 82 us write the table (604 MB).

@@ -84,9 +84,9 @@ __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
   return r;
 }
 
-// 2^t for two t <= 0 without the special function unit: 2^n from the exponent, n the nearest integer, times a polynomial
-// in the rest (|f| <= 1/2; degree 5, fitted for the smallest relative error: 2.2e-7 with fp32 roundings, as ex2). Below
-// -126 the result stays at 2^-126.
+// 2^t for two t <= 0 without the special function unit: 2^n from the exponent, n the nearest integer, times a
+// polynomial in the rest (|f| <= 1/2; degree 5, fitted for the smallest relative error: 2.2e-7 with fp32 roundings, as
+// ex2). Below -126 the result stays at 2^-126.
 __device__ __forceinline__ f32x2 ex2_by_fma(float a, float b) {
   const float kShift = 12582912.f;                 // 1.5 * 2^23: the sum's low bits are the nearest integer
   const f32x2 t = pack2(fmaxf(a, -126.f), fmaxf(b, -126.f));
@@ -204,8 +204,8 @@ __device__ __forceinline__ int2 part_of(int V, int rank, int blocks) {
 // ---- softmax statistics --------------------------------------------------------------------------------
 // A thread sums 2^(x c - M) with M = m c rounded: one packed multiply-add per two elements. The rounding of M is the
 // same in every term and is taken back from the logarithm at the end. Where m c leaves fp32, or every element lies
-// below the floor of the running maximum, the sum comes out as 0 (far below 1, where it should not) or NaN and the row is
-// summed again the careful way.
+// below the floor of the running maximum, the sum comes out as 0 (far below 1, where it should not) or NaN and the row
+// is summed again the careful way.
 constexpr int kNone = 0, kEntropy = 1, kSecond = 2;
 
 struct Stat {
@@ -297,8 +297,8 @@ __device__ __forceinline__ float warp_sum_of(float v) {
   return v;
 }
 
-// The block's statistics in every thread, the maximum first, then sums relative to it. Between the steps, and before `sh`
-// (kWarps entries) is used again, the block synchronises.
+// The block's statistics in every thread, the maximum first, then sums relative to it. Between the steps, and before
+// `sh` (kWarps entries) is used again, the block synchronises.
 __device__ __forceinline__ void stat_max(const Stat& a, Stat* sh) {
   const float m = warp_max_of(a.m);
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5].m = m;
@@ -336,13 +336,18 @@ __device__ __forceinline__ float log_sum(float s) { return s == 0.f ? INFINITY :
 
 // ln s of a positive, finite and normal s: the logarithm's argument is brought near 1, where its rounding is small.
 __device__ __forceinline__ double log_fine(float s) {
-  const int b = __float_as_int(s), e = (b - 0x3f400000) >> 23;       // s / 2^e is in [0.75, 1.5)
-  return fma(static_cast<double>(e), 0.69314718055994531, static_cast<double>(logf(__int_as_float(b - (e << 23)))));
+  int e;
+  float f = frexpf(s, &e);                                   // in [0.5, 1)
+  if (f < 0.75f) {
+    f += f;
+    --e;
+  }
+  return fma(static_cast<double>(e), 0.69314718055994531, static_cast<double>(logf(f)));
 }
 // ln sum exp((x - m) at the scale), from s = sum 2^(x c - M) with M rounded.
 __device__ __forceinline__ double log_fine(float s, float m, float c) {
-  return fma(-0.69314718055994531, fma(static_cast<double>(m), static_cast<double>(c), -static_cast<double>(scaled_max(m, c))),
-             log_fine(s));
+  const double rounded = fma(static_cast<double>(m), static_cast<double>(c), -static_cast<double>(scaled_max(m, c)));
+  return fma(-0.69314718055994531, rounded, log_fine(s));
 }
 
 // Row statistics from differences to the true maximum, by the whole block over the whole row.
@@ -402,9 +407,9 @@ __device__ __forceinline__ Row finish_row(const Stat& a, const LT* x, int V, Sta
 // Asks for what the warp reads in the iteration that begins at element `at`, 128 bytes per lane, so that its loads find
 // it in L2: a block's threads wait for each other only at a row's ends, but each has only one iteration's loads in
 // flight. One iteration ahead 8192 x 128256 bf16 with k = 64 takes 360 us, two 366 us, four 374 us, none 388 us; bulk
-// prefetches of 512 bytes 375 us. In the backward pass it pays where an element takes two terms (1000 x 262144 bf16 with
-// entropy: 163 us, 172 us without); with one, 4096 x 128256 takes 323 us instead of 326 us for itself, but 340 us instead
-// of 333 us in long runs under the power cap.
+// prefetches of 512 bytes 375 us. In the backward pass it pays where an element takes two terms (1000 x 262144 bf16
+// with entropy: 163 us, 172 us without); with one, 4096 x 128256 takes 323 us instead of 326 us for itself, but 340 us
+// instead of 333 us in long runs under the power cap.
 template <typename LT>
 __device__ __forceinline__ void ask_ahead(const LT* x, int at, int hi) {
   constexpr int line = 128 / sizeof(LT);                     // a warp's vectors side by side are four lines
@@ -477,8 +482,8 @@ __device__ __forceinline__ unsigned long long shfl_key(unsigned long long k, int
 }
 
 // Sorts n keys (all different) in shared memory from high to low. All threads call it. Short lists: four or two threads
-// count how many keys are above theirs. Longer ones: bitonic (slots n .. P-1 are filled with 0, P the next power of 2); up to
-// one key per thread stays in a register and strides below a warp are shuffles.
+// count how many keys are above theirs. Longer ones: bitonic (slots n .. P-1 are filled with 0, P the next power of 2);
+// up to one key per thread stays in a register and strides below a warp are shuffles.
 __device__ __forceinline__ void sort_keys(unsigned long long* keys, int n) {
   if (n <= kThreads / 2) {
     const int per = n <= kThreads / 4 ? 4 : 2, i = threadIdx.x / per, sub = threadIdx.x % per;
@@ -565,9 +570,9 @@ __device__ __forceinline__ float of_order(uint32_t o) {
   return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
 
-// The n-th largest number of a warp (1 <= n <= 32), neither 0 nor ~0 among them, from the nearer end: the extreme one is
-// taken away until it is that one's turn (8192 x 32000 bf16 with k = 20: 129 us, 135 us with a sort of the warp; with k =
-// 64, eight rounds, both are the same).
+// The n-th largest number of a warp (1 <= n <= 32), neither 0 nor ~0 among them, from the nearer end: the extreme one
+// is taken away until it is that one's turn (8192 x 32000 bf16 with k = 20: 129 us, 135 us with a sort of the warp;
+// with k = 64, eight rounds, both are the same).
 __device__ __forceinline__ uint32_t nth_largest(uint32_t v, int n) {
   const bool down = n <= 16;
   int left = down ? n : 33 - n;
@@ -858,13 +863,13 @@ __device__ __forceinline__ Stat top_of_part(Select& s, const LT* x, int base, in
 // A row per cluster of 1 .. kMaxSplit blocks, each with a part of the columns.
 //
 // Long rows with small k are bound by memory (8192 x 128256 bf16, k = 1: 312 us, 6.7 TB/s), with larger k by the
-// instructions of the selection, a fifth on top of those of the sums at k = 64 (349 us, 6.0 TB/s; k = 256: 430 us). Five
-// blocks of 256 threads per SM hide one row's serial parts (first threshold, last sort) behind the others' streaming.
-// Short rows are mostly those parts: 8192 x 32000, k = 20: 130 us, 4.0 TB/s (blocks of 128 threads take 113 us there, but
-// 357 us where this takes 349 us). Tried at 8192 x 128256, k = 64: a ring of asynchronous copies with two blocks per SM
-// 649 us where this took 415 us, two blocks per row 557 us and six blocks with 40 registers 390 us where it took 361 us.
-// 2047 x 151936 fp32 with entropy, k = 8: 198 us (6.3 TB/s). Under the power cap of a long run the clock falls and these
-// times grow by up to a tenth.
+// instructions of the selection, a fifth on top of those of the sums at k = 64 (349 us, 6.0 TB/s; k = 256: 430 us).
+// Five blocks of 256 threads per SM hide one row's serial parts (first threshold, last sort) behind the others'
+// streaming. Short rows are mostly those parts: 8192 x 32000, k = 20: 130 us, 4.0 TB/s (blocks of 128 threads take 113
+// us there, but 357 us where this takes 349 us). Tried at 8192 x 128256, k = 64: a ring of asynchronous copies with two
+// blocks per SM 649 us where this took 415 us, two blocks per row 557 us and six blocks with 40 registers 390 us where
+// it took 361 us. 2047 x 151936 fp32 with entropy, k = 8: 198 us (6.3 TB/s). Under the power cap of a long run the
+// clock falls and these times grow by up to a tenth.
 template <typename LT, int X>
 __global__ void __launch_bounds__(kThreads, X == kNone ? 5 : 4) top_fwd_kernel(TopArgs a) {
   extern __shared__ __align__(16) unsigned char shared[];
@@ -959,7 +964,8 @@ constexpr int kDistillStats = 8;
 // A divergence is a sum of differences of log-probabilities that can be much smaller than these: they are formed in 64
 // bits, a few operations per entry, where roundings in 32 bits were 2e-6 of the result and more.
 template <typename LT>
-__device__ __forceinline__ void distill_list(const DistillArgs& a, int row, const LT* x, float m, float ls1, double ls2) {
+__device__ __forceinline__ void distill_list(const DistillArgs& a, int row, const LT* x, float m, float ls1,
+                                             double ls2) {
   const int lane = threadIdx.x & 31, V = a.V, k = a.k;
   const long long* ids = a.ids + static_cast<long long>(row) * k;
   const float* values = a.values + static_cast<long long>(row) * k;
@@ -1027,7 +1033,8 @@ template <typename LT>
 __global__ void __launch_bounds__(kThreads) distill_list_kernel(DistillArgs a) {
   const int row = blockIdx.x * kWarps + (threadIdx.x >> 5);
   if (row >= a.T) return;
-  distill_list(a, row, static_cast<const LT*>(a.logits) + static_cast<long long>(row) * a.ld, -FLT_MAX, INFINITY, INFINITY);
+  const LT* x = static_cast<const LT*>(a.logits) + static_cast<long long>(row) * a.ld;
+  distill_list(a, row, x, -FLT_MAX, INFINITY, INFINITY);
 }
 
 // X: kNone (one softmax sum of the row, scale c1 in the exponent) or kSecond (c1 and c2). One sum is bound by memory

@@ -516,6 +516,8 @@ def _rows(name: str, logits: torch.Tensor) -> Optional[torch.Tensor]:
   if logits.get_device() != home:
     raise ValueError(f"{name}: logits are on {logits.device}, this process drives cuda:{home}")
   x2 = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])     # a view is a node of the graph
+  if max(x2.shape) > 0x7fff0000:
+    raise ValueError(f"{name}: rows and columns are counted in 31 bits, got {tuple(x2.shape)}")
   if x2.stride(1) != 1 and x2.shape[1] > 1 or x2.stride(0) < x2.shape[1] and x2.shape[0] > 1:
     x2 = x2.contiguous()
   return x2
