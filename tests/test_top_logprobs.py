@@ -594,3 +594,28 @@ def test_extreme_temperatures(device, tau):
   p, lp = log_softmax64(x.to(f64) / tau).exp(), log_softmax64(x.to(f64) / tau)
   size = torch.where(p > 0, p * lp.abs(), torch.zeros_like(p)).sum(1) + math.log(6001)
   close(got.entropy, want["entropy"], 4 * lse_tol(x, tau) * (1 + size) + U * 100 * size, "entropy")
+
+
+# ------------------------------------------------------------------------------ derivatives of other kinds
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_tangent_is_taken_along_or_refused(device):
+  """Forward mode: the plain statement on the CPU has it, the kernels refuse a dual tensor rather than drop its tangent."""
+  from torch.autograd import forward_ad
+  x = make_logits(3, 50, torch.float32, device)
+  v = torch.randn(3, 50, generator=torch.Generator().manual_seed(5)).to(device)
+  ids, values = make_list(x, 4)
+  table = torch.randn(9, 16, generator=torch.Generator().manual_seed(6)).to(device, torch.bfloat16 if device == "cuda" else torch.float32)
+  at = torch.arange(6, device=device)
+  calls = [(x, v, lambda z: F.top_logprobs(z, 4).top), (x, v, lambda z: F.top_distill_loss(z, ids, values).kl),
+           (table, torch.ones_like(table), lambda z: F.embedding(at, z, 2.0))]
+  with forward_ad.dual_level():
+    for t, tangent, fn in calls:
+      dual = forward_ad.make_dual(t, tangent)
+      if device == "cuda":
+        with pytest.raises(NotImplementedError):
+          fn(dual)
+        assert forward_ad.unpack_dual(fn(t)).tangent is None            # others are not affected
+      else:
+        assert forward_ad.unpack_dual(fn(dual)).tangent is not None
+    with pytest.raises(ValueError, match="detach"):
+      F.top_distill_loss(x, ids, forward_ad.make_dual(values, torch.ones_like(values)))

@@ -17,6 +17,7 @@ from typing import NamedTuple, Optional, Tuple
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from . import _lib, kernels, ref
 
@@ -31,6 +32,16 @@ def _use_kernels(*ts: torch.Tensor) -> bool:
     return False
   _lib.require()  # a CUDA bf16 tensor without the library is an error, never a silent fallback
   return True
+
+
+def _is_dual(t: torch.Tensor) -> bool:
+  return forward_ad.unpack_dual(t).tangent is not None
+
+
+def _differentiated(t: torch.Tensor) -> bool:
+  """Whether an operator on `t` has to go through its `Function`: a backward pass may follow, or `t` carries a tangent,
+  which the `Function` refuses where the kernel alone would drop it."""
+  return t.requires_grad and torch.is_grad_enabled() or _is_dual(t)
 
 
 def _main_grad(p: torch.Tensor) -> Optional[torch.Tensor]:
@@ -295,7 +306,7 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> tor
       raise ValueError(f"embedding: ids are on {ids.device}, the table on {table.device}, "
                        f"this process drives cuda:{home}")
     flat = ids if ids.dim() == 1 else ids.reshape(-1)
-    if table.requires_grad and torch.is_grad_enabled():
+    if _differentiated(table):
       out = _EmbeddingFn.apply(flat, table, scale)
     else:
       out = kernels.embedding_fwd(flat, table, scale)
@@ -556,7 +567,7 @@ def top_logprobs(logits: torch.Tensor, k: int, targets: Optional[torch.Tensor] =
   else:
     if k > kernels.MAX_TOP_K:
       raise ValueError(f"top_logprobs: k is at most {kernels.MAX_TOP_K} on the GPU, got {k}")
-    if x2.requires_grad and torch.is_grad_enabled():
+    if _differentiated(x2):
       ids, top, target, ent = _TopLogprobsFn.apply(x2, k, tg, 1.0 / float(temperature), bool(want_entropy))
     else:
       ids, top, target, ent, _ = kernels.top_logprobs_fwd(x2, k, tg, 1.0 / float(temperature), bool(want_entropy))
@@ -594,7 +605,7 @@ def top_distill_loss(logits: torch.Tensor, top_ids: torch.Tensor, top_values: to
                      f"got {top_values.dtype} {tuple(top_values.shape)}")
   if top_values.device != logits.device:
     raise ValueError(f"top_distill_loss: top_values is on {top_values.device}, the logits on {logits.device}")
-  if top_values.requires_grad and torch.is_grad_enabled():
+  if _differentiated(top_values):
     raise ValueError("top_distill_loss: the teacher's values get no gradient; detach them")
   x2 = _rows("top_distill_loss", logits)
   ids, tg = _ids64(top_ids, -1, k), _ids64(labels, -1)
@@ -607,7 +618,7 @@ def top_distill_loss(logits: torch.Tensor, top_ids: torch.Tensor, top_values: to
     values = top_values
     if values.dtype != torch.float32 or values.dim() != 2 or values.requires_grad or not values.is_contiguous():
       values = values.detach().reshape(-1, k).float().contiguous()
-    if x2.requires_grad and torch.is_grad_enabled():
+    if _differentiated(x2):
       kl, nll = _TopDistillFn.apply(x2, ids, values, tg, 1.0 / float(temperature), full)
     else:
       kl, nll, _ = kernels.top_distill_fwd(x2, ids, values, tg, 1.0 / float(temperature), full)
