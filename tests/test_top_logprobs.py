@@ -619,3 +619,15 @@ def test_a_tangent_is_taken_along_or_refused(device):
         assert forward_ad.unpack_dual(fn(dual)).tangent is not None
     with pytest.raises(ValueError, match="detach"):
       F.top_distill_loss(x, ids, forward_ad.make_dual(values, torch.ones_like(values)))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("tau", [1e-18, 1e-9, 1e-3, 1e9])
+def test_gradients_at_extreme_temperatures(device, tau):
+  """With masked columns; the smallest temperatures make factors that overflow against an unbounded exponent."""
+  x = make_logits(3, 6000, torch.float32, device)
+  x[:, 77] = x.amax(1) + 1.0                                       # a clear best token
+  x[:, 100:2000] = LOW
+  x[1, 2000:2100] = -1e4
+  check_score(x, 5, torch.full((3,), 77, device=device), tau, eps(x.dtype))
+  check_score(x, 5, torch.full((3,), 2000, device=device), tau, eps(x.dtype))

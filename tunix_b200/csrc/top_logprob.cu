@@ -1222,7 +1222,8 @@ __global__ void __launch_bounds__(kThreads) top_bwd_kernel(BwdArgs a) {
       const float2 e = unpack2(fma2(d, cc, ll));
       const f32x2 p = pack2(ex2(e.x), ex2(e.y));
       if (DENSE & 4)
-        r = mul2(p, fma2(GG, pack2(fmaxf(e.x, -1e30f), fmaxf(e.y, -1e30f)), AA));
+        // below 2^-126 p is 0: the exponent is bounded there, or its product with G could leave fp32 and 0 * inf is NaN
+        r = mul2(p, fma2(GG, pack2(fmaxf(e.x, -200.f), fmaxf(e.y, -200.f)), AA));
       else
         r = mul2(p, AA);
     }
