@@ -206,3 +206,37 @@ def test_captured_step_and_two_streams(kernel_lib):
   for n in range(2):
     for r in got[n]:
       assert all(torch.equal(a, b) for a, b in zip(r, want[n]))
+
+
+# ------------------------------------------------------------------------------ what the strategy took before it had a list
+def rows64(s, t, ids, k, tau, alpha):
+  """The strategy's loss in 64 bits, differentiable in both logits."""
+  s, t = s.to(f64), t.to(f64)
+  tk, idx = torch.topk(t, k, dim=-1)
+  lq, lp = F.log_softmax(tk / tau, -1), F.log_softmax(s.gather(-1, idx) / tau, -1)
+  soft = (lq.exp() * (lq - lp)).sum(-1).mean() * tau * tau
+  return alpha * soft + (1 - alpha) * -F.log_softmax(s, -1).gather(-1, ids[..., None]).mean()
+
+
+def some_logits(T, V, device, seed=0):
+  """Student, teacher with distinct values in every row, labels."""
+  g = torch.Generator().manual_seed(seed)
+  t = torch.stack([torch.randperm(V, generator=g) for _ in range(T)]).float() * 0.0625
+  return (torch.randn(T, V, generator=g) * 2).to(device), t.to(device), torch.randint(0, V, (T,), generator=g).to(device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_teacher_with_a_graph_gets_its_gradient(device):
+  T, V, k, tau, alpha = 5, 300, 8, 2.0, 0.6
+  s, t, ids = some_logits(T, V, device)
+  t = t.requires_grad_()
+  loss, _ = strategy(temperature=tau, alpha=alpha, distill_top_k=k).compute_loss(s, t, ids)
+  grad, = torch.autograd.grad(loss, t)
+  want, = torch.autograd.grad(rows64(s, t, ids, k, tau, alpha), t)
+  tk, idx = torch.topk(t.detach().to(f64), k, dim=-1)
+  lq, lp = F.log_softmax(tk / tau, -1), F.log_softmax(s.to(f64).gather(-1, idx) / tau, -1)
+  # d/dt = alpha tau / T q (lq - lp - kl): logits of at most 64 in size make log-probabilities that are off by 8 roundings
+  # of that, 512 U, so the bracket is off by 2048 U and every factor by 1024 U of its size
+  size = alpha * tau / T * lq.exp() * (1 + (lq - lp).abs() + (lq.exp() * (lq - lp)).sum(-1, keepdim=True))
+  tol = torch.zeros(T, V, dtype=f64, device=device).scatter_(-1, idx, 4096 * U * size)
+  assert float(((grad.to(f64) - want).abs() - tol).max()) <= 0

@@ -49,10 +49,17 @@ class LogitStrategy(BaseStrategy):
       metrics["distill/teacher_loss"] = teacher.detach()
     return loss, metrics
 
+  def _takes_list(self, student_output, teacher_output) -> bool:
+    """Whether these logits go through the teacher's list: what the operators do not take stays with the formulas."""
+    s, t, k = student_output, teacher_output, self.distill_top_k
+    if not s.is_cuda or not {s.dtype, t.dtype} <= {torch.float32, torch.bfloat16}:
+      return False
+    if not 0 < k <= min(kernels.MAX_TOP_K, t.shape[-1]):
+      return False
+    return not (t.requires_grad and torch.is_grad_enabled())           # a list has no gradient for the teacher
+
   def compute_loss(self, student_output, teacher_output, labels):
-    if isinstance(teacher_output, functional.TopLogprobs) or (
-        student_output.is_cuda and 0 < self.distill_top_k <= min(kernels.MAX_TOP_K, teacher_output.shape[-1])
-        and {student_output.dtype, teacher_output.dtype} <= {torch.float32, torch.bfloat16}):
+    if isinstance(teacher_output, functional.TopLogprobs) or self._takes_list(student_output, teacher_output):
       return self._compute_listed_loss(student_output, teacher_output, labels)
     s, t = student_output.float(), teacher_output.float()
     sk, tk = s, t
