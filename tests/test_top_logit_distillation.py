@@ -240,3 +240,33 @@ def test_a_teacher_with_a_graph_gets_its_gradient(device):
   size = alpha * tau / T * lq.exp() * (1 + (lq - lp).abs() + (lq.exp() * (lq - lp)).sum(-1, keepdim=True))
   tol = torch.zeros(T, V, dtype=f64, device=device).scatter_(-1, idx, 4096 * U * size)
   assert float(((grad.to(f64) - want).abs() - tol).max()) <= 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("way", ["dual", "jvp", "grad", "vmap"])
+def test_forward_mode_and_function_transforms_of_the_strategy(device, way):
+  from torch.autograd import forward_ad
+  T, V, k, tau, alpha = 5, 300, 8, 2.0, 0.6
+  s, t, ids = some_logits(T, V, device)
+  strat = strategy(temperature=tau, alpha=alpha, distill_top_k=k)
+  v = torch.randn(T, V, generator=torch.Generator().manual_seed(9)).to(device)
+  fn = lambda z: strat.compute_loss(z, t, ids)[0]   # noqa: E731
+  leaf = s.to(f64).requires_grad_()
+  want, = torch.autograd.grad(rows64(leaf, t, ids, k, tau, alpha), leaf)
+  terms = loss64(s[None], t[None], ids[None], k, tau, alpha)[3][0]
+  if way == "grad":
+    assert float(((torch.func.grad(fn)(s).to(f64) - want).abs() - 1024 * U * terms).max()) <= 0
+  elif way == "vmap":
+    two = torch.func.vmap(fn)(torch.stack([s, s + v]))
+    alone = torch.stack([rows64(s, t, ids, k, tau, alpha), rows64(s + v, t, ids, k, tau, alpha)])
+    # as in test_strategy_over_logits_and_over_a_list
+    assert float((two.to(f64) - alone).abs().max()) <= 64 * 16 * U * (tau * tau + 1)
+  else:
+    if way == "dual":
+      with forward_ad.dual_level():
+        tangent = forward_ad.unpack_dual(fn(forward_ad.make_dual(s, v))).tangent
+    else:
+      tangent = torch.func.jvp(fn, (s,), (v,))[1]
+    assert tangent is not None
+    # every product of a gradient (1024 U of its terms) and the tangent, in a sum of T V terms in any order
+    assert abs(float(tangent) - float((want * v).sum())) <= (1024 + T * V) * U * float((terms * v.abs()).sum())

@@ -56,7 +56,10 @@ class LogitStrategy(BaseStrategy):
       return False
     if not 0 < k <= min(kernels.MAX_TOP_K, t.shape[-1]):
       return False
-    return not (t.requires_grad and torch.is_grad_enabled())           # a list has no gradient for the teacher
+    if t.requires_grad and torch.is_grad_enabled():                    # a list has no gradient for the teacher
+      return False
+    # forward mode and the transforms of torch.func
+    return not (functional.is_dual(s) or functional.is_dual(t) or torch._C._are_functorch_transforms_active())
 
   def compute_loss(self, student_output, teacher_output, labels):
     if isinstance(teacher_output, functional.TopLogprobs) or self._takes_list(student_output, teacher_output):

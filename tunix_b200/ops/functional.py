@@ -34,14 +34,15 @@ def _use_kernels(*ts: torch.Tensor) -> bool:
   return True
 
 
-def _is_dual(t: torch.Tensor) -> bool:
+def is_dual(t: torch.Tensor) -> bool:
+  """Whether `t` carries a tangent of forward-mode differentiation."""
   return forward_ad.unpack_dual(t).tangent is not None
 
 
 def _differentiated(t: torch.Tensor) -> bool:
   """Whether an operator on `t` has to go through its `Function`: a backward pass may follow, or `t` carries a tangent,
   which the `Function` refuses where the kernel alone would drop it."""
-  return t.requires_grad and torch.is_grad_enabled() or _is_dual(t)
+  return t.requires_grad and torch.is_grad_enabled() or is_dual(t)
 
 
 def _main_grad(p: torch.Tensor) -> Optional[torch.Tensor]:
