@@ -270,3 +270,14 @@ def test_forward_mode_and_function_transforms_of_the_strategy(device, way):
     assert tangent is not None
     # every product of a gradient (1024 U of its terms) and the tangent, in a sum of T V terms in any order
     assert abs(float(tangent) - float((want * v).sum())) <= (1024 + T * V) * U * float((terms * v.abs()).sum())
+
+
+@pytest.mark.gpu
+def test_strategy_on_another_device_than_the_process(monkeypatch):
+  from tunix_b200.ops import _lib
+  s, t, ids = some_logits(5, 300, "cuda")
+  strat = strategy(temperature=2.0, alpha=0.6, distill_top_k=8)
+  want = rows64(s, t, ids, 8, 2.0, 0.6)
+  monkeypatch.setattr(_lib, "bind_thread", lambda: 1)
+  loss, _ = strat.compute_loss(s, t, ids)
+  assert abs(float(loss) - float(want)) <= 64 * 16 * U * 5

@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 
-from ...ops import functional, kernels
+from ...ops import _lib, functional, kernels
 from .base_strategy import BaseStrategy, softmax_cross_entropy
 
 
@@ -53,6 +53,8 @@ class LogitStrategy(BaseStrategy):
     """Whether these logits go through the teacher's list: what the operators do not take stays with the formulas."""
     s, t, k = student_output, teacher_output, self.distill_top_k
     if not s.is_cuda or not {s.dtype, t.dtype} <= {torch.float32, torch.bfloat16}:
+      return False
+    if not s.get_device() == t.get_device() == _lib.bind_thread():     # the kernels' GPU is the process's
       return False
     if not 0 < k <= min(kernels.MAX_TOP_K, t.shape[-1]):
       return False
