@@ -281,3 +281,16 @@ def test_strategy_on_another_device_than_the_process(monkeypatch):
   monkeypatch.setattr(_lib, "bind_thread", lambda: 1)
   loss, _ = strat.compute_loss(s, t, ids)
   assert abs(float(loss) - float(want)) <= 64 * 16 * U * 5
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_strategy_temperatures_and_rows_beyond_the_operators(device):
+  """A temperature that the operators refuse, and a teacher of fewer rows than the student (compared over its own)."""
+  s, t, ids = some_logits(6, 300, device)
+  loss, _ = strategy(temperature=1e19, alpha=0.0, distill_top_k=8).compute_loss(s, t, ids)
+  assert abs(float(loss) - float(rows64(s, t, ids, 8, 1.0, 0.0))) <= 64 * 16 * U * 2
+  s3, t3 = s.view(2, 3, 300), t.view(2, 3, 300)[:, :2]
+  strat = strategy(temperature=2.0, alpha=1.0, distill_top_k=8)
+  fewer, _ = strat.compute_loss(s3, t3, torch.zeros(2, 1, 300, device=device))
+  want = rows64(s3[:, :2].reshape(4, 300), t3.reshape(4, 300), ids[:4], 8, 2.0, 1.0)
+  assert abs(float(fewer) - float(want)) <= 64 * 16 * U * 5

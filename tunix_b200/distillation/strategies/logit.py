@@ -56,7 +56,9 @@ class LogitStrategy(BaseStrategy):
       return False
     if not s.get_device() == t.get_device() == _lib.bind_thread():     # the kernels' GPU is the process's
       return False
-    if not 0 < k <= min(kernels.MAX_TOP_K, t.shape[-1]):
+    if not 0 < k <= min(kernels.MAX_TOP_K, t.shape[-1]) or s.shape[:-1] != t.shape[:-1]:
+      return False
+    if not functional.MIN_TEMPERATURE <= self.temperature <= functional.MAX_TEMPERATURE:
       return False
     if t.requires_grad and torch.is_grad_enabled():                    # a list has no gradient for the teacher
       return False

@@ -432,6 +432,9 @@ def linear_logprob(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Te
 
 
 # ------------------------------------------------------------------------------ alternatives of a row of logits
+MIN_TEMPERATURE, MAX_TEMPERATURE = 1e-18, 1e18       # the inverse and products with logits stay within fp32
+
+
 class TopLogprobs(NamedTuple):
   """What `top_logprobs` says of every row of logits."""
   ids: torch.Tensor                    # int64 [..., k], likeliest first
@@ -505,7 +508,7 @@ def _check_rows(name: str, logits: torch.Tensor, temperature: float) -> None:
   """Arguments that `top_logprobs` and `top_distill_loss` share: floating logits [..., V], a positive temperature."""
   if logits.dim() < 1 or not logits.is_floating_point():
     raise ValueError(f"{name}: logits must be a floating tensor [..., V], got {logits.dtype} {tuple(logits.shape)}")
-  if not 1e-18 <= temperature <= 1e18:       # its inverse and products with logits stay within fp32
+  if not MIN_TEMPERATURE <= temperature <= MAX_TEMPERATURE:
     raise ValueError(f"{name}: temperature must be positive and finite (1e-18 to 1e18), got {temperature}")
 
 
