@@ -294,3 +294,24 @@ def test_strategy_temperatures_and_rows_beyond_the_operators(device):
   fewer, _ = strat.compute_loss(s3, t3, torch.zeros(2, 1, 300, device=device))
   want = rows64(s3[:, :2].reshape(4, 300), t3.reshape(4, 300), ids[:4], 8, 2.0, 1.0)
   assert abs(float(fewer) - float(want)) <= 64 * 16 * U * 5
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_second_derivatives_through_the_strategy(device):
+  T, V, k, tau, alpha = 3, 40, 6, 2.0, 0.6
+  s, t, ids = some_logits(T, V, device)
+  v = torch.randn(T, V, generator=torch.Generator().manual_seed(9)).to(device)
+  strat = strategy(temperature=tau, alpha=alpha, distill_top_k=k)
+  for stored in (False, True):
+    leaf, leaf64 = s.clone().requires_grad_(), s.to(f64).requires_grad_()
+    teacher = functional.top_logprobs(t, k, ids) if stored else t
+    g, = torch.autograd.grad(strat.compute_loss(leaf, teacher, ids)[0], leaf, create_graph=True)
+    hv, = torch.autograd.grad((g * v).sum(), leaf)
+    g64, = torch.autograd.grad(rows64(leaf64, t, ids, k, tau, alpha), leaf64, create_graph=True)
+    hv64, = torch.autograd.grad((g64 * v).sum(), leaf64)
+    # rows of H v: w p (v - p.v) for each of the two softmaxes, w <= 1 / T; a probability is off by 1024 U of its size,
+    # its product with v - p.v by 4096 U of p (|v| + 1) max |v|
+    lp, at = F.log_softmax(s.to(f64), -1).exp(), torch.topk(t, k, -1).indices
+    ps = F.log_softmax(s.to(f64).gather(-1, at) / tau, -1).exp()
+    size = (1 - alpha) / T * lp + torch.zeros_like(lp).scatter_(-1, at, alpha / T * ps)
+    assert float(((hv.to(f64) - hv64).abs() - 4096 * U * size * (v.abs() + 1) * float(v.abs().max())).max()) <= 0

@@ -39,7 +39,8 @@ class LogitStrategy(BaseStrategy):
         top = functional.top_logprobs(teacher_output.detach(), self.distill_top_k, ids)
         teacher = -top.target.mean() if ids is not None else softmax_cross_entropy(teacher_output, labels).mean()
     k = min(top.ids.shape[-1], self.distill_top_k or V)
-    terms = functional.top_distill_loss(student_output, top.ids[..., :k], top.top.detach()[..., :k], ids, self.temperature)
+    terms = functional.top_distill_loss(student_output, top.ids[..., :k], top.top.detach()[..., :k], ids, self.temperature,
+                                        twice=True)
     soft = (terms.kl * self.temperature ** 2).mean()
     hard = terms.nll.mean() if ids is not None else softmax_cross_entropy(student_output, labels).mean()
     loss = self.alpha * soft + (1.0 - self.alpha) * hard

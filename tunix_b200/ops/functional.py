@@ -488,20 +488,25 @@ class _TopLogprobsFn(torch.autograd.Function):
 class _TopDistillFn(torch.autograd.Function):
 
   @staticmethod
-  def forward(ctx, x2, ids, values, labels, inv_temp, full):
+  def forward(ctx, x2, ids, values, labels, inv_temp, full, temperature):
     kl, nll, ctx.stats = kernels.top_distill_fwd(x2, ids, values, labels, inv_temp, full)
     ctx.save_for_backward(x2, ids, values, labels)
-    ctx.cfg = (inv_temp, full)
+    ctx.cfg, ctx.again = (inv_temp, full), temperature
     ctx.set_materialize_grads(False)
     return kl, nll
 
   @staticmethod
   def backward(ctx, g_kl, g_nll):
     x2, ids, values, labels = ctx.saved_tensors
+    rest = (None,) * 6
     if g_kl is None and g_nll is None:
-      return None, None, None, None, None, None
+      return None, *rest
+    if ctx.again is not None and torch.is_grad_enabled():
+      outs = ref.top_distill_loss(x2, ids, values, labels, ctx.again, ctx.cfg[1])
+      pairs = [(o, g) for o, g in zip(outs, (g_kl, g_nll)) if g is not None]
+      return torch.autograd.grad([o for o, _ in pairs], x2, [g for _, g in pairs], create_graph=True)[0], *rest
     dx = kernels.top_distill_bwd(x2, ids, values, labels, ctx.stats, _grad32(g_kl), _grad32(g_nll), *ctx.cfg)
-    return _once(dx), None, None, None, None, None
+    return _once(dx), *rest
 
 
 def _check_rows(name: str, logits: torch.Tensor, temperature: float) -> None:
@@ -580,7 +585,7 @@ def top_logprobs(logits: torch.Tensor, k: int, targets: Optional[torch.Tensor] =
 
 def top_distill_loss(logits: torch.Tensor, top_ids: torch.Tensor, top_values: torch.Tensor,
                      labels: Optional[torch.Tensor] = None, temperature: float = 1.0,
-                     normalize: str = "top") -> DistillLoss:
+                     normalize: str = "top", twice: bool = False) -> DistillLoss:
   """Distillation from a teacher's best tokens: per row of the student's logits [..., V] the divergence from the
   teacher's list (`top_ids`, `top_values` [..., k]) and, with `labels` [...], the cross entropy at temperature 1.
 
@@ -593,6 +598,8 @@ def top_distill_loss(logits: torch.Tensor, top_ids: torch.Tensor, top_values: to
   The gradient goes to the logits only. An id outside the vocabulary is an absent entry and a label outside it is
   ignored; an entry of probability 0 adds nothing. A row without a usable entry (no id left, teacher's values all
   -inf, student's logits there all -inf) has divergence 0 and no gradient, a row of -inf also no cross entropy.
+  With `twice` a backward pass that builds a graph takes the plain statement, whose gradient can be differentiated
+  again; without it such a gradient leads to an error.
   fp32 and bf16 logits on the GPU take one kernel in each direction; there the list has at most 1024 entries."""
   _check_rows("top_distill_loss", logits, temperature)
   V, lead = logits.shape[-1], logits.shape[:-1]
@@ -623,7 +630,8 @@ def top_distill_loss(logits: torch.Tensor, top_ids: torch.Tensor, top_values: to
     if values.dtype != torch.float32 or values.dim() != 2 or values.requires_grad or not values.is_contiguous():
       values = values.detach().reshape(-1, k).float().contiguous()
     if _differentiated(x2):
-      kl, nll = _TopDistillFn.apply(x2, ids, values, tg, 1.0 / float(temperature), full)
+      kl, nll = _TopDistillFn.apply(x2, ids, values, tg, 1.0 / float(temperature), full,
+                                    float(temperature) if twice else None)
     else:
       kl, nll, _ = kernels.top_distill_fwd(x2, ids, values, tg, 1.0 / float(temperature), full)
   return DistillLoss(_lead(kl, *lead), _lead(nll, *lead))
