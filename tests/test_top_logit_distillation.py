@@ -315,3 +315,27 @@ def test_second_derivatives_through_the_strategy(device):
     ps = F.log_softmax(s.to(f64).gather(-1, at) / tau, -1).exp()
     size = (1 - alpha) / T * lp + torch.zeros_like(lp).scatter_(-1, at, alpha / T * ps)
     assert float(((hv.to(f64) - hv64).abs() - 4096 * U * size * (v.abs() + 1) * float(v.abs().max())).max()) <= 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("top_k", [0, 8])
+@pytest.mark.parametrize("stored", [False, True])
+@pytest.mark.parametrize("label", [-100, 300])
+def test_labels_outside_the_vocabulary_are_an_error(device, top_k, stored, label):
+  """On the host they raise; on the GPU, where the host would have to wait for the labels, the loss and its gradient are
+  NaN. The same with and without a list."""
+  s, t, ids = some_logits(4, 300, device)
+  s = s.requires_grad_()
+  teacher = functional.top_logprobs(t, 8, ids) if stored else t
+  strat = strategy(temperature=2.0, alpha=0.6, distill_top_k=top_k)
+  good, _ = strat.compute_loss(s, teacher, ids)
+  assert math.isfinite(float(good.detach()))
+  ids = ids.clone()
+  ids[2] = label
+  if device == "cpu":
+    with pytest.raises(RuntimeError, match="out of bounds|outside"):
+      strat.compute_loss(s, teacher, ids)
+    return
+  loss, m = strat.compute_loss(s, teacher, ids)
+  assert math.isnan(float(loss.detach())) and math.isnan(float(m["distill/hard_loss"]))
+  assert bool(torch.autograd.grad(loss, s)[0].isnan().any())

@@ -8,6 +8,8 @@ in the place of its logits: a `teacher_forward_fn` that returns `ops.functional.
 stored earlier, keeps k numbers per token instead of V."""
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn.functional as F
 
@@ -15,7 +17,26 @@ from ...ops import _lib, functional, kernels
 from .base_strategy import BaseStrategy, softmax_cross_entropy
 
 
+def _class_ids(logits, labels):
+  """Integer labels as ids, None for distributions over the vocabulary."""
+  if labels.dtype in (torch.int32, torch.int64, torch.int16, torch.uint8) and labels.ndim == logits.ndim - 1:
+    return labels.long()
+  return None
+
+
+def _refuse(outside, what):
+  """Ids outside the vocabulary are an error: on the host it is raised. On the GPU, where the host would have to wait to
+  see them, the answer is a factor for the loss, 1 or, where there are some, NaN."""
+  if outside.is_cuda:
+    return torch.where(outside.any(), math.nan, 1.0)
+  if bool(outside.any()):
+    raise RuntimeError(f"LogitStrategy: {what} outside the vocabulary")
+  return 1.0
+
+
 class LogitStrategy(BaseStrategy):
+  """Integer labels outside the vocabulary raise on the CPU and make the loss NaN on the GPU, with and without a top-k."""
+
   def __init__(self, student_forward_fn, teacher_forward_fn, labels_fn, temperature: float = 2.0,
                alpha: float = 0.5, distill_top_k: int = 0):
     super().__init__(student_forward_fn, teacher_forward_fn, labels_fn)
@@ -29,20 +50,23 @@ class LogitStrategy(BaseStrategy):
     return softmax_cross_entropy(student_output, labels).mean(), {}
 
   def _compute_listed_loss(self, student_output, teacher_output, labels):
-    V = student_output.shape[-1]
-    ids = labels.long() if not labels.is_floating_point() and labels.ndim == student_output.ndim - 1 else None
-    if isinstance(teacher_output, functional.TopLogprobs):
+    V, stored = student_output.shape[-1], isinstance(teacher_output, functional.TopLogprobs)
+    ids, sound = _class_ids(student_output, labels), 1.0
+    if ids is not None:
+      known = ids.clamp(0, (V if stored else min(V, teacher_output.shape[-1])) - 1)
+      ids, sound = known, _refuse(known != ids, "labels")
+    if stored:
       top = teacher_output
       teacher = None if top.target is None else -top.target.mean()
     else:
       with torch.no_grad():
         top = functional.top_logprobs(teacher_output.detach(), self.distill_top_k, ids)
-        teacher = -top.target.mean() if ids is not None else softmax_cross_entropy(teacher_output, labels).mean()
+        teacher = (-top.target.mean() if ids is not None else softmax_cross_entropy(teacher_output, labels).mean()) * sound
     k = min(top.ids.shape[-1], self.distill_top_k or V)
     terms = functional.top_distill_loss(student_output, top.ids[..., :k], top.top.detach()[..., :k], ids, self.temperature,
                                         twice=True)
     soft = (terms.kl * self.temperature ** 2).mean()
-    hard = terms.nll.mean() if ids is not None else softmax_cross_entropy(student_output, labels).mean()
+    hard = (terms.nll.mean() if ids is not None else softmax_cross_entropy(student_output, labels).mean()) * sound
     loss = self.alpha * soft + (1.0 - self.alpha) * hard
     metrics = {"distill/soft_loss": soft.detach(), "distill/hard_loss": hard.detach(),
                "distill/kl_div": terms.kl.mean().detach()}
@@ -50,7 +74,7 @@ class LogitStrategy(BaseStrategy):
       metrics["distill/teacher_loss"] = teacher.detach()
     return loss, metrics
 
-  def _takes_list(self, student_output, teacher_output) -> bool:
+  def _takes_list(self, student_output, teacher_output, labels) -> bool:
     """Whether these logits go through the teacher's list: what the operators do not take stays with the formulas."""
     s, t, k = student_output, teacher_output, self.distill_top_k
     if not s.is_cuda or not {s.dtype, t.dtype} <= {torch.float32, torch.bfloat16}:
@@ -58,6 +82,9 @@ class LogitStrategy(BaseStrategy):
     if not s.get_device() == t.get_device() == _lib.bind_thread():     # the kernels' GPU is the process's
       return False
     if not 0 < k <= min(kernels.MAX_TOP_K, t.shape[-1]) or s.shape[:-1] != t.shape[:-1]:
+      return False
+    ids = _class_ids(s, labels)
+    if ids is not None and (ids.shape != s.shape[:-1] or ids.device != s.device):
       return False
     if not functional.MIN_TEMPERATURE <= self.temperature <= functional.MAX_TEMPERATURE:
       return False
@@ -67,7 +94,7 @@ class LogitStrategy(BaseStrategy):
     return not (functional.is_dual(s) or functional.is_dual(t) or torch._C._are_functorch_transforms_active())
 
   def compute_loss(self, student_output, teacher_output, labels):
-    if isinstance(teacher_output, functional.TopLogprobs) or self._takes_list(student_output, teacher_output):
+    if isinstance(teacher_output, functional.TopLogprobs) or self._takes_list(student_output, teacher_output, labels):
       return self._compute_listed_loss(student_output, teacher_output, labels)
     s, t = student_output.float(), teacher_output.float()
     sk, tk = s, t
@@ -79,9 +106,13 @@ class LogitStrategy(BaseStrategy):
     pt = log_pt.exp()
     kl = (pt * (torch.where(pt > 0, log_pt, torch.zeros_like(log_pt)) - log_ps)).sum(-1)
     soft = (kl * self.temperature ** 2).mean()
-    hard = softmax_cross_entropy(s, labels).mean()
+    ids, sound = _class_ids(s, labels), 1.0
+    if ids is not None and ids.is_cuda:                                # on the host the lookup itself raises
+      labels = ids.clamp(0, min(s.shape[-1], t.shape[-1]) - 1)
+      sound = _refuse(labels != ids, "labels")
+    hard = softmax_cross_entropy(s, labels).mean() * sound
     with torch.no_grad():
-      teacher = softmax_cross_entropy(t, labels).mean()
+      teacher = softmax_cross_entropy(t, labels).mean() * sound
     loss = self.alpha * soft + (1.0 - self.alpha) * hard
     return loss, {"distill/soft_loss": soft.detach(), "distill/hard_loss": hard.detach(),
                   "distill/kl_div": kl.mean().detach(), "distill/teacher_loss": teacher}
