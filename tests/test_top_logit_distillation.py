@@ -339,3 +339,26 @@ def test_labels_outside_the_vocabulary_are_an_error(device, top_k, stored, label
   loss, m = strat.compute_loss(s, teacher, ids)
   assert math.isnan(float(loss.detach())) and math.isnan(float(m["distill/hard_loss"]))
   assert bool(torch.autograd.grad(loss, s)[0].isnan().any())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("k", [8, 280])
+@pytest.mark.parametrize("stored", [False, True])
+def test_a_teacher_of_more_tokens_than_the_student(device, k, stored):
+  """Fine as long as its list stays within the student's tokens; else an error, on the GPU a loss of NaN."""
+  s, t, ids = some_logits(4, 300, device)
+  wide = torch.cat([t, torch.full((4, 60), -50.0, device=device)], 1)
+  if stored and k > 256 and device == "cuda":
+    pytest.skip("lists of the GPU end at 256")
+  of = lambda z: functional.top_logprobs(z, k, ids) if stored else z   # noqa: E731
+  strat = strategy(temperature=2.0, alpha=0.6, distill_top_k=k)
+  loss, _ = strat.compute_loss(s, of(wide), ids)
+  want = rows64(s, wide, ids, k, 2.0, 0.6)
+  assert abs(float(loss) - float(want)) <= 64 * 16 * U * 5
+  wide[1, 310] = 60.0
+  if device == "cpu":
+    with pytest.raises(RuntimeError, match="out of bounds|outside"):
+      strat.compute_loss(s, of(wide), ids)
+  else:
+    loss, m = strat.compute_loss(s, of(wide), ids)
+    assert math.isnan(float(loss)) and math.isnan(float(m["distill/kl_div"]))

@@ -35,7 +35,8 @@ def _refuse(outside, what):
 
 
 class LogitStrategy(BaseStrategy):
-  """Integer labels outside the vocabulary raise on the CPU and make the loss NaN on the GPU, with and without a top-k."""
+  """Integer labels outside the vocabulary, and tokens among the teacher's top-k that the student does not have, raise on
+  the CPU and make the loss NaN on the GPU, whether the teacher's list is used or its logits."""
 
   def __init__(self, student_forward_fn, teacher_forward_fn, labels_fn, temperature: float = 2.0,
                alpha: float = 0.5, distill_top_k: int = 0):
@@ -63,13 +64,17 @@ class LogitStrategy(BaseStrategy):
         top = functional.top_logprobs(teacher_output.detach(), self.distill_top_k, ids)
         teacher = (-top.target.mean() if ids is not None else softmax_cross_entropy(teacher_output, labels).mean()) * sound
     k = min(top.ids.shape[-1], self.distill_top_k or V)
-    terms = functional.top_distill_loss(student_output, top.ids[..., :k], top.top.detach()[..., :k], ids, self.temperature,
-                                        twice=True)
-    soft = (terms.kl * self.temperature ** 2).mean()
+    listed = top.ids[..., :k]
+    within = 1.0
+    if stored or teacher_output.shape[-1] > V:                         # negative ids are absent entries
+      within = _refuse(listed >= V, "the teacher's tokens")
+    terms = functional.top_distill_loss(student_output, listed, top.top.detach()[..., :k], ids, self.temperature, twice=True)
+    kl = terms.kl * within
+    soft = (kl * self.temperature ** 2).mean()
     hard = (terms.nll.mean() if ids is not None else softmax_cross_entropy(student_output, labels).mean()) * sound
     loss = self.alpha * soft + (1.0 - self.alpha) * hard
     metrics = {"distill/soft_loss": soft.detach(), "distill/hard_loss": hard.detach(),
-               "distill/kl_div": terms.kl.mean().detach()}
+               "distill/kl_div": kl.mean().detach()}
     if teacher is not None:
       metrics["distill/teacher_loss"] = teacher.detach()
     return loss, metrics
@@ -97,14 +102,17 @@ class LogitStrategy(BaseStrategy):
     if isinstance(teacher_output, functional.TopLogprobs) or self._takes_list(student_output, teacher_output, labels):
       return self._compute_listed_loss(student_output, teacher_output, labels)
     s, t = student_output.float(), teacher_output.float()
-    sk, tk = s, t
+    sk, tk, within = s, t, 1.0
     if self.distill_top_k > 0:
       tk, idx = torch.topk(t, self.distill_top_k, dim=-1)
+      if idx.is_cuda and t.shape[-1] > s.shape[-1]:                    # on the host the lookup itself raises
+        within = _refuse(idx >= s.shape[-1], "the teacher's tokens")
+        idx = idx.clamp_max(s.shape[-1] - 1)
       sk = s.gather(-1, idx)
     log_ps = F.log_softmax(sk / self.temperature, dim=-1)
     log_pt = F.log_softmax(tk / self.temperature, dim=-1)
     pt = log_pt.exp()
-    kl = (pt * (torch.where(pt > 0, log_pt, torch.zeros_like(log_pt)) - log_ps)).sum(-1)
+    kl = (pt * (torch.where(pt > 0, log_pt, torch.zeros_like(log_pt)) - log_ps)).sum(-1) * within
     soft = (kl * self.temperature ** 2).mean()
     ids, sound = _class_ids(s, labels), 1.0
     if ids is not None and ids.is_cuda:                                # on the host the lookup itself raises
