@@ -362,3 +362,23 @@ def test_a_teacher_of_more_tokens_than_the_student(device, k, stored):
   else:
     loss, m = strat.compute_loss(s, of(wide), ids)
     assert math.isnan(float(loss)) and math.isnan(float(m["distill/kl_div"]))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_list_of_another_temperature_is_refused(device):
+  import copy
+  import pickle
+  from tunix_b200.sft.sharding_utils import shard_input
+  s, t, ids = some_logits(4, 300, device)
+  strat = strategy(temperature=2.0, alpha=0.6, distill_top_k=10)
+  warm = functional.top_logprobs(t, 12, ids, temperature=2.0)
+  for teacher in (warm, pickle.loads(pickle.dumps(warm)), copy.deepcopy(warm), warm._replace(entropy=None),
+                  shard_input(warm, device=device)):
+    assert teacher.temperature == 2.0 and len(teacher) == 4
+    with pytest.raises(ValueError, match="temperature"):
+      strat.compute_loss(s, teacher, ids)
+  kept = pickle.loads(pickle.dumps(functional.top_logprobs(t, 12, ids)))
+  by_hand = functional.TopLogprobs(kept.ids, kept.top, None, None)
+  for teacher in (kept, by_hand):
+    loss, _ = strat.compute_loss(s, teacher, ids)
+    assert abs(float(loss) - float(rows64(s, t, ids, 10, 2.0, 0.6))) <= 64 * 16 * U * 5

@@ -5,7 +5,7 @@
 With a top-k the GPU runs two operators instead of passes over [.., V] in fp32: `top_logprobs` makes the teacher's list
 (and its loss on integer labels) and `top_distill_loss` reads the student's logits once. A teacher's list may also stand
 in the place of its logits: a `teacher_forward_fn` that returns `ops.functional.TopLogprobs`, computed on the spot or
-stored earlier, keeps k numbers per token instead of V."""
+stored earlier at temperature 1, keeps k numbers per token instead of V."""
 from __future__ import annotations
 
 import math
@@ -58,6 +58,9 @@ class LogitStrategy(BaseStrategy):
       ids, sound = known, _refuse(known != ids, "labels")
     if stored:
       top = teacher_output
+      if top.temperature != 1.0:
+        raise ValueError(f"LogitStrategy: a teacher's list is taken to its temperature here and has to come at temperature "
+                         f"1, this one was made at {top.temperature}")
       teacher = None if top.target is None else -top.target.mean()
     else:
       with torch.no_grad():

@@ -435,12 +435,26 @@ def linear_logprob(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Te
 MIN_TEMPERATURE, MAX_TEMPERATURE = 1e-18, 1e18       # the inverse and products with logits stay within fp32
 
 
-class TopLogprobs(NamedTuple):
-  """What `top_logprobs` says of every row of logits."""
+class _TopLogprobs(NamedTuple):
   ids: torch.Tensor                    # int64 [..., k], likeliest first
   top: torch.Tensor                    # fp32 [..., k], their log-probabilities
   target: Optional[torch.Tensor]       # fp32 [...], log-probability of the given token
   entropy: Optional[torch.Tensor]      # fp32 [...]
+
+
+class TopLogprobs(_TopLogprobs):
+  """What `top_logprobs` says of every row of logits. `temperature`, at which it says so, is an attribute beside the four
+  fields: copies, pickles and `_replace` keep it, a tuple built anew from the fields is at temperature 1."""
+  temperature = 1.0
+
+  def __new__(cls, ids, top, target, entropy, temperature: float = 1.0):
+    self = super().__new__(cls, ids, top, target, entropy)
+    if temperature != 1.0:
+      self.temperature = float(temperature)
+    return self
+
+  def _replace(self, **fields):
+    return TopLogprobs(*super()._replace(**fields), temperature=self.temperature)
 
 
 class DistillLoss(NamedTuple):
@@ -580,7 +594,8 @@ def top_logprobs(logits: torch.Tensor, k: int, targets: Optional[torch.Tensor] =
       ids, top, target, ent = _TopLogprobsFn.apply(x2, k, tg, 1.0 / float(temperature), bool(want_entropy))
     else:
       ids, top, target, ent, _ = kernels.top_logprobs_fwd(x2, k, tg, 1.0 / float(temperature), bool(want_entropy))
-  return TopLogprobs(_lead(ids, *lead, k), _lead(top, *lead, k), _lead(target, *lead), _lead(ent, *lead))
+  return TopLogprobs(_lead(ids, *lead, k), _lead(top, *lead, k), _lead(target, *lead), _lead(ent, *lead),
+                     temperature)
 
 
 def top_distill_loss(logits: torch.Tensor, top_ids: torch.Tensor, top_values: torch.Tensor,

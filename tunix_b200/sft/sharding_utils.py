@@ -65,7 +65,7 @@ def shard_input(batch: Any, data_sharding_axis: Sequence[str] = ("fsdp",), devic
       return dataclasses.replace(x, **{f.name: rec(getattr(x, f.name)) for f in dataclasses.fields(x)})
     if isinstance(x, (list, tuple)) and not isinstance(x, str):
       t = [rec(v) for v in x]
-      return type(x)(t) if not hasattr(x, "_fields") else type(x)(*t)
+      return type(x)(t) if not hasattr(x, "_fields") else x._replace(**dict(zip(x._fields, t)))
     return _place(x, rank, size, device)
 
   return rec(batch)
