@@ -61,12 +61,15 @@ class LogitStrategy(BaseStrategy):
       if top.temperature != 1.0:
         raise ValueError(f"LogitStrategy: a teacher's list is taken to its temperature here and has to come at temperature "
                          f"1, this one was made at {top.temperature}")
+      if top.ids.shape[-1] < self.distill_top_k:
+        raise ValueError(f"LogitStrategy: the teacher's list has {top.ids.shape[-1]} entries, too few for a top-k of "
+                         f"{self.distill_top_k}")
       teacher = None if top.target is None else -top.target.mean()
     else:
       with torch.no_grad():
         top = functional.top_logprobs(teacher_output.detach(), self.distill_top_k, ids)
         teacher = (-top.target.mean() if ids is not None else softmax_cross_entropy(teacher_output, labels).mean()) * sound
-    k = min(top.ids.shape[-1], self.distill_top_k or V)
+    k = self.distill_top_k or top.ids.shape[-1]
     listed = top.ids[..., :k]
     within = 1.0
     if stored or teacher_output.shape[-1] > V:                         # negative ids are absent entries
