@@ -373,7 +373,7 @@ def test_a_list_of_another_temperature_is_refused(device):
   strat = strategy(temperature=2.0, alpha=0.6, distill_top_k=10)
   warm = functional.top_logprobs(t, 12, ids, temperature=2.0)
   for teacher in (warm, pickle.loads(pickle.dumps(warm)), copy.deepcopy(warm), warm._replace(entropy=None),
-                  shard_input(warm, device=device)):
+                  shard_input(warm, device=torch.device(device))):
     assert teacher.temperature == 2.0 and len(teacher) == 4
     with pytest.raises(ValueError, match="temperature"):
       strat.compute_loss(s, teacher, ids)
