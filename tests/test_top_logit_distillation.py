@@ -388,6 +388,6 @@ def test_a_list_of_another_temperature_is_refused(device):
 def test_a_list_shorter_than_the_top_k_is_refused(device):
   s, t, ids = some_logits(4, 300, device)
   for labels in (ids, F.one_hot(ids, 300).float()):
-    with pytest.raises(ValueError, match="4 entries .* top-k of 10"):
+    with pytest.raises(ValueError, match="4 entries.* top-k of 10"):
       strategy(distill_top_k=10).compute_loss(s, functional.top_logprobs(t, 4, ids), labels)
     strategy(distill_top_k=4).compute_loss(s, functional.top_logprobs(t, 4, ids), labels)
