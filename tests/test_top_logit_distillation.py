@@ -391,3 +391,21 @@ def test_a_list_shorter_than_the_top_k_is_refused(device):
     with pytest.raises(ValueError, match="4 entries.* top-k of 10"):
       strategy(distill_top_k=10).compute_loss(s, functional.top_logprobs(t, 4, ids), labels)
     strategy(distill_top_k=4).compute_loss(s, functional.top_logprobs(t, 4, ids), labels)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("one_hot", [False, True])
+def test_a_bf16_gradient_is_rounded_once(device, one_hot):
+  T, V, k, tau, alpha = 6, 700, 12, 2.0, 0.6
+  s, t, ids = some_logits(T, V, device)
+  s = s.to(bf16)
+  labels = F.one_hot(ids, V).float() if one_hot else ids
+  _, g_soft, g_hard, terms = (z[0] if z.ndim else z for z in loss64(s[None], t[None], ids[None], k, tau, alpha))
+  # 1024 U of a term before the one rounding, half a step of 2^-7 of the value
+  off = 1024 * U * terms
+  for teacher in (t, functional.top_logprobs(t, k, ids)):
+    leaf = s.clone().requires_grad_()
+    loss, _ = strategy(temperature=tau, alpha=alpha, distill_top_k=k).compute_loss(leaf, teacher, labels)
+    grad, = torch.autograd.grad(loss, leaf)
+    near = (grad.to(f64) - (g_soft + g_hard)).abs() - off - 2.0 ** -8 * ((g_soft + g_hard).abs() + off)
+    assert float(near.max()) <= 0

@@ -70,6 +70,8 @@ class LogitStrategy(BaseStrategy):
         top = functional.top_logprobs(teacher_output.detach(), self.distill_top_k, ids)
         teacher = (-top.target.mean() if ids is not None else softmax_cross_entropy(teacher_output, labels).mean()) * sound
     k = self.distill_top_k or top.ids.shape[-1]
+    if ids is None:                                                    # two gradients: they meet in fp32 and are rounded once
+      student_output = student_output.float()
     listed = top.ids[..., :k]
     within = 1.0
     if stored or teacher_output.shape[-1] > V:                         # negative ids are absent entries
