@@ -221,3 +221,15 @@ def test_tables_and_batches_beyond_32_bits(kernel_lib):
   kernels.embedding_bwd(ids, dout, grad)
   assert torch.equal(grad[6], dout[-2].float() + dout[-1].float())
   assert float((grad[3] - T / 1000).abs().max()) == 0.0                  # 600 ones: exact in fp32
+
+
+def test_more_tokens_than_the_gradient_counts_are_refused(kernel_lib):
+  """The sort's indices run past the last token by up to a tile: the limit leaves room for that. Nothing is allocated."""
+  from tunix_b200.ops import kernels
+  for T in (0x7fff0001, 2 ** 31 - 1, 2 ** 31):
+    ids = torch.zeros(1, dtype=torch.long).expand(T)
+    dout = torch.zeros(1, 8, dtype=bf16).expand(T, 8)
+    with pytest.raises(ValueError, match="31 bits"):
+      kernels.embedding_bwd(ids, dout, torch.zeros(4, 8))
+  for T in (0x7fff0001, 2 ** 31 - 1):
+    assert kernel_lib.tx_embedding_grad(None, 1, None, None, 0, T, 8, 4, 1.0, None, None) == 1

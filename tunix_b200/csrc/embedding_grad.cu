@@ -29,6 +29,7 @@ namespace cg = cooperative_groups;
 
 namespace {
 
+constexpr int kMaxTokens = 0x7fff0000;        // indices run past the last token by a tile of the sort at most
 constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kMaxDigits = 1024;              // 10 bits a pass
@@ -457,11 +458,11 @@ extern "C" long long tx_embedding_grad_workspace(int T, int D) {
   return 2 * ((8ll * T + 15) / 16 * 16) + (8 * chunks + 15) / 16 * 16 + 16 + 2 * chunks * D * 4;
 }
 
-// ids int64 or int32 [T], dout bf16 [T, D] with D a multiple of 8. grad_bf16 == 0: grad is fp32 and added to; else it
+// ids int64 or int32 [T], T at most kMaxTokens, dout bf16 [T, D] with D a multiple of 8. grad_bf16 == 0: grad is fp32 and added to; else it
 // is bf16 and written whole.
 extern "C" int tx_embedding_grad(const void* ids, int ids64, const void* dout, void* grad, int grad_bf16, int T, int D,
                                  int V, float scale, void* workspace, cudaStream_t s) {
-  if (D % 8 || D <= 0 || V <= 0 || V > 0x3fffffff) return 1;
+  if (D % 8 || D <= 0 || V <= 0 || V > 0x3fffffff || T > kMaxTokens) return 1;
   if (T <= 0) return grad_bf16 && cudaMemsetAsync(grad, 0, 2ll * V * D, s) != cudaSuccess ? 403 : 0;
   const long long chunks = (T + chunk_of(T) - 1) / chunk_of(T);
   int2* a = static_cast<int2*>(workspace);

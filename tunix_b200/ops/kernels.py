@@ -170,14 +170,19 @@ def embedding_fwd(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) ->
   return out
 
 
+MAX_TOKENS = 0x7fff0000   # of one embedding gradient (csrc/embedding_grad.cu: kMaxTokens)
+
+
 def embedding_bwd(ids: torch.Tensor, dout: torch.Tensor, grad_table: torch.Tensor, scale: float = 1.0) -> None:
   """Sums scale * dout [T, D] (bf16) over the positions of every id, in a fixed order. grad_table [V, D] fp32 is added
   to; a bf16 one is written whole, rows that do not occur are zero. Ids outside the vocabulary are left out."""
-  ids = _flat_ids(ids)
   T = ids.numel()
+  if T > MAX_TOKENS:
+    raise ValueError(f"embedding: the gradient's tokens are counted in 31 bits, got {T}")
+  ids = _flat_ids(ids)
   V, D = grad_table.shape
   assert dout.dtype == bf16 and dout.is_contiguous() and dout.numel() == T * D and grad_table.is_contiguous()
-  assert grad_table.dtype in (bf16, torch.float32) and T < 2 ** 31 and ids.is_cuda
+  assert grad_table.dtype in (bf16, torch.float32) and ids.is_cuda
   if dout.data_ptr() % 16:
     dout = dout.clone()
   lib = _lib.require()
