@@ -233,3 +233,19 @@ def test_more_tokens_than_the_gradient_counts_are_refused(kernel_lib):
       kernels.embedding_bwd(ids, dout, torch.zeros(4, 8))
   for T in (0x7fff0001, 2 ** 31 - 1):
     assert kernel_lib.tx_embedding_grad(None, 1, None, None, 0, T, 8, 4, 1.0, None, None) == 1
+
+
+@pytest.mark.gpu
+def test_ids_outside_a_table_that_the_kernels_do_not_take(kernel_lib):
+  """As with the kernels: the nearest row is read and gets no gradient."""
+  wide = torch.randn(30, 48, device="cuda").to(bf16)
+  flat = torch.randn(30 * 32 + 1, device="cuda").to(bf16)
+  ids = torch.tensor([-1, 0, 29, 30, 2 ** 40, 5], device="cuda")
+  dout = torch.randn(6, 32, device="cuda").to(bf16)
+  for table in (wide[:, :32], flat[1:].view(30, 32)):
+    taken = table.detach().clone(memory_format=torch.contiguous_format).requires_grad_()
+    leaf = table.detach().requires_grad_()
+    a, b = F.embedding(ids, leaf, 2.0), F.embedding(ids, taken, 2.0)
+    assert torch.equal(a, b)
+    ga, gb = torch.autograd.grad(a, leaf, dout)[0], torch.autograd.grad(b, taken, dout)[0]
+    assert torch.equal(ga, gb) and bool((ga[0] == gb[0]).all())

@@ -301,7 +301,12 @@ class _EmbeddingFn(torch.autograd.Function):
 def embedding(ids: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
   """Rows of `table` [V, D] times `scale`. The table's gradient is summed by sorted tokens: repeatable to the bit,
   fp32 sums rounded once, straight into `main_grad` where the table has one."""
-  if _use_kernels(table) and table.shape[1] % 8 == 0 and table.is_contiguous() and table.data_ptr() % 16 == 0:
+  if _use_kernels(table) and table.shape[1] % 8 == 0:
+    if not table.is_contiguous() or table.data_ptr() % 16:
+      # the plain statement, with the kernels' rule for ids outside the table: the nearest row, which gets no gradient
+      known = ids.clamp(0, table.shape[0] - 1)
+      rows = ref.embedding(known, table, scale)
+      return torch.where((known == ids)[..., None], rows, rows.detach())
     home = _lib.bind_thread()
     if ids.get_device() != home or table.get_device() != home:
       raise ValueError(f"embedding: ids are on {ids.device}, the table on {table.device}, "
