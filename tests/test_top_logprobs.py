@@ -631,3 +631,25 @@ def test_gradients_at_extreme_temperatures(device, tau):
   x[1, 2000:2100] = -1e4
   check_score(x, 5, torch.full((3,), 77, device=device), tau, eps(x.dtype))
   check_score(x, 5, torch.full((3,), 2000, device=device), tau, eps(x.dtype))
+
+
+@pytest.mark.gpu
+def test_row_statistics_belong_to_the_graph():
+  """What the backward pass reads is saved with the graph: seen by saved-tensor hooks and freed with it."""
+  import weakref
+  x = make_logits(3, 50, torch.float32, "cuda").requires_grad_()
+  ids, values = make_list(x, 4)
+  for call in (lambda: F.top_logprobs(x, 4).top, lambda: F.top_distill_loss(x, ids, values, normalize="full").kl):
+    seen = []
+
+    def pack(t):
+      seen.append((tuple(t.shape), weakref.ref(t)))
+      return t
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+      out = call()
+    stats = [r for shape, r in seen if shape in ((3, 2), (3, 8))]
+    assert len(stats) == 1
+    out.sum().backward()
+    del out
+    assert stats[0]() is None

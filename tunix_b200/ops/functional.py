@@ -487,8 +487,8 @@ class _TopLogprobsFn(torch.autograd.Function):
 
   @staticmethod
   def forward(ctx, x2, k, targets, inv_temp, want_entropy):
-    ids, top, target, ent, ctx.stats = kernels.top_logprobs_fwd(x2, k, targets, inv_temp, want_entropy)
-    ctx.save_for_backward(x2, ids, targets, ent)
+    ids, top, target, ent, stats = kernels.top_logprobs_fwd(x2, k, targets, inv_temp, want_entropy)
+    ctx.save_for_backward(x2, ids, targets, ent, stats)
     ctx.inv_temp = inv_temp
     ctx.mark_non_differentiable(ids)
     ctx.set_materialize_grads(False)
@@ -496,10 +496,10 @@ class _TopLogprobsFn(torch.autograd.Function):
 
   @staticmethod
   def backward(ctx, _, g_top, g_target, g_ent):
-    x2, ids, targets, ent = ctx.saved_tensors
+    x2, ids, targets, ent, stats = ctx.saved_tensors
     if g_top is None and g_target is None and g_ent is None:
       return None, None, None, None, None
-    dx = kernels.top_logprobs_bwd(x2, ids, targets, ctx.stats, ent, _grad32(g_top), _grad32(g_target), _grad32(g_ent),
+    dx = kernels.top_logprobs_bwd(x2, ids, targets, stats, ent, _grad32(g_top), _grad32(g_target), _grad32(g_ent),
                                   ctx.inv_temp)
     return _once(dx), None, None, None, None
 
@@ -508,15 +508,15 @@ class _TopDistillFn(torch.autograd.Function):
 
   @staticmethod
   def forward(ctx, x2, ids, values, labels, inv_temp, full, temperature):
-    kl, nll, ctx.stats = kernels.top_distill_fwd(x2, ids, values, labels, inv_temp, full)
-    ctx.save_for_backward(x2, ids, values, labels)
+    kl, nll, stats = kernels.top_distill_fwd(x2, ids, values, labels, inv_temp, full)
+    ctx.save_for_backward(x2, ids, values, labels, stats)
     ctx.cfg, ctx.again = (inv_temp, full), temperature
     ctx.set_materialize_grads(False)
     return kl, nll
 
   @staticmethod
   def backward(ctx, g_kl, g_nll):
-    x2, ids, values, labels = ctx.saved_tensors
+    x2, ids, values, labels, stats = ctx.saved_tensors
     rest = (None,) * 6
     if g_kl is None and g_nll is None:
       return None, *rest
@@ -524,7 +524,7 @@ class _TopDistillFn(torch.autograd.Function):
       outs = ref.top_distill_loss(x2, ids, values, labels, ctx.again, ctx.cfg[1])
       pairs = [(o, g) for o, g in zip(outs, (g_kl, g_nll)) if g is not None]
       return torch.autograd.grad([o for o, _ in pairs], x2, [g for _, g in pairs], create_graph=True)[0], *rest
-    dx = kernels.top_distill_bwd(x2, ids, values, labels, ctx.stats, _grad32(g_kl), _grad32(g_nll), *ctx.cfg)
+    dx = kernels.top_distill_bwd(x2, ids, values, labels, stats, _grad32(g_kl), _grad32(g_nll), *ctx.cfg)
     return _once(dx), *rest
 
 
