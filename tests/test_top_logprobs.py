@@ -653,3 +653,25 @@ def test_row_statistics_belong_to_the_graph():
     out.sum().backward()
     del out
     assert stats[0]() is None
+
+
+@pytest.mark.gpu
+def test_both_exponentials_over_their_range():
+  """With two temperatures a part of a row's exponentials is made by multiply-adds: one element of every such place and
+  of every size, against 64 bits."""
+  d = torch.cat([torch.linspace(0, 18, 6000), torch.linspace(18, 90, 1000)])
+  d = torch.cat([-d, torch.full((1,), LOW)]).to(torch.bfloat16)
+  T = d.numel()
+  for place in range(1, 16):
+    x = torch.full((T, 16), LOW, dtype=torch.bfloat16)
+    x[:, 0] = 0.0
+    x[:, place] = d
+    x = x.cuda()
+    ids, values = torch.zeros(T, 1, dtype=torch.long, device="cuda"), torch.zeros(T, 1, device="cuda")
+    got = F.top_distill_loss(x, ids, values, torch.zeros(T, dtype=torch.long, device="cuda"), temperature=2.0, normalize="full")
+    w2, w1 = torch.exp(d.to(f64).cuda() / 2), torch.exp(d.to(f64).cuda())
+    # ln(1 + w): w off by 2^-22 of itself and by the rounding of its exponent (at most 2^7 in size, 2^-24 of that by
+    # the scale and again by the product), the sum by U, the logarithm by 2 U of a number below 1
+    for value, w in ((got.kl, w2), (got.nll, w1)):
+      tol = w * (2.0 ** -22 + 2 * U * d.to(f64).cuda().abs().clamp_max(100.0)) + 4 * U
+      assert float(((value.to(f64) - torch.log1p(w)).abs() - tol).max()) <= 0
