@@ -322,8 +322,10 @@ def test_second_derivatives_through_the_strategy(device):
 @pytest.mark.parametrize("stored", [False, True])
 @pytest.mark.parametrize("label", [-100, 300])
 def test_labels_outside_the_vocabulary_are_an_error(device, top_k, stored, label):
-  """On the host they raise; on the GPU, where the host would have to wait for the labels, the loss and its gradient are
-  NaN. The same with and without a list."""
+  """On the host they raise, with and without a list; on the GPU the loss and its gradient are NaN with a list (without
+  one the lookup's own assertion is the error, which no test may set off)."""
+  if device == "cuda" and not stored and top_k == 0:
+    pytest.skip("an assertion on the device")
   s, t, ids = some_logits(4, 300, device)
   s = s.requires_grad_()
   teacher = functional.top_logprobs(t, 8, ids) if stored else t
@@ -345,7 +347,7 @@ def test_labels_outside_the_vocabulary_are_an_error(device, top_k, stored, label
 @pytest.mark.parametrize("k", [8, 280])
 @pytest.mark.parametrize("stored", [False, True])
 def test_a_teacher_of_more_tokens_than_the_student(device, k, stored):
-  """Fine as long as its list stays within the student's tokens; else an error, on the GPU a loss of NaN."""
+  """Fine as long as its list stays within the student's tokens; else an error, on the GPU a loss of NaN with a list."""
   s, t, ids = some_logits(4, 300, device)
   wide = torch.cat([t, torch.full((4, 60), -50.0, device=device)], 1)
   if stored and k > 256 and device == "cuda":
@@ -355,6 +357,8 @@ def test_a_teacher_of_more_tokens_than_the_student(device, k, stored):
   loss, _ = strat.compute_loss(s, of(wide), ids)
   want = rows64(s, wide, ids, k, 2.0, 0.6)
   assert abs(float(loss) - float(want)) <= 64 * 16 * U * 5
+  if k > 256 and device == "cuda":
+    return                                                          # without a list: the lookup's assertion on the device
   wide[1, 310] = 60.0
   if device == "cpu":
     with pytest.raises(RuntimeError, match="out of bounds|outside"):

@@ -25,18 +25,23 @@ def _class_ids(logits, labels):
 
 
 def _refuse(outside, what):
-  """Ids outside the vocabulary are an error: on the host it is raised. On the GPU, where the host would have to wait to
-  see them, the answer is a factor for the loss, 1 or, where there are some, NaN."""
+  """Ids outside the vocabulary are an error, as in a lookup: on the host it is raised. On the GPU a lookup's assertion
+  ends the process; here the answer is a factor for the loss instead, 1 or, where there are some, NaN."""
   if outside.is_cuda:
     return torch.where(outside.any(), math.nan, 1.0)
   if bool(outside.any()):
     raise RuntimeError(f"LogitStrategy: {what} outside the vocabulary")
-  return 1.0
+  return None
+
+
+def _times(x, factor):
+  return x if factor is None else x * factor
 
 
 class LogitStrategy(BaseStrategy):
-  """Integer labels outside the vocabulary, and tokens among the teacher's top-k that the student does not have, raise on
-  the CPU and make the loss NaN on the GPU, whether the teacher's list is used or its logits."""
+  """Integer labels outside the vocabulary, and tokens among the teacher's top-k that the student does not have, are an
+  error: raised on the CPU; on the GPU, where the host does not see them, the loss and its gradient are NaN with a
+  teacher's list, and the lookup in torch asserts on the device where the formulas run."""
 
   def __init__(self, student_forward_fn, teacher_forward_fn, labels_fn, temperature: float = 2.0,
                alpha: float = 0.5, distill_top_k: int = 0):
@@ -52,7 +57,7 @@ class LogitStrategy(BaseStrategy):
 
   def _compute_listed_loss(self, student_output, teacher_output, labels):
     V, stored = student_output.shape[-1], isinstance(teacher_output, functional.TopLogprobs)
-    ids, sound = _class_ids(student_output, labels), 1.0
+    ids, sound = _class_ids(student_output, labels), None
     if ids is not None:
       known = ids.clamp(0, (V if stored else min(V, teacher_output.shape[-1])) - 1)
       ids, sound = known, _refuse(known != ids, "labels")
@@ -68,23 +73,23 @@ class LogitStrategy(BaseStrategy):
     else:
       with torch.no_grad():
         top = functional.top_logprobs(teacher_output.detach(), self.distill_top_k, ids)
-        teacher = (-top.target.mean() if ids is not None else softmax_cross_entropy(teacher_output, labels).mean()) * sound
+        teacher = -top.target.mean() if ids is not None else softmax_cross_entropy(teacher_output, labels).mean()
     k = self.distill_top_k or top.ids.shape[-1]
     if ids is None:                                                    # two gradients: they meet in fp32 and are rounded once
       student_output = student_output.float()
     listed = top.ids[..., :k]
-    within = 1.0
+    within = None
     if stored or teacher_output.shape[-1] > V:                         # negative ids are absent entries
       within = _refuse(listed >= V, "the teacher's tokens")
     terms = functional.top_distill_loss(student_output, listed, top.top.detach()[..., :k], ids, self.temperature, twice=True)
-    kl = terms.kl * within
+    kl = _times(terms.kl, within)
     soft = (kl * self.temperature ** 2).mean()
-    hard = (terms.nll.mean() if ids is not None else softmax_cross_entropy(student_output, labels).mean()) * sound
+    hard = _times(terms.nll.mean() if ids is not None else softmax_cross_entropy(student_output, labels).mean(), sound)
     loss = self.alpha * soft + (1.0 - self.alpha) * hard
     metrics = {"distill/soft_loss": soft.detach(), "distill/hard_loss": hard.detach(),
                "distill/kl_div": kl.mean().detach()}
     if teacher is not None:
-      metrics["distill/teacher_loss"] = teacher.detach()
+      metrics["distill/teacher_loss"] = _times(teacher.detach(), sound)
     return loss, metrics
 
   def _takes_list(self, student_output, teacher_output, labels) -> bool:
@@ -110,25 +115,18 @@ class LogitStrategy(BaseStrategy):
     if isinstance(teacher_output, functional.TopLogprobs) or self._takes_list(student_output, teacher_output, labels):
       return self._compute_listed_loss(student_output, teacher_output, labels)
     s, t = student_output.float(), teacher_output.float()
-    sk, tk, within = s, t, 1.0
+    sk, tk = s, t
     if self.distill_top_k > 0:
       tk, idx = torch.topk(t, self.distill_top_k, dim=-1)
-      if idx.is_cuda and t.shape[-1] > s.shape[-1]:                    # on the host the lookup itself raises
-        within = _refuse(idx >= s.shape[-1], "the teacher's tokens")
-        idx = idx.clamp_max(s.shape[-1] - 1)
       sk = s.gather(-1, idx)
     log_ps = F.log_softmax(sk / self.temperature, dim=-1)
     log_pt = F.log_softmax(tk / self.temperature, dim=-1)
     pt = log_pt.exp()
-    kl = (pt * (torch.where(pt > 0, log_pt, torch.zeros_like(log_pt)) - log_ps)).sum(-1) * within
+    kl = (pt * (torch.where(pt > 0, log_pt, torch.zeros_like(log_pt)) - log_ps)).sum(-1)
     soft = (kl * self.temperature ** 2).mean()
-    ids, sound = _class_ids(s, labels), 1.0
-    if ids is not None and ids.is_cuda:                                # on the host the lookup itself raises
-      labels = ids.clamp(0, min(s.shape[-1], t.shape[-1]) - 1)
-      sound = _refuse(labels != ids, "labels")
-    hard = softmax_cross_entropy(s, labels).mean() * sound
+    hard = softmax_cross_entropy(s, labels).mean()
     with torch.no_grad():
-      teacher = softmax_cross_entropy(t, labels).mean() * sound
+      teacher = softmax_cross_entropy(t, labels).mean()
     loss = self.alpha * soft + (1.0 - self.alpha) * hard
     return loss, {"distill/soft_loss": soft.detach(), "distill/hard_loss": hard.detach(),
                   "distill/kl_div": kl.mean().detach(), "distill/teacher_loss": teacher}
