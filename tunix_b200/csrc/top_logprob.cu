@@ -1105,8 +1105,7 @@ struct BwdArgs {
   const float* g_entropy;      // [T] or null
   const float* entropy;        // [T] when g_entropy
   const float* stats;          // [T, 2] (score: m, ln s) or [T, kDistillStats]
-  void* dx;
-  long long ldd;
+  void* dx;                    // [T, V], dense
   int blocks;                  // a row's columns are cut into this many parts
   int one;                     // both softmaxes are the same: their factors are added
 };
@@ -1130,7 +1129,7 @@ __global__ void __launch_bounds__(kThreads) top_bwd_kernel(BwdArgs a) {
   const int2 part = part_of(a.V, blockIdx.x - row * a.blocks, a.blocks);
   const int lo = part.x, hi = part.y;
   const LT* x = static_cast<const LT*>(a.logits) + static_cast<long long>(row) * a.ld;
-  LT* dx = static_cast<LT*>(a.dx) + static_cast<long long>(row) * a.ldd;
+  LT* dx = static_cast<LT*>(a.dx) + static_cast<long long>(row) * a.V;
   const int V = a.V, k = a.k, mode = a.mode;
   const int from = lo - misalign(dx + lo);
   const bool aligned = misalign(x + lo) == misalign(dx + lo);
@@ -1345,7 +1344,7 @@ int launch_bwd(BwdArgs a, int dense, cudaStream_t s) {
   a.blocks = max((a.V + kBwdPart - 1) / kBwdPart, min(most, (want + a.T - 1) / a.T));
   if (dense == 0) {
     a.blocks = 1;
-    const long long bytes = a.T * a.ldd * static_cast<long long>(sizeof(LT)), tile = 16 * kClearThreads * kClearVecs;
+    const long long bytes = static_cast<long long>(a.T) * a.V * static_cast<long long>(sizeof(LT)), tile = 16 * kClearThreads * kClearVecs;
     clear_kernel<<<static_cast<unsigned>((bytes + tile - 1) / tile), kClearThreads, 0, s>>>(
         static_cast<unsigned char*>(a.dx), bytes);
   }
@@ -1407,7 +1406,7 @@ extern "C" int tx_top_logprob_bwd(const void* logits, int logits_fp32, long long
   if (T <= 0) return 0;
   if (V < 1 || k < 1 || k > kMaxTop || V > 0x7fff0000) return 1;
   const BwdArgs a{logits, ld, T, V, k, kScore, inv_temp, ids, g_top, targets, nullptr, g_target, g_entropy, entropy,
-                  stats, dx, V, 1, 0};
+                  stats, dx, 1, 0};
   const int dense = g_entropy ? 5 : 1;
   return logits_fp32 ? launch_bwd<float>(a, dense, s) : launch_bwd<__nv_bfloat16>(a, dense, s);
 }
@@ -1421,7 +1420,7 @@ extern "C" int tx_top_distill_bwd(const void* logits, int logits_fp32, long long
   if (V < 1 || k < 1 || k > kMaxList || V > 0x7fff0000) return 1;
   const int both = full && g_kl && g_nll && inv_temp == 1.f;
   const BwdArgs a{logits, ld, T, V, k, full ? kFull : kListed, inv_temp, ids, values, labels, g_kl, g_nll, nullptr,
-                  nullptr, stats, dx, V, 1, both};
+                  nullptr, stats, dx, 1, both};
   const int dense = (full && g_kl ? 1 : 0) | (g_nll && !both ? 2 : 0);
   return logits_fp32 ? launch_bwd<float>(a, dense, s) : launch_bwd<__nv_bfloat16>(a, dense, s);
 }
