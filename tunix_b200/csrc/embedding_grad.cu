@@ -1,5 +1,6 @@
 // Gradient of an embedding table, summed by sorted tokens: grad[v, :] (+)= scale * sum over the positions t with
-// ids[t] == v of dout[t, :], every sum in fp32, in one fixed order and without atomics.
+// ids[t] == v of dout[t, :], every sum in fp32 and in one fixed order. Atomics (a reduction into the fp32 buffer, places in
+// the list of long runs) only where their order cannot matter: each element gets one addition.
 //
 // Launches. (1) The pairs (id, position) are sorted by id, equal ids by position. Few tokens: every pair counts the
 // pairs before it. More: one cluster, a radix sort from the low digit up whose per-warp digit counts live in shared
@@ -15,7 +16,8 @@
 // and 5 us more in the two cases below, 1 us of 7 for 512 tokens). Fetching a part of dout into L2 while the ids are
 // sorted gained nothing.
 //
-// 16384 tokens x 4096 into an fp32 buffer: 96 us (134 MB of dout and 115 MB of rows read and written: 3.8 TB/s).
+// 16384 tokens x 4096 into an fp32 buffer: 96 us (134 MB of dout and 115 MB of rows read and written: 3.8 TB/s; latency of
+// the sums, whose next rows are asked for when the last ones have come).
 // 65536 x 1152, half of them one id, new table of 262144 rows: 145 us, of which 82 us write the table (604 MB).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>

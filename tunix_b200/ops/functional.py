@@ -580,7 +580,7 @@ def top_logprobs(logits: torch.Tensor, k: int, targets: Optional[torch.Tensor] =
   Tokens of equal logits come by the lowest id, a NaN counts as the largest logit. A target outside the vocabulary
   is ignored (0, no gradient). Logits of -inf are masked out; a row that has nothing else gets log-probabilities of
   -inf, entropy 0 and no gradient. fp32 and bf16 logits on the GPU, rows of any alignment and stride, take one
-  kernel in each direction; there `k` is at most 256."""
+  kernel in each direction; there `k` is at most 256, and a logit tensor with a tangent of forward mode is refused."""
   _check_rows("top_logprobs", logits, temperature)
   V, lead = logits.shape[-1], logits.shape[:-1]
   if targets is not None:
@@ -620,7 +620,8 @@ def top_distill_loss(logits: torch.Tensor, top_ids: torch.Tensor, top_values: to
   -inf, student's logits there all -inf) has divergence 0 and no gradient, a row of -inf also no cross entropy.
   With `twice` a backward pass that builds a graph takes the plain statement, whose gradient can be differentiated
   again; without it such a gradient leads to an error.
-  fp32 and bf16 logits on the GPU take one kernel in each direction; there the list has at most 1024 entries."""
+  fp32 and bf16 logits on the GPU take one kernel in each direction (a list without labels two for its gradient); there
+  the list has at most 1024 entries and a tangent of forward mode is refused."""
   _check_rows("top_distill_loss", logits, temperature)
   V, lead = logits.shape[-1], logits.shape[:-1]
   k = top_ids.shape[-1] if top_ids.dim() else 0
