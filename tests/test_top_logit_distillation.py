@@ -413,3 +413,37 @@ def test_a_bf16_gradient_is_rounded_once(device, one_hot):
     grad, = torch.autograd.grad(loss, leaf)
     near = (grad.to(f64) - (g_soft + g_hard)).abs() - off - 2.0 ** -8 * ((g_soft + g_hard).abs() + off)
     assert float(near.max()) <= 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("stored", [False, True])
+def test_captured_strategy_step(stored):
+  """A loss with its gradient replays on new inputs, labels outside the vocabulary among them."""
+  T, V, k = 40, 500, 8
+  strat = strategy(temperature=2.0, alpha=0.6, distill_top_k=k)
+  inputs = [list(some_logits(T, V, "cuda", seed)) for seed in (0, 1)]
+  bad = [x.clone() for x in inputs[1]]
+  bad[2][3] = V
+
+  def run(s, t, ids):
+    leaf = s.detach().requires_grad_()
+    loss, _ = strat.compute_loss(leaf, functional.top_logprobs(t, k, ids) if stored else t, ids)
+    return loss.detach(), torch.autograd.grad(loss, leaf)[0]
+
+  static = [x.clone() for x in inputs[0]]
+  side = torch.cuda.Stream()
+  side.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(side):
+    for _ in range(2):
+      run(*static)
+  torch.cuda.current_stream().wait_stream(side)
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    captured = run(*static)
+  for case in (inputs[1], bad, inputs[0]):
+    for dst, src in zip(static, case):
+      dst.copy_(src)
+    graph.replay()
+    want = run(*case)
+    assert all(torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) for a, b in zip(captured, want))
+    assert bool(captured[0].isnan()) == (case is bad)

@@ -1,6 +1,6 @@
 // Gradient of an embedding table, summed by sorted tokens: grad[v, :] (+)= scale * sum over the positions t with
-// ids[t] == v of dout[t, :], every sum in fp32 and in one fixed order. Atomics (a reduction into the fp32 buffer, places in
-// the list of long runs) only where their order cannot matter: each element gets one addition.
+// ids[t] == v of dout[t, :], every sum in fp32 and in one fixed order. Atomics (a reduction into the fp32 buffer, places
+// in the list of long runs) only where their order cannot matter: each element gets one addition.
 //
 // Launches. (1) The pairs (id, position) are sorted by id, equal ids by position. Few tokens: every pair counts the
 // pairs before it. More: one cluster, a radix sort from the low digit up whose per-warp digit counts live in shared
@@ -16,8 +16,8 @@
 // and 5 us more in the two cases below, 1 us of 7 for 512 tokens). Fetching a part of dout into L2 while the ids are
 // sorted gained nothing.
 //
-// 16384 tokens x 4096 into an fp32 buffer: 96 us (134 MB of dout and 115 MB of rows read and written: 3.8 TB/s; latency of
-// the sums, whose next rows are asked for when the last ones have come).
+// 16384 tokens x 4096 into an fp32 buffer: 96 us (134 MB of dout and 115 MB of rows read and written: 3.8 TB/s; latency
+// of the sums, whose next rows are asked for when the last ones have come).
 // 65536 x 1152, half of them one id, new table of 262144 rows: 145 us, of which 82 us write the table (604 MB).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -460,8 +460,8 @@ extern "C" long long tx_embedding_grad_workspace(int T, int D) {
   return 2 * ((8ll * T + 15) / 16 * 16) + (8 * chunks + 15) / 16 * 16 + 16 + 2 * chunks * D * 4;
 }
 
-// ids int64 or int32 [T], T at most kMaxTokens, dout bf16 [T, D] with D a multiple of 8. grad_bf16 == 0: grad is fp32 and added to; else it
-// is bf16 and written whole.
+// ids int64 or int32 [T], T at most kMaxTokens, dout bf16 [T, D] with D a multiple of 8. grad_bf16 == 0: grad is fp32
+// and added to; else it is bf16 and written whole.
 extern "C" int tx_embedding_grad(const void* ids, int ids64, const void* dout, void* grad, int grad_bf16, int T, int D,
                                  int V, float scale, void* workspace, cudaStream_t s) {
   if (D % 8 || D <= 0 || V <= 0 || V > 0x3fffffff || T > kMaxTokens) return 1;

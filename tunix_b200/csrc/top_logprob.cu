@@ -1344,7 +1344,7 @@ int launch_bwd(BwdArgs a, int dense, cudaStream_t s) {
   a.blocks = max((a.V + kBwdPart - 1) / kBwdPart, min(most, (want + a.T - 1) / a.T));
   if (dense == 0) {
     a.blocks = 1;
-    const long long bytes = static_cast<long long>(a.T) * a.V * static_cast<long long>(sizeof(LT)), tile = 16 * kClearThreads * kClearVecs;
+    const long long bytes = static_cast<long long>(sizeof(LT)) * a.T * a.V, tile = 16 * kClearThreads * kClearVecs;
     clear_kernel<<<static_cast<unsigned>((bytes + tile - 1) / tile), kClearThreads, 0, s>>>(
         static_cast<unsigned char*>(a.dx), bytes);
   }
